@@ -12,6 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libfuelq.so")
 
 OK, MISALIGNED, INVALID_PROBLEM, NOT_SUPPORTED, WORKSPACE, LAUNCH_FAILURE = range(6)
+DEVICE_ERROR_INDEX = 7
 NUMERICS_INTEGER, NUMERICS_BF16, NUMERICS_TF32, NUMERICS_F16 = range(4)
 OPT_PDL, OPT_DECODE_MAX_M, OPT_DECODE_GRID, OPT_DECODE_KERNEL, OPT_L2_PREFETCH, OPT_FUSED_QUANT, OPT_PEER_WAIT_MS, OPT_PREFILL_TF32, OPT_PREFILL_BF16, OPT_PREFILL_ONE_KERNEL = 1, 2, 3, 4, 5, 6, 7, 8, 9, 10
 
@@ -107,6 +108,14 @@ PROTOTYPES = {
     "fuelq_argmax_last_peer": (_i32, [_vp, _i64, _vp, _pp, _i32, _vp, _vp]),
     "fuelq_swiglu": (_i32, [_vp, _vp, _vp, _i64, _vp]),
     "fuelq_argmax_last": (_i32, [_vp, _i64, _vp, _vp]),
+    "fuelq_paged_append": (_i32, [_i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
+                                  _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "fuelq_paged_attn_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
+    "fuelq_paged_attn_decode": (_i32, [_i32, _i32, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                                       ctypes.c_float, _vp, _sz, _vp]),
+    "fuelq_prompt_attn_workspace_bytes": (_sz, [_i32, _i64, _i32, _i32, _i32]),
+    "fuelq_prompt_attn": (_i32, [_i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _i32, _i32, _i32, ctypes.c_float,
+                                 _vp, _sz, _vp]),
     # include/fuelq_host.h
     "fuelq_last_error": (ctypes.c_char_p, []),
     "fuelq_qtensor_load": (_i32, [_i32, _vp, _i32, _i64, _i64, _vp, _sz, ctypes.POINTER(_vp)]),

@@ -1,0 +1,160 @@
+// C ABI of the paged-cache and prompt attention (include/fuelq.h, "Attention for batches of sequences"), in a translation unit
+// of its own beside fuelq.cu.
+#include "../../include/fuelq.h"
+
+#include "attn.cuh"
+#include "launch.cuh"
+
+#include <type_traits>
+
+namespace fq {
+namespace {
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline int type_bytes(int t) { return t == kF32 ? 4 : t == kF16 || t == kBF16 ? 2 : 0; }
+inline bool type_pair(int act, int cache) { return type_bytes(act) && type_bytes(cache) && (act == kF32 || act == cache); }
+// page_size as a shift, -1 if it is none of the sizes
+inline int page_shift_of(int page_size) {
+  for (int s = 0; s <= 10; ++s)
+    if (page_size == 1 << s) return s;
+  return -1;
+}
+// a row stride in elements: whole 16-byte words, and rows that do not overlap
+inline bool stride_ok(int64_t stride, int heads, int head_dim, int act) {
+  return stride >= (int64_t)heads * head_dim && stride * type_bytes(act) % 16 == 0;
+}
+constexpr int64_t kMaxRows = 0x7fffffff;
+
+// f(activation type, cache type, head size) for one of the pairs the entries take
+template <typename A, typename C, typename F>
+int32_t with_head(int head_dim, F f) {
+  if (head_dim == 128) return f(A(), C(), std::integral_constant<int, 128>());
+  return f(A(), C(), std::integral_constant<int, 64>());
+}
+template <typename F>
+int32_t with_types(int act, int cache, int head_dim, F f) {
+  if (act == kF16) return with_head<__half, __half>(head_dim, f);
+  if (act == kBF16) return with_head<__nv_bfloat16, __nv_bfloat16>(head_dim, f);
+  if (cache == kF16) return with_head<float, __half>(head_dim, f);
+  if (cache == kBF16) return with_head<float, __nv_bfloat16>(head_dim, f);
+  return with_head<float, float>(head_dim, f);
+}
+inline int32_t status_of(cudaError_t e) { return e == cudaSuccess ? kOk : kLaunchFailure; }
+
+}  // namespace
+
+cudaError_t attn_device_error(int* code, bool clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(code, g_fq_dev_error, sizeof(int));
+  if (e == cudaSuccess && clear && *code) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_fq_dev_error, &zero, sizeof(int));
+  }
+  return e;
+}
+
+}  // namespace fq
+
+using namespace fq;
+
+extern "C" {
+
+int32_t fuelq_paged_append(int32_t act_type, int32_t cache_type, const void* k, int64_t k_stride, const void* v,
+                           int64_t v_stride, const void* q, int64_t q_stride, void* q_out, void* k_out, void* kcache,
+                           void* vcache, const int32_t* page_table, const int32_t* seq_ids, const int32_t* positions,
+                           const float* cos_table, const float* sin_table, int64_t n_rows, int32_t n_seqs, int32_t n_heads,
+                           int32_t n_kv, int32_t head_dim, int32_t page_size, int32_t n_pages, int32_t max_pages,
+                           int32_t max_pos, void* stream) {
+  if (!type_pair(act_type, cache_type) || (head_dim != 64 && head_dim != 128)) return kNotSupported;
+  const int shift = page_shift_of(page_size);
+  if (shift < 0) return kNotSupported;
+  if (n_rows < 0 || n_rows > kMaxRows || n_seqs < 0 || n_kv <= 0 || n_pages < 0 || max_pages < 0 || max_pos < 0) return kInvalidProblem;
+  if (q && (n_heads <= 0 || n_heads % n_kv)) return kInvalidProblem;
+  if (n_rows == 0) return kOk;
+  if (!k || !v || !kcache || !vcache || !page_table || !positions || !cos_table || !sin_table || (q && !q_out)) return kInvalidProblem;
+  if (!stride_ok(k_stride, n_kv, head_dim, act_type) || !stride_ok(v_stride, n_kv, head_dim, act_type)) return kInvalidProblem;
+  if (q && !stride_ok(q_stride, n_heads, head_dim, act_type)) return kInvalidProblem;
+  if (!seq_ids && n_rows > n_seqs) return kInvalidProblem;
+  // in place only where a row is written where it was read
+  if ((q && q_out == q && q_stride != (int64_t)n_heads * head_dim) || (k_out == k && k_stride != (int64_t)n_kv * head_dim)) return kInvalidProblem;
+  if (!aligned16(k) || !aligned16(v) || !aligned16(kcache) || !aligned16(vcache) || !aligned16(cos_table) || !aligned16(sin_table) ||
+      (q && (!aligned16(q) || !aligned16(q_out))) || !aligned16(k_out))
+    return kMisaligned;
+  AppendParams p = {};
+  p.k = k, p.v = v, p.q = q, p.q_out = q_out, p.k_out = k_out, p.kc = kcache, p.vc = vcache;
+  p.k_stride = k_stride, p.v_stride = v_stride, p.q_stride = q ? q_stride : 0;
+  p.table = page_table, p.seq_ids = seq_ids, p.positions = positions, p.cos_table = cos_table, p.sin_table = sin_table;
+  p.n_seqs = n_seqs, p.n_heads = q ? n_heads : 0, p.n_kv = n_kv;
+  p.page_shift = shift, p.n_pages = n_pages, p.max_pages = max_pages, p.max_pos = max_pos;
+  // few rows: a block for every 16 (head_dim 64: 32) lines, so that all loads of the call are in flight at once
+  const int lines = p.n_heads + 2 * n_kv, slots = kAppendThreads / (head_dim / 16);
+  const int pieces = (lines + slots - 1) / slots;
+  const bool few = n_rows * pieces <= 1024;
+  p.lines_per_block = few ? slots : lines;
+  const dim3 grid((unsigned)n_rows, (unsigned)(few ? pieces : 1));
+  return with_types(act_type, cache_type, head_dim, [&](auto a, auto c, auto hd) {
+    return status_of(launch(paged_append_kernel<decltype(a), decltype(c), decltype(hd)::value>, grid, dim3(kAppendThreads), 0,
+                            (cudaStream_t)stream, p));
+  });
+}
+
+size_t fuelq_paged_attn_workspace_bytes(int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t head_dim) {
+  if (n_seqs <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || (head_dim != 64 && head_dim != 128)) return 0;
+  return 0;
+}
+
+int32_t fuelq_paged_attn_decode(int32_t act_type, int32_t cache_type, const void* q, int64_t q_stride, const void* kcache,
+                                const void* vcache, void* out, const int32_t* page_table, const int32_t* seq_lens,
+                                int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t page_size,
+                                int32_t n_pages, int32_t max_pages, float scale, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  if (!type_pair(act_type, cache_type) || (head_dim != 64 && head_dim != 128)) return kNotSupported;
+  const int shift = page_shift_of(page_size);
+  if (shift < 0) return kNotSupported;
+  if (n_seqs < 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || n_heads > 65535 || n_pages < 0 || max_pages < 0) return kInvalidProblem;
+  if (n_seqs == 0) return kOk;
+  if (!q || !kcache || !vcache || !out || !page_table || !seq_lens) return kInvalidProblem;
+  if (!stride_ok(q_stride, n_heads, head_dim, act_type)) return kInvalidProblem;
+  const size_t need = fuelq_paged_attn_workspace_bytes(n_seqs, n_heads, n_kv, head_dim);
+  if (need && (!workspace || workspace_bytes < need)) return kWorkspace;
+  if (!aligned16(q) || !aligned16(kcache) || !aligned16(vcache) || !aligned16(out) || !aligned16(workspace)) return kMisaligned;
+  RowAttnParams p = {};
+  p.q = q, p.k = kcache, p.v = vcache, p.out = out, p.q_stride = q_stride, p.table = page_table, p.lens = seq_lens;
+  p.n_rows = n_seqs, p.n_seqs = n_seqs, p.n_heads = n_heads, p.n_kv = n_kv, p.page_shift = shift, p.n_pages = n_pages;
+  p.max_pages = max_pages, p.scale = scale;
+  const dim3 grid((unsigned)n_seqs, (unsigned)n_heads);
+  return with_types(act_type, cache_type, head_dim, [&](auto a, auto c, auto hd) {
+    return status_of(launch(row_attn_kernel<decltype(a), decltype(c), decltype(hd)::value, true>, grid, dim3(128), 0,
+                            (cudaStream_t)stream, p));
+  });
+}
+
+size_t fuelq_prompt_attn_workspace_bytes(int32_t act_type, int64_t n_rows, int32_t n_heads, int32_t n_kv, int32_t head_dim) {
+  if (!type_bytes(act_type) || n_rows <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || (head_dim != 64 && head_dim != 128)) return 0;
+  return 0;
+}
+
+int32_t fuelq_prompt_attn(int32_t act_type, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                          int64_t v_stride, void* out, const int32_t* cu_seqlens, int32_t n_seqs, int64_t n_rows,
+                          int32_t n_heads, int32_t n_kv, int32_t head_dim, float scale, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  if (!type_bytes(act_type) || (head_dim != 64 && head_dim != 128)) return kNotSupported;
+  if (n_seqs < 0 || n_rows < 0 || n_rows > kMaxRows || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || n_heads > 65535) return kInvalidProblem;
+  if (n_seqs == 0 || n_rows == 0) return kOk;
+  if (!q || !k || !v || !out || !cu_seqlens) return kInvalidProblem;
+  if (!stride_ok(q_stride, n_heads, head_dim, act_type) || !stride_ok(k_stride, n_kv, head_dim, act_type) ||
+      !stride_ok(v_stride, n_kv, head_dim, act_type))
+    return kInvalidProblem;
+  const size_t need = fuelq_prompt_attn_workspace_bytes(act_type, n_rows, n_heads, n_kv, head_dim);
+  if (need && (!workspace || workspace_bytes < need)) return kWorkspace;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(workspace)) return kMisaligned;
+  RowAttnParams p = {};
+  p.q = q, p.k = k, p.v = v, p.out = out, p.q_stride = q_stride, p.k_stride = k_stride, p.v_stride = v_stride, p.lens = cu_seqlens;
+  p.n_rows = n_rows, p.n_seqs = n_seqs, p.n_heads = n_heads, p.n_kv = n_kv, p.scale = scale;
+  const dim3 grid((unsigned)n_rows, (unsigned)n_heads);
+  return with_types(act_type, act_type, head_dim, [&](auto a, auto c, auto hd) {
+    return status_of(launch(row_attn_kernel<decltype(a), decltype(c), decltype(hd)::value, false>, grid, dim3(128), 0,
+                            (cudaStream_t)stream, p));
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,241 @@
+// Attention for batches of sequences: keys and values appended to a paged cache, one new token per sequence over its pages,
+// whole packed prompts. Entries in attn.cu, contract in include/fuelq.h.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "fq_common.cuh"
+
+namespace fq {
+
+cudaError_t attn_device_error(int* code, bool clear);  // the error word of these kernels (attn.cu)
+
+// ---- values of the three types
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// eight consecutive values, held as they are in memory
+template <typename T>
+struct Vec8 {
+  static constexpr int kWords = sizeof(T) / 2;  // 16-byte words
+  uint4 w[kWords];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = to_f32(reinterpret_cast<const T*>(w)[i]);
+  }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(w)[i] = from_f32<T>(f[i]);
+  }
+};
+
+// ---- append -------------------------------------------------------------------------------------
+//   lo' = lo * cos - hi * sin,  hi' = hi * cos + lo * sin   with lo, hi the halves of a head, in f32, rounded once into the
+//   output's type; the same operations in the same order as rope_store_kernel, so the same bits.
+// Bound by HBM for prompts and by latency for single tokens. A thread block takes one row of the batch: its position, page and
+// angles are read once per thread and serve all the heads ("lines": query heads, key heads, value heads) the thread walks.
+// A thread holds eight elements of the lower half of a line and the eight that they turn with: 16-byte accesses for every type.
+struct AppendParams {
+  const void *k, *v, *q;
+  void *q_out, *k_out, *kc, *vc;
+  int64_t k_stride, v_stride, q_stride;
+  const int *table, *seq_ids, *positions;
+  const float *cos_table, *sin_table;
+  int n_seqs, n_heads, n_kv;  // n_heads: 0 without q
+  int page_shift, n_pages, max_pages, max_pos;
+  int lines_per_block;
+};
+constexpr int kAppendThreads = 128;
+
+template <typename A, typename C, int kHd>
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendParams p) {
+  constexpr int kHalf = kHd / 2, kChunks = kHalf / 8, kSlots = kAppendThreads / kChunks;
+  constexpr int kBatch = sizeof(A) == 4 ? 2 : 4;  // lines a thread has in flight
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t row = blockIdx.x;
+  const int pos = p.positions[row];
+  const int64_t seq = p.seq_ids ? (int64_t)p.seq_ids[row] : row;
+  if (pos < 0 || seq < 0) return;  // padding
+  const int page_at = pos >> p.page_shift;
+  const bool in_table = seq < p.n_seqs && page_at < p.max_pages && pos < p.max_pos;
+  const int page = in_table ? p.table[seq * p.max_pages + page_at] : -1;
+  if (page < 0 || page >= p.n_pages) {
+    if (threadIdx.x == 0) record_dev_error(kErrIndex);
+    return;
+  }
+  const int c = threadIdx.x % kChunks;
+  float cs[8], sn[8];
+  Vec8<float> t;
+  t.load(p.cos_table + (int64_t)pos * kHd + 8 * c);
+  t.get(cs);
+  t.load(p.sin_table + (int64_t)pos * kHd + 8 * c);
+  t.get(sn);
+  const int first = blockIdx.y * p.lines_per_block;
+  const int last = min(first + p.lines_per_block, p.n_heads + 2 * p.n_kv);
+  const int64_t in_page = pos & ((1 << p.page_shift) - 1);
+  const A* q = reinterpret_cast<const A*>(p.q) + row * p.q_stride;
+  const A* k = reinterpret_cast<const A*>(p.k) + row * p.k_stride;
+  const A* v = reinterpret_cast<const A*>(p.v) + row * p.v_stride;
+  for (int l0 = first + threadIdx.x / kChunks; l0 < last; l0 += kBatch * kSlots) {
+    Vec8<A> lo[kBatch], hi[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int l = l0 + b * kSlots;
+      if (l >= last) break;
+      const A* src = l < p.n_heads ? q + l * kHd : l < p.n_heads + p.n_kv ? k + (l - p.n_heads) * kHd : v + (l - p.n_heads - p.n_kv) * kHd;
+      lo[b].load(src + 8 * c);
+      hi[b].load(src + kHalf + 8 * c);
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int l = l0 + b * kSlots;
+      if (l >= last) break;
+      float x[8], y[8];
+      lo[b].get(x);
+      hi[b].get(y);
+      const bool value = l >= p.n_heads + p.n_kv;
+      if (!value) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float a = x[i], z = y[i];
+          x[i] = __fsub_rn(__fmul_rn(a, cs[i]), __fmul_rn(z, sn[i]));
+          y[i] = __fadd_rn(__fmul_rn(z, cs[i]), __fmul_rn(a, sn[i]));
+        }
+      }
+      A* out = nullptr;  // the contiguous result beside the cache
+      if (l < p.n_heads)
+        out = reinterpret_cast<A*>(p.q_out) + (row * p.n_heads + l) * kHd;
+      else if (!value && p.k_out)
+        out = reinterpret_cast<A*>(p.k_out) + (row * p.n_kv + (l - p.n_heads)) * kHd;
+      if (out) {
+        Vec8<A> o;
+        o.set(x);
+        o.store(out + 8 * c);
+        o.set(y);
+        o.store(out + kHalf + 8 * c);
+      }
+      if (l >= p.n_heads) {
+        const int head = value ? l - p.n_heads - p.n_kv : l - p.n_heads;
+        C* dst = reinterpret_cast<C*>(value ? p.vc : p.kc) + ((((int64_t)page * p.n_kv + head) << p.page_shift) + in_page) * kHd;
+        Vec8<C> o;
+        o.set(x);
+        o.store(dst + 8 * c);
+        o.set(y);
+        o.store(dst + kHalf + 8 * c);
+      }
+    }
+  }
+}
+
+// ---- attention of one row and one head at a time: the plain form of both operators -----------------
+struct RowAttnParams {
+  const void *q, *k, *v;  // k, v: the caches when paged
+  void* out;
+  int64_t q_stride, k_stride, v_stride;
+  const int *table, *lens;  // lens: seq_lens when paged, cu_seqlens otherwise
+  int64_t n_rows;
+  int n_seqs, n_heads, n_kv, page_shift, n_pages, max_pages;
+  float scale;
+};
+template <typename A, typename C, int kHd, bool kPaged>
+__global__ void __launch_bounds__(128) row_attn_kernel(const RowAttnParams p) {
+  constexpr int kPer = kHd / 32;
+  __shared__ float acc_s[4][kHd];
+  __shared__ float m_s[4], l_s[4];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t row = blockIdx.x;
+  const int head = blockIdx.y, kvh = head / (p.n_heads / p.n_kv);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int64_t first = 0, n = 0;
+  bool bad = false;
+  if (kPaged) {
+    n = p.lens[row];
+    const int64_t most = (int64_t)p.max_pages << p.page_shift;
+    if (n > most) n = most, bad = true;
+    if (n < 0) n = 0;
+  } else {
+    int s = 0, e = p.n_seqs;  // the sequence that holds the row: the last one that starts at or before it
+    while (e - s > 1) {
+      const int mid = (s + e) >> 1;
+      if (p.lens[mid] <= row) s = mid; else e = mid;
+    }
+    first = p.lens[s];
+    const int64_t end = p.lens[s + 1];
+    if (first < 0 || end < first || end > p.n_rows) {
+      if (threadIdx.x == 0) record_dev_error(kErrIndex);
+      return;
+    }
+    if (row < first || row >= end) return;
+    n = row - first + 1;
+  }
+  const A* q = reinterpret_cast<const A*>(p.q) + row * p.q_stride + head * kHd + lane * kPer;
+  float qv[kPer], acc[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) qv[i] = to_f32(q[i]) * p.scale, acc[i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  for (int64_t j = warp; j < n; j += 4) {
+    const C *kr, *vr;
+    if (kPaged) {
+      const int page = p.table[row * p.max_pages + (j >> p.page_shift)];
+      if (page < 0 || page >= p.n_pages) {
+        bad = true;
+        continue;
+      }
+      const int64_t at = ((((int64_t)page * p.n_kv + kvh) << p.page_shift) + (j & ((1 << p.page_shift) - 1))) * kHd;
+      kr = reinterpret_cast<const C*>(p.k) + at, vr = reinterpret_cast<const C*>(p.v) + at;
+    } else {
+      kr = reinterpret_cast<const C*>(p.k) + (first + j) * p.k_stride + kvh * kHd;
+      vr = reinterpret_cast<const C*>(p.v) + (first + j) * p.v_stride + kvh * kHd;
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) s += qv[i] * to_f32(kr[lane * kPer + i]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    const float top = fmaxf(m, s);
+    const float keep = m == -INFINITY ? 0.f : expf(m - top), e = s == -INFINITY ? 0.f : expf(s - top);
+    l = l * keep + e;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * keep + e * to_f32(vr[lane * kPer + i]);
+    m = top;
+  }
+  if (bad && lane == 0) record_dev_error(kErrIndex);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) acc_s[warp][lane * kPer + i] = acc[i];
+  if (lane == 0) m_s[warp] = m, l_s[warp] = l;
+  __syncthreads();
+  if (threadIdx.x < kHd) {
+    float top = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3])), num = 0.f, den = 0.f;
+    for (int w = 0; w < 4; ++w) {
+      if (m_s[w] == -INFINITY) continue;
+      const float f = expf(m_s[w] - top);
+      num += f * acc_s[w][threadIdx.x], den += f * l_s[w];
+    }
+    reinterpret_cast<A*>(p.out)[(row * p.n_heads + head) * kHd + threadIdx.x] = from_f32<A>(den == 0.f ? 0.f : num / den);
+  }
+}
+
+}  // namespace fq

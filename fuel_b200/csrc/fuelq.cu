@@ -1,5 +1,6 @@
 // libfuelq.so — C ABI over the sm_100a kernels (see include/fuelq.h for the contract).
-// The kernels live in the .cuh files included below; those of ibatch.cuh are compiled beside this file, in ibatch.cu.
+// The kernels live in the .cuh files included below; those of ibatch.cuh are compiled beside this file, in ibatch.cu, and the
+// paged-cache and prompt attention entries with their kernels in attn.cu.
 #include "../../include/fuelq.h"
 
 #include <cuda_bf16.h>
@@ -8,6 +9,7 @@
 
 #include <cmath>
 
+#include "attn.cuh"
 #include "decode.cuh"
 #include "decode_regs.cuh"
 #include "dequantize.cuh"
@@ -1107,13 +1109,14 @@ int32_t fuelq_device_error(int32_t* host_code_out, int32_t clear) {
   int code = 0;
   if (cudaDeviceSynchronize() != cudaSuccess) return kLaunchFailure;
   if (cudaMemcpyFromSymbol(&code, g_fq_dev_error, sizeof(int)) != cudaSuccess) return kLaunchFailure;
-  int batch = 0;
+  int batch = 0, attn = 0;
   if (ibatch_device_error(&batch, clear != 0) != cudaSuccess) return kLaunchFailure;
+  if (attn_device_error(&attn, clear != 0) != cudaSuccess) return kLaunchFailure;
   if (clear && code) {
     const int zero = 0;
     if (cudaMemcpyToSymbol(g_fq_dev_error, &zero, sizeof(int)) != cudaSuccess) return kLaunchFailure;
   }
-  if (host_code_out) *host_code_out = code ? code : batch;
+  if (host_code_out) *host_code_out = code ? code : batch ? batch : attn;
   return kOk;
 }
 

@@ -135,6 +135,157 @@ def dequantize(dtype: GgmlDType, blocks: torch.Tensor, elem_count: int,
     return out
 
 
+# ---- attention for batches of sequences: a paged key-value cache, whole packed prompts
+
+def _heads(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) -> int:
+    """Checks a [rows, heads, head_dim] tensor whose rows may lie apart; its row stride in elements."""
+    if not t.is_cuda or t.device != device:
+        raise ValueError(f"{name} must be a CUDA tensor on the device of the other operands (there is no CPU path)")
+    if t.dim() != 3 or t.dtype != dtype:
+        raise ValueError(f"{name} must be a {dtype} tensor of [rows, heads, head_dim]")
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise ValueError(f"the heads of a row of {name} must be contiguous")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _indices(t: torch.Tensor, name: str, dims: int, device: torch.device) -> None:
+    if t.dtype != torch.int32 or t.dim() != dims or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {dims} dimension(s) on the device of the other operands")
+
+
+def _paged(kcache: torch.Tensor, vcache: torch.Tensor, device: torch.device):
+    """Checks a paged cache; (pages, kv heads, page size, head_dim)."""
+    if kcache.dim() != 4 or kcache.shape != vcache.shape or kcache.dtype != vcache.dtype or kcache.dtype not in _OUT_TYPES:
+        raise ValueError("the caches must be two f32, f16 or bf16 tensors of [pages, kv_heads, page_size, head_dim]")
+    if kcache.device != device or vcache.device != device or not kcache.is_contiguous() or not vcache.is_contiguous():
+        raise ValueError("the caches must be contiguous, on the device of the other operands")
+    return kcache.shape
+
+
+def _result(out: torch.Tensor | None, like: torch.Tensor, name: str) -> torch.Tensor:
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {like.dtype} tensor of {tuple(like.shape)} on the device of the operands")
+    return out
+
+
+def _scratch(workspace: torch.Tensor | None, nbytes: int, device: torch.device) -> torch.Tensor:
+    if workspace is None:
+        return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    if workspace.device != device or not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous, on the device of the operands")
+    return workspace
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, page_table: torch.Tensor,
+                 positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *, seq_ids: torch.Tensor | None = None,
+                 q: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+                 k_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Keys k [rows, kv_heads, head_dim], rotated by positions[row], and values v go to that position of sequence
+    seq_ids[row] (None: sequence `row`) in the paged caches [pages, kv_heads, page_size, head_dim]; page_table is
+    [sequences, pages of the longest]. Rows with a negative position or sequence number are padding. Returns the rotated
+    queries (q_out, or a new tensor) if q is given; k_out, if given, receives the rotated keys. The rows of q, k and v may be
+    column ranges of one stacked projection."""
+    dev = k.device
+    ks, vs = _heads(k, "k", k.dtype, dev), _heads(v, "v", k.dtype, dev)
+    if k.dtype not in _OUT_TYPES or v.shape != k.shape:
+        raise ValueError("k and v must be f32, f16 or bf16 and of one shape")
+    rows, kv, hd = k.shape
+    pages, ckv, page, chd = _paged(kcache, vcache, dev)
+    if (ckv, chd) != (kv, hd):
+        raise ValueError(f"the caches hold {ckv} heads of {chd}, k has {kv} of {hd}")
+    _indices(page_table, "page_table", 2, dev)
+    _indices(positions, "positions", 1, dev)
+    if seq_ids is not None:
+        _indices(seq_ids, "seq_ids", 1, dev)
+    if positions.shape[0] != rows or (seq_ids is not None and seq_ids.shape[0] != rows):
+        raise ValueError("positions and seq_ids need one entry per row")
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != hd or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous f32 table of [positions, head_dim]")
+    heads, qs = 0, 0
+    if q is not None:
+        qs = _heads(q, "q", k.dtype, dev)
+        if q.shape[0] != rows or q.shape[2] != hd:
+            raise ValueError("q must have the rows and the head_dim of k")
+        heads = q.shape[1]
+        q_out = _result(q_out, q, "q_out")
+    if k_out is not None:
+        _result(k_out, k, "k_out")
+    with torch.cuda.device(dev):
+        _lib.check(_L.fuelq_paged_append(int(_OUT_TYPES[k.dtype]), int(_OUT_TYPES[kcache.dtype]), k.data_ptr(), ks, v.data_ptr(), vs,
+                                         q.data_ptr() if q is not None else None, qs, q_out.data_ptr() if q is not None else None,
+                                         k_out.data_ptr() if k_out is not None else None, kcache.data_ptr(), vcache.data_ptr(),
+                                         page_table.data_ptr(), seq_ids.data_ptr() if seq_ids is not None else None,
+                                         positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), rows, page_table.shape[0], heads, kv,
+                                         hd, page, pages, page_table.shape[1], min(cos.shape[0], sin.shape[0]), _stream()),
+                   "fuelq_paged_append")
+    return q_out if q is not None else None
+
+
+def paged_attn_workspace(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
+    """Scratch for paged_attn_decode; one serves every layer of a model, and every call on one stream."""
+    nbytes = _L.fuelq_paged_attn_workspace_bytes(n_seqs, n_heads, n_kv_heads, head_dim)
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+
+
+def paged_attn_decode(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, page_table: torch.Tensor,
+                      seq_lens: torch.Tensor, scale: float | None = None, out: torch.Tensor | None = None,
+                      workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token per sequence, q [sequences, heads, head_dim] already rotated, over the first seq_lens[s]
+    positions of its pages. A length of zero, a free slot of the batch, gives zeros. Default scale: 1 / sqrt(head_dim)."""
+    dev = q.device
+    qs = _heads(q, "q", q.dtype, dev)
+    n, heads, hd = q.shape
+    pages, kv, page, chd = _paged(kcache, vcache, dev)
+    if q.dtype not in _OUT_TYPES or chd != hd:
+        raise ValueError("q must be f32, f16 or bf16 with the head_dim of the caches")
+    _indices(page_table, "page_table", 2, dev)
+    _indices(seq_lens, "seq_lens", 1, dev)
+    if page_table.shape[0] != n or seq_lens.shape[0] != n:
+        raise ValueError("page_table and seq_lens need one row per sequence")
+    out = _result(out, q, "out")
+    workspace = _scratch(workspace, _L.fuelq_paged_attn_workspace_bytes(n, heads, kv, hd), dev)
+    with torch.cuda.device(dev):
+        _lib.check(_L.fuelq_paged_attn_decode(int(_OUT_TYPES[q.dtype]), int(_OUT_TYPES[kcache.dtype]), q.data_ptr(), qs,
+                                              kcache.data_ptr(), vcache.data_ptr(), out.data_ptr(), page_table.data_ptr(),
+                                              seq_lens.data_ptr(), n, heads, kv, hd, page, pages, page_table.shape[1],
+                                              hd ** -0.5 if scale is None else scale, workspace.data_ptr(),
+                                              workspace.numel() * workspace.element_size(), _stream()), "fuelq_paged_attn_decode")
+    return out
+
+
+def prompt_attn_workspace(q: torch.Tensor, k: torch.Tensor) -> torch.Tensor:
+    """Scratch for prompt_attn on tensors of these shapes; calls on one stream may share it."""
+    nbytes = _L.fuelq_prompt_attn_workspace_bytes(int(_OUT_TYPES[q.dtype]), q.shape[0], q.shape[1], k.shape[1], q.shape[2])
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+
+
+def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float | None = None,
+                out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention inside packed prompts: rows cu_seqlens[s] .. cu_seqlens[s + 1] of q [rows, heads, head_dim] (rotated)
+    and of k, v [rows, kv_heads, head_dim] are sequence s. Rows behind the last sequence are padding: not read, and left as
+    they were in `out`. Default scale: 1 / sqrt(head_dim)."""
+    dev = q.device
+    qs, ks, vs = _heads(q, "q", q.dtype, dev), _heads(k, "k", q.dtype, dev), _heads(v, "v", q.dtype, dev)
+    rows, heads, hd = q.shape
+    if q.dtype not in _OUT_TYPES or k.shape != v.shape or k.shape[0] != rows or k.shape[2] != hd:
+        raise ValueError("q, k and v must be f32, f16 or bf16 with the same rows and head_dim")
+    _indices(cu_seqlens, "cu_seqlens", 1, dev)
+    if cu_seqlens.shape[0] < 1:
+        raise ValueError("cu_seqlens needs n_seqs + 1 entries")
+    out = _result(out, q, "out")
+    kv = k.shape[1]
+    workspace = _scratch(workspace, _L.fuelq_prompt_attn_workspace_bytes(int(_OUT_TYPES[q.dtype]), rows, heads, kv, hd), dev)
+    with torch.cuda.device(dev):
+        _lib.check(_L.fuelq_prompt_attn(int(_OUT_TYPES[q.dtype]), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+                                        out.data_ptr(), cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1, rows, heads, kv, hd,
+                                        hd ** -0.5 if scale is None else scale, workspace.data_ptr(),
+                                        workspace.numel() * workspace.element_size(), _stream()), "fuelq_prompt_attn")
+    return out
+
+
 def device_error(clear: bool = True) -> int:
     import ctypes
     code = ctypes.c_int32(0)

@@ -104,7 +104,10 @@ int32_t fuelq_set_option(int32_t key, int64_t value);
 int64_t fuelq_get_option(int32_t key);
 
 /* Reads (and, if `clear`, resets) the device-side error word set by a kernel whose
- * bounded wait expired. Synchronizes the device. 0 = no error recorded. */
+ * bounded wait expired (codes 1 to 6), or by one of the paged-cache and prompt entries that met a page, a position, a
+ * length or a sequence number outside its table (FUELQ_DEVICE_ERROR_INDEX) and left that part of its work out.
+ * Synchronizes the device. 0 = no error recorded. */
+#define FUELQ_DEVICE_ERROR_INDEX 7
 int32_t fuelq_device_error(int32_t* host_code_out, int32_t clear);
 
 /* Activation quantization to the weight format's dot-product partner: Q8_K blocks for Q2K / Q3K / Q4K / Q5K / Q6K
@@ -399,6 +402,54 @@ int32_t fuelq_swiglu(const float* gate, const float* up, float* out, int64_t n, 
 /* index of the LAST maximum of x[0..n) (LogitsProcessor argmax: max_by + total_cmp,
  * fuel-transformers/src/generation/mod.rs:84-93). */
 int32_t fuelq_argmax_last(const float* x, int64_t n, int32_t* out_index, void* stream);
+
+/* ---- Attention for batches of sequences: a paged key-value cache, and whole prompts.
+ * The reference keeps paged attention and flash decoding as ops of its CUDA backend (fuel-core/tests/paged_attn_oracle.rs,
+ * fuel-dispatch/src/baracuda_dispatch.rs:3421-3453); the arithmetic here is that of fuelq_attn_decode: scores in f32, softmax
+ * with the maximum taken off, f32 sums.
+ * Types: act_type is the type of q, k, v and the outputs, cache_type that of the pages: F32, F16 or BF16. f32 activations go
+ * with every cache type, 16-bit ones with a cache of their own type. head_dim is 64 or 128, n_heads a multiple of n_kv (query
+ * head h reads kv head h / (n_heads / n_kv)).
+ * Rows: q, k and v are [rows][heads][head_dim], the heads of a row contiguous, rows q_stride / k_stride / v_stride elements
+ * apart, so that they may be column ranges of a stacked projection; outputs are contiguous. All base addresses and row
+ * strides are multiples of 16 bytes.
+ * Pages: a cache is [n_pages][n_kv][page_size][head_dim], page_size a power of two up to 1024. page_table is
+ * [n_seqs][max_pages] int32: position p of sequence s is row p % page_size of page page_table[s][p / page_size]; entries
+ * behind a sequence's last page are not read. A sequence number, a page or a position that is out of range is never
+ * followed: the part of the work that needs it is left out and device error FUELQ_DEVICE_ERROR_INDEX recorded.
+ * All index arrays are device memory and are read by the kernels, so that a step can be replayed from a CUDA graph with
+ * other lengths. Results never depend on the order in which thread blocks finish. */
+
+/* Row t of k, rotated (rotate-half RoPE as in fuelq_rope_store, in f32) by position positions[t], and row t of v go to that
+ * position of sequence seq_ids[t] (null: sequence t). A row whose position or sequence number is negative is padding and
+ * skipped whole. q, if not null, is rotated into q_out (contiguous; may be q itself if q is contiguous); k_out, if not
+ * null, receives the rotated keys contiguously in act_type (what fuelq_prompt_attn reads; may be k itself likewise). No two
+ * rows may name one position of one sequence. cos_table, sin_table: f32 [max_pos][head_dim], both halves of a row alike (the
+ * first is read); positions from max_pos up are out of range. */
+int32_t fuelq_paged_append(int32_t act_type, int32_t cache_type, const void* k, int64_t k_stride, const void* v,
+                           int64_t v_stride, const void* q, int64_t q_stride, void* q_out, void* k_out, void* kcache,
+                           void* vcache, const int32_t* page_table, const int32_t* seq_ids, const int32_t* positions,
+                           const float* cos_table, const float* sin_table, int64_t n_rows, int32_t n_seqs, int32_t n_heads,
+                           int32_t n_kv, int32_t head_dim, int32_t page_size, int32_t n_pages, int32_t max_pages,
+                           int32_t max_pos, void* stream);
+/* One new token per sequence: out[s][h] = softmax(q[s][h] . K[0..seq_lens[s])^T * scale) . V over the sequence's pages (its
+ * new token already appended). seq_lens[s] <= 0, a free slot of the batch, gives a row of zeros. The workspace is
+ * fuelq_paged_attn_workspace_bytes() bytes, holds nothing between calls and needs no clearing. */
+size_t fuelq_paged_attn_workspace_bytes(int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t head_dim);
+int32_t fuelq_paged_attn_decode(int32_t act_type, int32_t cache_type, const void* q, int64_t q_stride, const void* kcache,
+                                const void* vcache, void* out, const int32_t* page_table, const int32_t* seq_lens,
+                                int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t page_size,
+                                int32_t n_pages, int32_t max_pages, float scale, void* workspace, size_t workspace_bytes,
+                                void* stream);
+/* Whole prompts, packed: rows cu_seqlens[s] .. cu_seqlens[s + 1] (device, n_seqs + 1 ascending values from 0) of q, k, v are
+ * sequence s, and each of its rows attends to the sequence's rows up to itself. Rows of q, k, v behind the last sequence are
+ * not read and rows of out behind it are left as they were; n_rows is the number of rows the buffers have. Nothing that
+ * stands behind a row in its sequence, or in another sequence, reaches it, infinities and NaN included. */
+size_t fuelq_prompt_attn_workspace_bytes(int32_t act_type, int64_t n_rows, int32_t n_heads, int32_t n_kv, int32_t head_dim);
+int32_t fuelq_prompt_attn(int32_t act_type, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                          int64_t v_stride, void* out, const int32_t* cu_seqlens, int32_t n_seqs, int64_t n_rows,
+                          int32_t n_heads, int32_t n_kv, int32_t head_dim, float scale, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
