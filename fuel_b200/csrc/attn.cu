@@ -2,10 +2,11 @@
 // of its own beside fuelq.cu.
 #include "../../include/fuelq.h"
 
+#include <type_traits>
+
 #include "attn.cuh"
 #include "launch.cuh"
-
-#include <type_traits>
+#include "paged_decode.cuh"
 
 namespace fq {
 namespace {
@@ -39,6 +40,43 @@ int32_t with_types(int act, int cache, int head_dim, F f) {
   if (cache == kBF16) return with_head<float, __nv_bfloat16>(head_dim, f);
   return with_head<float, float>(head_dim, f);
 }
+// the current device's number of SMs, 0 on failure
+int sm_count() {
+  static int count[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if (count[dev] == 0 && cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  return count[dev];
+}
+// once for each kernel and device: more dynamic shared memory than a launch gets by default
+template <typename K>
+bool allow_smem(K kernel, int bytes, bool (&set)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (!set[dev]) set[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+  return set[dev];
+}
+
+// heads of an item of the decode kernel, in eights: one for groups up to eight heads, two beyond (in pieces of sixteen)
+inline int decode_tiles_of_heads(int group) { return group <= 8 ? 1 : 2; }
+constexpr size_t kDecodeMetaBytes = (size_t)kDecodeMaxBlocks * 2 * sizeof(int4);
+
+template <typename A, typename C, int kHd, int kNT>
+int32_t launch_decode(DecodeParams& p, cudaStream_t stream) {
+  using Cfg = DecodeCfg<A, C, kHd, kNT>;
+  static bool set[64] = {};
+  const int sms = sm_count();
+  auto kernel = paged_decode_kernel<A, C, kHd, kNT>;
+  if (sms == 0 || !allow_smem(kernel, Cfg::kSmem, set)) return kLaunchFailure;
+  p.chunks = (p.group + Cfg::kHeads - 1) / Cfg::kHeads;
+  const int blocks = sms * Cfg::kPerSm < kDecodeMaxBlocks ? sms * Cfg::kPerSm : kDecodeMaxBlocks;
+  cudaError_t e = launch(kernel, dim3((unsigned)blocks), dim3(32 * kDecodeWarps), Cfg::kSmem, stream, p);
+  if (e == cudaSuccess)
+    e = launch(paged_join_kernel<A, C, kHd, kNT>, dim3((unsigned)blocks, (unsigned)(p.group < Cfg::kHeads ? p.group : Cfg::kHeads)), dim3(kHd), 0,
+               stream, p);
+  return e == cudaSuccess ? kOk : kLaunchFailure;
+}
+
 inline int32_t status_of(cudaError_t e) { return e == cudaSuccess ? kOk : kLaunchFailure; }
 
 }  // namespace
@@ -99,7 +137,8 @@ int32_t fuelq_paged_append(int32_t act_type, int32_t cache_type, const void* k, 
 
 size_t fuelq_paged_attn_workspace_bytes(int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t head_dim) {
   if (n_seqs <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || (head_dim != 64 && head_dim != 128)) return 0;
-  return 0;
+  const size_t slot = (size_t)decode_tiles_of_heads(n_heads / n_kv) * 8 * (head_dim + 2) * sizeof(float);
+  return kDecodeMetaBytes + 2 * kDecodeMaxBlocks * slot;
 }
 
 int32_t fuelq_paged_attn_decode(int32_t act_type, int32_t cache_type, const void* q, int64_t q_stride, const void* kcache,
@@ -117,14 +156,17 @@ int32_t fuelq_paged_attn_decode(int32_t act_type, int32_t cache_type, const void
   const size_t need = fuelq_paged_attn_workspace_bytes(n_seqs, n_heads, n_kv, head_dim);
   if (need && (!workspace || workspace_bytes < need)) return kWorkspace;
   if (!aligned16(q) || !aligned16(kcache) || !aligned16(vcache) || !aligned16(out) || !aligned16(workspace)) return kMisaligned;
-  RowAttnParams p = {};
+  DecodeParams p = {};
   p.q = q, p.k = kcache, p.v = vcache, p.out = out, p.q_stride = q_stride, p.table = page_table, p.lens = seq_lens;
-  p.n_rows = n_seqs, p.n_seqs = n_seqs, p.n_heads = n_heads, p.n_kv = n_kv, p.page_shift = shift, p.n_pages = n_pages;
-  p.max_pages = max_pages, p.scale = scale;
-  const dim3 grid((unsigned)n_seqs, (unsigned)n_heads);
+  p.n_seqs = n_seqs, p.n_heads = n_heads, p.n_kv = n_kv, p.group = n_heads / n_kv;
+  p.page_shift = shift, p.n_pages = n_pages, p.max_pages = max_pages, p.scale = scale;
+  p.meta = (int4*)workspace, p.slots = (float*)((uint8_t*)workspace + kDecodeMetaBytes);
   return with_types(act_type, cache_type, head_dim, [&](auto a, auto c, auto hd) {
-    return status_of(launch(row_attn_kernel<decltype(a), decltype(c), decltype(hd)::value, true>, grid, dim3(128), 0,
-                            (cudaStream_t)stream, p));
+    using Act = decltype(a);
+    using Cache = decltype(c);
+    constexpr int kHd = decltype(hd)::value;
+    return decode_tiles_of_heads(p.group) == 1 ? launch_decode<Act, Cache, kHd, 1>(p, (cudaStream_t)stream)
+                                               : launch_decode<Act, Cache, kHd, 2>(p, (cudaStream_t)stream);
   });
 }
 
