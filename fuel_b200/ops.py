@@ -6,6 +6,8 @@ the reference's quantized storage API (fuel-backend-contract/src/quantized.rs:29
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _lib
@@ -14,10 +16,18 @@ from .ggml import GgmlDType
 _L = _lib.lib
 _raw_stream = torch._C._cuda_getCurrentRawStream   # the handle alone: a Stream object costs microseconds
 _OUT_TYPES = {torch.float32: GgmlDType.F32, torch.float16: GgmlDType.F16, torch.bfloat16: GgmlDType.BF16}
+_TYPE_IDS = {t: int(g) for t, g in _OUT_TYPES.items()}
+_current_device = torch._C._cuda_getDevice
+_HERE = contextlib.nullcontext()
 
 
 def _stream() -> int:
     return _raw_stream(torch.cuda.current_device())
+
+
+def _on(dev: int):
+    """The device of the operands made current, which costs microseconds only where it is not."""
+    return _HERE if dev == _current_device() else torch.cuda.device(dev)
 
 
 def _need_cuda(t: torch.Tensor, name: str) -> None:
@@ -137,43 +147,46 @@ def dequantize(dtype: GgmlDType, blocks: torch.Tensor, elem_count: int,
 
 # ---- attention for batches of sequences: a paged key-value cache, whole packed prompts
 
-def _heads(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) -> int:
-    """Checks a [rows, heads, head_dim] tensor whose rows may lie apart; its row stride in elements."""
-    if not t.is_cuda or t.device != device:
+def _heads(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int) -> int:
+    """Checks a [rows, heads, head_dim] tensor on device `dev` whose rows may lie apart; its row stride in elements."""
+    if dev < 0 or t.get_device() != dev:
         raise ValueError(f"{name} must be a CUDA tensor on the device of the other operands (there is no CPU path)")
-    if t.dim() != 3 or t.dtype != dtype:
+    if t.dtype is not dtype or t.dim() != 3:
         raise ValueError(f"{name} must be a {dtype} tensor of [rows, heads, head_dim]")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+    rows, heads, hd = t.shape
+    row, head, one = t.stride()
+    if (one != 1 and hd > 1) or (head != hd and heads > 1):
         raise ValueError(f"the heads of a row of {name} must be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return row if rows > 1 else heads * hd
 
 
-def _indices(t: torch.Tensor, name: str, dims: int, device: torch.device) -> None:
-    if t.dtype != torch.int32 or t.dim() != dims or t.device != device or not t.is_contiguous():
+def _indices(t: torch.Tensor, name: str, dims: int, dev: int) -> None:
+    if t.dtype is not torch.int32 or t.dim() != dims or t.get_device() != dev or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of {dims} dimension(s) on the device of the other operands")
 
 
-def _paged(kcache: torch.Tensor, vcache: torch.Tensor, device: torch.device):
+def _paged(kcache: torch.Tensor, vcache: torch.Tensor, dev: int):
     """Checks a paged cache; (pages, kv heads, page size, head_dim)."""
-    if kcache.dim() != 4 or kcache.shape != vcache.shape or kcache.dtype != vcache.dtype or kcache.dtype not in _OUT_TYPES:
+    shape = kcache.shape
+    if len(shape) != 4 or shape != vcache.shape or kcache.dtype is not vcache.dtype or kcache.dtype not in _TYPE_IDS:
         raise ValueError("the caches must be two f32, f16 or bf16 tensors of [pages, kv_heads, page_size, head_dim]")
-    if kcache.device != device or vcache.device != device or not kcache.is_contiguous() or not vcache.is_contiguous():
+    if kcache.get_device() != dev or vcache.get_device() != dev or not kcache.is_contiguous() or not vcache.is_contiguous():
         raise ValueError("the caches must be contiguous, on the device of the other operands")
-    return kcache.shape
+    return shape
 
 
 def _result(out: torch.Tensor | None, like: torch.Tensor, name: str) -> torch.Tensor:
     if out is None:
         return torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous():
+    if out.shape != like.shape or out.dtype is not like.dtype or out.get_device() != like.get_device() or not out.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {like.dtype} tensor of {tuple(like.shape)} on the device of the operands")
     return out
 
 
-def _scratch(workspace: torch.Tensor | None, nbytes: int, device: torch.device) -> torch.Tensor:
+def _scratch(workspace: torch.Tensor | None, nbytes: int, like: torch.Tensor) -> torch.Tensor:
     if workspace is None:
-        return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
-    if workspace.device != device or not workspace.is_contiguous():
+        return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=like.device)
+    if workspace.get_device() != like.get_device() or not workspace.is_contiguous():
         raise ValueError("the workspace must be contiguous, on the device of the operands")
     return workspace
 
@@ -187,13 +200,14 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, kcache: torch.Tensor, vcache:
     [sequences, pages of the longest]. Rows with a negative position or sequence number are padding. Returns the rotated
     queries (q_out, or a new tensor) if q is given; k_out, if given, receives the rotated keys. The rows of q, k and v may be
     column ranges of one stacked projection."""
-    dev = k.device
-    ks, vs = _heads(k, "k", k.dtype, dev), _heads(v, "v", k.dtype, dev)
-    if k.dtype not in _OUT_TYPES or v.shape != k.shape:
+    dev, dtype = k.get_device(), k.dtype
+    ks, vs = _heads(k, "k", dtype, dev), _heads(v, "v", dtype, dev)
+    shape = k.shape
+    if dtype not in _TYPE_IDS or v.shape != shape:
         raise ValueError("k and v must be f32, f16 or bf16 and of one shape")
-    rows, kv, hd = k.shape
+    rows, kv, hd = shape
     pages, ckv, page, chd = _paged(kcache, vcache, dev)
-    if (ckv, chd) != (kv, hd):
+    if ckv != kv or chd != hd:
         raise ValueError(f"the caches hold {ckv} heads of {chd}, k has {kv} of {hd}")
     _indices(page_table, "page_table", 2, dev)
     _indices(positions, "positions", 1, dev)
@@ -202,26 +216,28 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, kcache: torch.Tensor, vcache:
     if positions.shape[0] != rows or (seq_ids is not None and seq_ids.shape[0] != rows):
         raise ValueError("positions and seq_ids need one entry per row")
     for t, name in ((cos, "cos"), (sin, "sin")):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != hd or t.device != dev or not t.is_contiguous():
+        if t.dtype is not torch.float32 or t.dim() != 2 or t.shape[1] != hd or t.get_device() != dev or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous f32 table of [positions, head_dim]")
-    heads, qs = 0, 0
+    heads = qs = 0
     if q is not None:
-        qs = _heads(q, "q", k.dtype, dev)
+        qs = _heads(q, "q", dtype, dev)
         if q.shape[0] != rows or q.shape[2] != hd:
             raise ValueError("q must have the rows and the head_dim of k")
         heads = q.shape[1]
         q_out = _result(q_out, q, "q_out")
     if k_out is not None:
         _result(k_out, k, "k_out")
-    with torch.cuda.device(dev):
-        _lib.check(_L.fuelq_paged_append(int(_OUT_TYPES[k.dtype]), int(_OUT_TYPES[kcache.dtype]), k.data_ptr(), ks, v.data_ptr(), vs,
-                                         q.data_ptr() if q is not None else None, qs, q_out.data_ptr() if q is not None else None,
-                                         k_out.data_ptr() if k_out is not None else None, kcache.data_ptr(), vcache.data_ptr(),
-                                         page_table.data_ptr(), seq_ids.data_ptr() if seq_ids is not None else None,
-                                         positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), rows, page_table.shape[0], heads, kv,
-                                         hd, page, pages, page_table.shape[1], min(cos.shape[0], sin.shape[0]), _stream()),
-                   "fuelq_paged_append")
-    return q_out if q is not None else None
+    seqs, width = page_table.shape
+    with _on(dev):
+        status = _L.fuelq_paged_append(_TYPE_IDS[dtype], _TYPE_IDS[kcache.dtype], k.data_ptr(), ks, v.data_ptr(), vs,
+                                       None if q is None else q.data_ptr(), qs, None if q is None else q_out.data_ptr(),
+                                       None if k_out is None else k_out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(),
+                                       page_table.data_ptr(), None if seq_ids is None else seq_ids.data_ptr(), positions.data_ptr(),
+                                       cos.data_ptr(), sin.data_ptr(), rows, seqs, heads, kv, hd, page, pages, width,
+                                       min(cos.shape[0], sin.shape[0]), _raw_stream(dev))
+    if status:
+        _lib.check(status, "fuelq_paged_append")
+    return None if q is None else q_out
 
 
 def paged_attn_workspace(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
@@ -235,24 +251,26 @@ def paged_attn_decode(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tenso
                       workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of one new token per sequence, q [sequences, heads, head_dim] already rotated, over the first seq_lens[s]
     positions of its pages. A length of zero, a free slot of the batch, gives zeros. Default scale: 1 / sqrt(head_dim)."""
-    dev = q.device
-    qs = _heads(q, "q", q.dtype, dev)
+    dev, dtype = q.get_device(), q.dtype
+    qs = _heads(q, "q", dtype, dev)
     n, heads, hd = q.shape
     pages, kv, page, chd = _paged(kcache, vcache, dev)
-    if q.dtype not in _OUT_TYPES or chd != hd:
+    if dtype not in _TYPE_IDS or chd != hd:
         raise ValueError("q must be f32, f16 or bf16 with the head_dim of the caches")
     _indices(page_table, "page_table", 2, dev)
     _indices(seq_lens, "seq_lens", 1, dev)
-    if page_table.shape[0] != n or seq_lens.shape[0] != n:
+    seqs, width = page_table.shape
+    if seqs != n or seq_lens.shape[0] != n:
         raise ValueError("page_table and seq_lens need one row per sequence")
     out = _result(out, q, "out")
-    workspace = _scratch(workspace, _L.fuelq_paged_attn_workspace_bytes(n, heads, kv, hd), dev)
-    with torch.cuda.device(dev):
-        _lib.check(_L.fuelq_paged_attn_decode(int(_OUT_TYPES[q.dtype]), int(_OUT_TYPES[kcache.dtype]), q.data_ptr(), qs,
-                                              kcache.data_ptr(), vcache.data_ptr(), out.data_ptr(), page_table.data_ptr(),
-                                              seq_lens.data_ptr(), n, heads, kv, hd, page, pages, page_table.shape[1],
-                                              hd ** -0.5 if scale is None else scale, workspace.data_ptr(),
-                                              workspace.numel() * workspace.element_size(), _stream()), "fuelq_paged_attn_decode")
+    workspace = _scratch(workspace, _L.fuelq_paged_attn_workspace_bytes(n, heads, kv, hd) if workspace is None else 0, q)
+    with _on(dev):
+        status = _L.fuelq_paged_attn_decode(_TYPE_IDS[dtype], _TYPE_IDS[kcache.dtype], q.data_ptr(), qs, kcache.data_ptr(),
+                                            vcache.data_ptr(), out.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), n, heads,
+                                            kv, hd, page, pages, width, hd ** -0.5 if scale is None else scale,
+                                            workspace.data_ptr(), workspace.nbytes, _raw_stream(dev))
+    if status:
+        _lib.check(status, "fuelq_paged_attn_decode")
     return out
 
 
@@ -267,22 +285,25 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: t
     """Causal attention inside packed prompts: rows cu_seqlens[s] .. cu_seqlens[s + 1] of q [rows, heads, head_dim] (rotated)
     and of k, v [rows, kv_heads, head_dim] are sequence s. Rows behind the last sequence are padding: not read, and left as
     they were in `out`. Default scale: 1 / sqrt(head_dim)."""
-    dev = q.device
-    qs, ks, vs = _heads(q, "q", q.dtype, dev), _heads(k, "k", q.dtype, dev), _heads(v, "v", q.dtype, dev)
+    dev, dtype = q.get_device(), q.dtype
+    qs, ks, vs = _heads(q, "q", dtype, dev), _heads(k, "k", dtype, dev), _heads(v, "v", dtype, dev)
     rows, heads, hd = q.shape
-    if q.dtype not in _OUT_TYPES or k.shape != v.shape or k.shape[0] != rows or k.shape[2] != hd:
+    shape = k.shape
+    if dtype not in _TYPE_IDS or shape != v.shape or shape[0] != rows or shape[2] != hd:
         raise ValueError("q, k and v must be f32, f16 or bf16 with the same rows and head_dim")
+    kv = shape[1]
     _indices(cu_seqlens, "cu_seqlens", 1, dev)
-    if cu_seqlens.shape[0] < 1:
+    seqs = cu_seqlens.shape[0] - 1
+    if seqs < 0:
         raise ValueError("cu_seqlens needs n_seqs + 1 entries")
     out = _result(out, q, "out")
-    kv = k.shape[1]
-    workspace = _scratch(workspace, _L.fuelq_prompt_attn_workspace_bytes(int(_OUT_TYPES[q.dtype]), rows, heads, kv, hd), dev)
-    with torch.cuda.device(dev):
-        _lib.check(_L.fuelq_prompt_attn(int(_OUT_TYPES[q.dtype]), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
-                                        out.data_ptr(), cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1, rows, heads, kv, hd,
-                                        hd ** -0.5 if scale is None else scale, workspace.data_ptr(),
-                                        workspace.numel() * workspace.element_size(), _stream()), "fuelq_prompt_attn")
+    workspace = _scratch(workspace, _L.fuelq_prompt_attn_workspace_bytes(_TYPE_IDS[dtype], rows, heads, kv, hd) if workspace is None else 0, q)
+    with _on(dev):
+        status = _L.fuelq_prompt_attn(_TYPE_IDS[dtype], q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(),
+                                      cu_seqlens.data_ptr(), seqs, rows, heads, kv, hd, hd ** -0.5 if scale is None else scale,
+                                      workspace.data_ptr(), workspace.nbytes, _raw_stream(dev))
+    if status:
+        _lib.check(status, "fuelq_prompt_attn")
     return out
 
 
