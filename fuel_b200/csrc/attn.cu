@@ -2,11 +2,13 @@
 // of its own beside fuelq.cu.
 #include "../../include/fuelq.h"
 
+#include <cmath>
 #include <type_traits>
 
 #include "attn.cuh"
 #include "launch.cuh"
 #include "paged_decode.cuh"
+#include "prompt_attn.cuh"
 
 namespace fq {
 namespace {
@@ -75,6 +77,44 @@ int32_t launch_decode(DecodeParams& p, cudaStream_t stream) {
     e = launch(paged_join_kernel<A, C, kHd, kNT>, dim3((unsigned)blocks, (unsigned)(p.group < Cfg::kHeads ? p.group : Cfg::kHeads)), dim3(kHd), 0,
                stream, p);
   return e == cudaSuccess ? kOk : kLaunchFailure;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// tensor map of 16-bit rows [rows][heads][head_dim], `stride` elements apart: boxes of 128 bytes of one head x box_rows rows, 128-byte
+// swizzle, zeros behind the last row
+bool make_rows_map(const void* x, int64_t rows, int heads, int head_dim, int64_t stride, int box_rows, CUtensorMap* map) {
+  static EncodeTiledFn encode = nullptr;
+  if (!encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess || !fn)
+      return false;
+    encode = (EncodeTiledFn)fn;
+  }
+  const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)head_dim * 2, (cuuint64_t)stride * 2};
+  const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows}, ones[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(x), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int kHd>
+int32_t launch_prompt(const PromptParams& p, const RowAttnParams& r, cudaStream_t stream) {
+  using Cfg = PromptCfg<T, kHd>;
+  static bool set[64] = {};
+  const int sms = sm_count();
+  auto kernel = prompt_attn_kernel<T, kHd>;
+  if (sms == 0 || !allow_smem(kernel, Cfg::kSmem, set)) return kLaunchFailure;
+  CUtensorMap qmap, kmap, vmap;
+  if (!make_rows_map(r.q, r.n_rows, r.n_heads, kHd, r.q_stride, kPaTile, &qmap) ||
+      !make_rows_map(r.k, r.n_rows, r.n_kv, kHd, r.k_stride, kPaTile, &kmap) ||
+      !make_rows_map(r.v, r.n_rows, r.n_kv, kHd, r.v_stride, kPaTile, &vmap))
+    return kLaunchFailure;
+  const dim3 grid((unsigned)(p.n_items < sms ? p.n_items : sms));
+  return launch(kernel, grid, dim3(kPaThreads), Cfg::kSmem, stream, p, qmap, kmap, vmap) == cudaSuccess ? kOk : kLaunchFailure;
 }
 
 inline int32_t status_of(cudaError_t e) { return e == cudaSuccess ? kOk : kLaunchFailure; }
@@ -149,7 +189,7 @@ int32_t fuelq_paged_attn_decode(int32_t act_type, int32_t cache_type, const void
   if (!type_pair(act_type, cache_type) || (head_dim != 64 && head_dim != 128)) return kNotSupported;
   const int shift = page_shift_of(page_size);
   if (shift < 0) return kNotSupported;
-  if (n_seqs < 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || n_heads > 65535 || n_pages < 0 || max_pages < 0) return kInvalidProblem;
+  if (n_seqs < 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || !(scale >= 0.f) || std::isinf(scale) || n_pages < 0 || max_pages < 0) return kInvalidProblem;
   if (n_seqs == 0) return kOk;
   if (!q || !kcache || !vcache || !out || !page_table || !seq_lens) return kInvalidProblem;
   if (!stride_ok(q_stride, n_heads, head_dim, act_type)) return kInvalidProblem;
@@ -180,7 +220,7 @@ int32_t fuelq_prompt_attn(int32_t act_type, const void* q, int64_t q_stride, con
                           int32_t n_heads, int32_t n_kv, int32_t head_dim, float scale, void* workspace,
                           size_t workspace_bytes, void* stream) {
   if (!type_bytes(act_type) || (head_dim != 64 && head_dim != 128)) return kNotSupported;
-  if (n_seqs < 0 || n_rows < 0 || n_rows > kMaxRows || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || n_heads > 65535) return kInvalidProblem;
+  if (n_seqs < 0 || n_rows < 0 || n_rows > kMaxRows || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || !(scale >= 0.f) || std::isinf(scale)) return kInvalidProblem;
   if (n_seqs == 0 || n_rows == 0) return kOk;
   if (!q || !k || !v || !out || !cu_seqlens) return kInvalidProblem;
   if (!stride_ok(q_stride, n_heads, head_dim, act_type) || !stride_ok(k_stride, n_kv, head_dim, act_type) ||
@@ -192,6 +232,15 @@ int32_t fuelq_prompt_attn(int32_t act_type, const void* q, int64_t q_stride, con
   RowAttnParams p = {};
   p.q = q, p.k = k, p.v = v, p.out = out, p.q_stride = q_stride, p.k_stride = k_stride, p.v_stride = v_stride, p.lens = cu_seqlens;
   p.n_rows = n_rows, p.n_seqs = n_seqs, p.n_heads = n_heads, p.n_kv = n_kv, p.scale = scale;
+  if (act_type != kF32) {
+    PromptParams a = {};
+    a.out = out, a.cu = cu_seqlens, a.n_rows = n_rows, a.n_items = prompt_slots(n_rows, n_seqs) * n_heads;
+    a.n_seqs = n_seqs, a.n_heads = n_heads, a.group = n_heads / n_kv, a.c = scale * 1.4426950408889634f;
+    if (act_type == kF16)
+      return head_dim == 128 ? launch_prompt<__half, 128>(a, p, (cudaStream_t)stream) : launch_prompt<__half, 64>(a, p, (cudaStream_t)stream);
+    return head_dim == 128 ? launch_prompt<__nv_bfloat16, 128>(a, p, (cudaStream_t)stream)
+                           : launch_prompt<__nv_bfloat16, 64>(a, p, (cudaStream_t)stream);
+  }
   const dim3 grid((unsigned)n_rows, (unsigned)n_heads);
   return with_types(act_type, act_type, head_dim, [&](auto a, auto c, auto hd) {
     return status_of(launch(row_attn_kernel<decltype(a), decltype(c), decltype(hd)::value, false>, grid, dim3(128), 0,

@@ -488,8 +488,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
           for (int sub = 0; sub < kSub; ++sub) top = fmaxf(top, fmaxf(s[sub][nt][j], s[sub][nt][j + 2]));
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-          const float keep = top == -INFINITY ? 1.f : exp2f(m[nt][j] - top);
-          m[nt][j] = top;
+          const bool move = top > m[nt][j] + 8.f;  // by this head's scores alone: its bits do not depend on the others'
+          const float keep = move ? exp2f(m[nt][j] - top) : 1.f;
+          if (move) m[nt][j] = top;
           l[nt][j] *= keep;
 #pragma unroll
           for (int t = 0; t < kMt; ++t) o[nt][t][j] *= keep, o[nt][t][j + 2] *= keep;
