@@ -9,6 +9,7 @@
 #include "launch.cuh"
 #include "paged_decode.cuh"
 #include "prompt_attn.cuh"
+#include "prompt_attn_f32.cuh"
 
 namespace fq {
 namespace {
@@ -26,7 +27,8 @@ inline int page_shift_of(int page_size) {
 inline bool stride_ok(int64_t stride, int heads, int head_dim, int act) {
   return stride >= (int64_t)heads * head_dim && stride * type_bytes(act) % 16 == 0;
 }
-constexpr int64_t kMaxRows = 0x7fffffff;
+constexpr int64_t kMaxRows = 0x7fffffff, kMaxPromptRows = 1 << 30;
+constexpr int kMaxHeads = 32767;  // q, k and v heads together are a grid dimension
 
 // f(activation type, cache type, head size) for one of the pairs the entries take
 template <typename A, typename C, typename F>
@@ -101,13 +103,25 @@ bool make_rows_map(const void* x, int64_t rows, int heads, int head_dim, int64_t
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+struct PromptArgs {
+  const void *q, *k, *v;
+  void* out;
+  const int* cu;
+  int64_t q_stride, k_stride, v_stride, n_rows;
+  int n_seqs, n_heads, n_kv;
+  float c;
+  uint8_t* workspace;
+};
 template <typename T, int kHd>
-int32_t launch_prompt(const PromptParams& p, const RowAttnParams& r, cudaStream_t stream) {
+int32_t launch_prompt(const PromptArgs& r, cudaStream_t stream) {
   using Cfg = PromptCfg<T, kHd>;
   static bool set[64] = {};
   const int sms = sm_count();
   auto kernel = prompt_attn_kernel<T, kHd>;
   if (sms == 0 || !allow_smem(kernel, Cfg::kSmem, set)) return kLaunchFailure;
+  PromptParams p = {};
+  p.out = r.out, p.cu = r.cu, p.n_rows = r.n_rows, p.n_items = prompt_slots(r.n_rows, r.n_seqs, kPaRows) * r.n_heads;
+  p.n_seqs = r.n_seqs, p.n_heads = r.n_heads, p.group = r.n_heads / r.n_kv, p.c = r.c;
   CUtensorMap qmap, kmap, vmap;
   if (!make_rows_map(r.q, r.n_rows, r.n_heads, kHd, r.q_stride, kPaTile, &qmap) ||
       !make_rows_map(r.k, r.n_rows, r.n_kv, kHd, r.k_stride, kPaTile, &kmap) ||
@@ -115,6 +129,53 @@ int32_t launch_prompt(const PromptParams& p, const RowAttnParams& r, cudaStream_
     return kLaunchFailure;
   const dim3 grid((unsigned)(p.n_items < sms ? p.n_items : sms));
   return launch(kernel, grid, dim3(kPaThreads), Cfg::kSmem, stream, p, qmap, kmap, vmap) == cudaSuccess ? kOk : kLaunchFailure;
+}
+
+// Workspace of the 32-bit form: the parts and powers of q, k and v; where each begins, and the whole
+struct PromptF32Workspace {
+  size_t q, k, v, q_up, kv_up, marked, bytes;
+};
+PromptF32Workspace prompt_f32_workspace(int64_t rows, int heads, int kv, int head_dim) {
+  PromptF32Workspace w;
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t begin = at;
+    at += align_up(n, 256);
+    return begin;
+  };
+  w.q = take((size_t)rows * heads * head_dim * 4);
+  w.k = take((size_t)rows * kv * head_dim * 4);
+  w.v = take((size_t)rows * kv * head_dim * 4);
+  w.q_up = take((size_t)rows * heads * sizeof(float));
+  w.kv_up = take((size_t)rows * kv * sizeof(float2));
+  w.marked = take((size_t)rows * kv * sizeof(int));
+  w.bytes = at;
+  return w;
+}
+template <int kHd>
+int32_t launch_prompt_f32(const PromptArgs& r, cudaStream_t stream) {
+  using Cfg = PromptF32Cfg<kHd>;
+  static bool set[64] = {};
+  const int sms = sm_count();
+  auto kernel = prompt_attn_f32_kernel<kHd>;
+  if (sms == 0 || !allow_smem(kernel, Cfg::kSmem, set)) return kLaunchFailure;
+  const PromptF32Workspace w = prompt_f32_workspace(r.n_rows, r.n_heads, r.n_kv, kHd);
+  const int64_t slots = prompt_slots(r.n_rows, r.n_seqs, kPaTile);
+  PromptF32Params p = {};
+  p.q = (const float*)r.q, p.k = (const float*)r.k, p.v = (const float*)r.v, p.out = (float*)r.out;
+  p.q_stride = r.q_stride, p.k_stride = r.k_stride, p.v_stride = r.v_stride, p.cu = r.cu, p.n_rows = r.n_rows;
+  p.n_items = slots * r.n_heads, p.n_seqs = r.n_seqs, p.n_heads = r.n_heads, p.n_kv = r.n_kv, p.group = r.n_heads / r.n_kv, p.c = r.c;
+  p.qp = (__half*)(r.workspace + w.q), p.kp = (__half*)(r.workspace + w.k), p.vp = (__half*)(r.workspace + w.v);
+  p.q_up = (float*)(r.workspace + w.q_up), p.kv_up = (float2*)(r.workspace + w.kv_up), p.marked = (int*)(r.workspace + w.marked);
+  CUtensorMap qmap, kmap, vmap;  // both parts in one map, the second behind the first
+  if (!make_rows_map(p.qp, 2 * r.n_rows, r.n_heads, kHd, (int64_t)r.n_heads * kHd, kPaTile, &qmap) ||
+      !make_rows_map(p.kp, 2 * r.n_rows, r.n_kv, kHd, (int64_t)r.n_kv * kHd, kPaTile, &kmap) ||
+      !make_rows_map(p.vp, 2 * r.n_rows, r.n_kv, kHd, (int64_t)r.n_kv * kHd, kPaTile, &vmap))
+    return kLaunchFailure;
+  cudaError_t e = launch(prompt_split_kernel<kHd>, dim3((unsigned)slots, (unsigned)(r.n_heads + 2 * r.n_kv)), dim3(256), 0, stream, p);
+  if (e != cudaSuccess) return kLaunchFailure;
+  const dim3 grid((unsigned)(p.n_items < sms ? p.n_items : sms));
+  return launch(kernel, grid, dim3(kPfaThreads), Cfg::kSmem, stream, p, qmap, kmap, vmap) == cudaSuccess ? kOk : kLaunchFailure;
 }
 
 inline int32_t status_of(cudaError_t e) { return e == cudaSuccess ? kOk : kLaunchFailure; }
@@ -189,7 +250,7 @@ int32_t fuelq_paged_attn_decode(int32_t act_type, int32_t cache_type, const void
   if (!type_pair(act_type, cache_type) || (head_dim != 64 && head_dim != 128)) return kNotSupported;
   const int shift = page_shift_of(page_size);
   if (shift < 0) return kNotSupported;
-  if (n_seqs < 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || !(scale >= 0.f) || std::isinf(scale) || n_pages < 0 || max_pages < 0) return kInvalidProblem;
+  if (n_seqs < 0 || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !(scale >= 0.f) || std::isinf(scale) || n_pages < 0 || max_pages < 0) return kInvalidProblem;
   if (n_seqs == 0) return kOk;
   if (!q || !kcache || !vcache || !out || !page_table || !seq_lens) return kInvalidProblem;
   if (!stride_ok(q_stride, n_heads, head_dim, act_type)) return kInvalidProblem;
@@ -211,8 +272,10 @@ int32_t fuelq_paged_attn_decode(int32_t act_type, int32_t cache_type, const void
 }
 
 size_t fuelq_prompt_attn_workspace_bytes(int32_t act_type, int64_t n_rows, int32_t n_heads, int32_t n_kv, int32_t head_dim) {
-  if (!type_bytes(act_type) || n_rows <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || (head_dim != 64 && head_dim != 128)) return 0;
-  return 0;
+  if (!type_bytes(act_type) || n_rows <= 0 || n_rows > kMaxPromptRows || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv ||
+      (head_dim != 64 && head_dim != 128))
+    return 0;
+  return act_type == kF32 ? prompt_f32_workspace(n_rows, n_heads, n_kv, head_dim).bytes : 0;
 }
 
 int32_t fuelq_prompt_attn(int32_t act_type, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
@@ -220,7 +283,7 @@ int32_t fuelq_prompt_attn(int32_t act_type, const void* q, int64_t q_stride, con
                           int32_t n_heads, int32_t n_kv, int32_t head_dim, float scale, void* workspace,
                           size_t workspace_bytes, void* stream) {
   if (!type_bytes(act_type) || (head_dim != 64 && head_dim != 128)) return kNotSupported;
-  if (n_seqs < 0 || n_rows < 0 || n_rows > kMaxRows || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || !(scale >= 0.f) || std::isinf(scale)) return kInvalidProblem;
+  if (n_seqs < 0 || n_rows < 0 || n_rows > kMaxPromptRows || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !(scale >= 0.f) || std::isinf(scale)) return kInvalidProblem;
   if (n_seqs == 0 || n_rows == 0) return kOk;
   if (!q || !k || !v || !out || !cu_seqlens) return kInvalidProblem;
   if (!stride_ok(q_stride, n_heads, head_dim, act_type) || !stride_ok(k_stride, n_kv, head_dim, act_type) ||
@@ -229,23 +292,14 @@ int32_t fuelq_prompt_attn(int32_t act_type, const void* q, int64_t q_stride, con
   const size_t need = fuelq_prompt_attn_workspace_bytes(act_type, n_rows, n_heads, n_kv, head_dim);
   if (need && (!workspace || workspace_bytes < need)) return kWorkspace;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(workspace)) return kMisaligned;
-  RowAttnParams p = {};
-  p.q = q, p.k = k, p.v = v, p.out = out, p.q_stride = q_stride, p.k_stride = k_stride, p.v_stride = v_stride, p.lens = cu_seqlens;
-  p.n_rows = n_rows, p.n_seqs = n_seqs, p.n_heads = n_heads, p.n_kv = n_kv, p.scale = scale;
-  if (act_type != kF32) {
-    PromptParams a = {};
-    a.out = out, a.cu = cu_seqlens, a.n_rows = n_rows, a.n_items = prompt_slots(n_rows, n_seqs) * n_heads;
-    a.n_seqs = n_seqs, a.n_heads = n_heads, a.group = n_heads / n_kv, a.c = scale * 1.4426950408889634f;
-    if (act_type == kF16)
-      return head_dim == 128 ? launch_prompt<__half, 128>(a, p, (cudaStream_t)stream) : launch_prompt<__half, 64>(a, p, (cudaStream_t)stream);
-    return head_dim == 128 ? launch_prompt<__nv_bfloat16, 128>(a, p, (cudaStream_t)stream)
-                           : launch_prompt<__nv_bfloat16, 64>(a, p, (cudaStream_t)stream);
-  }
-  const dim3 grid((unsigned)n_rows, (unsigned)n_heads);
-  return with_types(act_type, act_type, head_dim, [&](auto a, auto c, auto hd) {
-    return status_of(launch(row_attn_kernel<decltype(a), decltype(c), decltype(hd)::value, false>, grid, dim3(128), 0,
-                            (cudaStream_t)stream, p));
-  });
+  PromptArgs a = {};
+  a.q = q, a.k = k, a.v = v, a.out = out, a.cu = cu_seqlens, a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride;
+  a.n_rows = n_rows, a.n_seqs = n_seqs, a.n_heads = n_heads, a.n_kv = n_kv, a.c = scale * 1.4426950408889634f;
+  a.workspace = (uint8_t*)workspace;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (act_type == kF16) return head_dim == 128 ? launch_prompt<__half, 128>(a, st) : launch_prompt<__half, 64>(a, st);
+  if (act_type == kBF16) return head_dim == 128 ? launch_prompt<__nv_bfloat16, 128>(a, st) : launch_prompt<__nv_bfloat16, 64>(a, st);
+  return head_dim == 128 ? launch_prompt_f32<128>(a, st) : launch_prompt_f32<64>(a, st);
 }
 
 }  // extern "C"

@@ -149,93 +149,4 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
   }
 }
 
-// ---- attention of one row and one head at a time: the plain form of both operators -----------------
-struct RowAttnParams {
-  const void *q, *k, *v;  // k, v: the caches when paged
-  void* out;
-  int64_t q_stride, k_stride, v_stride;
-  const int *table, *lens;  // lens: seq_lens when paged, cu_seqlens otherwise
-  int64_t n_rows;
-  int n_seqs, n_heads, n_kv, page_shift, n_pages, max_pages;
-  float scale;
-};
-template <typename A, typename C, int kHd, bool kPaged>
-__global__ void __launch_bounds__(128) row_attn_kernel(const RowAttnParams p) {
-  constexpr int kPer = kHd / 32;
-  __shared__ float acc_s[4][kHd];
-  __shared__ float m_s[4], l_s[4];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int64_t row = blockIdx.x;
-  const int head = blockIdx.y, kvh = head / (p.n_heads / p.n_kv);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int64_t first = 0, n = 0;
-  bool bad = false;
-  if (kPaged) {
-    n = p.lens[row];
-    const int64_t most = (int64_t)p.max_pages << p.page_shift;
-    if (n > most) n = most, bad = true;
-    if (n < 0) n = 0;
-  } else {
-    int s = 0, e = p.n_seqs;  // the sequence that holds the row: the last one that starts at or before it
-    while (e - s > 1) {
-      const int mid = (s + e) >> 1;
-      if (p.lens[mid] <= row) s = mid; else e = mid;
-    }
-    first = p.lens[s];
-    const int64_t end = p.lens[s + 1];
-    if (first < 0 || end < first || end > p.n_rows) {
-      if (threadIdx.x == 0) record_dev_error(kErrIndex);
-      return;
-    }
-    if (row < first || row >= end) return;
-    n = row - first + 1;
-  }
-  const A* q = reinterpret_cast<const A*>(p.q) + row * p.q_stride + head * kHd + lane * kPer;
-  float qv[kPer], acc[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) qv[i] = to_f32(q[i]) * p.scale, acc[i] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  for (int64_t j = warp; j < n; j += 4) {
-    const C *kr, *vr;
-    if (kPaged) {
-      const int page = p.table[row * p.max_pages + (j >> p.page_shift)];
-      if (page < 0 || page >= p.n_pages) {
-        bad = true;
-        continue;
-      }
-      const int64_t at = ((((int64_t)page * p.n_kv + kvh) << p.page_shift) + (j & ((1 << p.page_shift) - 1))) * kHd;
-      kr = reinterpret_cast<const C*>(p.k) + at, vr = reinterpret_cast<const C*>(p.v) + at;
-    } else {
-      kr = reinterpret_cast<const C*>(p.k) + (first + j) * p.k_stride + kvh * kHd;
-      vr = reinterpret_cast<const C*>(p.v) + (first + j) * p.v_stride + kvh * kHd;
-    }
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) s += qv[i] * to_f32(kr[lane * kPer + i]);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    const float top = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.f : expf(m - top), e = s == -INFINITY ? 0.f : expf(s - top);
-    l = l * keep + e;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * keep + e * to_f32(vr[lane * kPer + i]);
-    m = top;
-  }
-  if (bad && lane == 0) record_dev_error(kErrIndex);
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) acc_s[warp][lane * kPer + i] = acc[i];
-  if (lane == 0) m_s[warp] = m, l_s[warp] = l;
-  __syncthreads();
-  if (threadIdx.x < kHd) {
-    float top = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3])), num = 0.f, den = 0.f;
-    for (int w = 0; w < 4; ++w) {
-      if (m_s[w] == -INFINITY) continue;
-      const float f = expf(m_s[w] - top);
-      num += f * acc_s[w][threadIdx.x], den += f * l_s[w];
-    }
-    reinterpret_cast<A*>(p.out)[(row * p.n_heads + head) * kHd + threadIdx.x] = from_f32<A>(den == 0.f ? 0.f : num / den);
-  }
-}
-
 }  // namespace fq

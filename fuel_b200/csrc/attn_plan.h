@@ -25,23 +25,22 @@ FQ_HD int seq_keys(int len, int max_pages, int page_shift) {
 }
 FQ_HD int seq_tiles(int len, int max_pages, int page_shift, int tile) { return (int)(((int64_t)seq_keys(len, max_pages, page_shift) + tile - 1) / tile); }
 
-// ---- prompts. An item is a block of kPromptRows rows of one sequence and one query head. Sequence s has the block numbers
-// ("slots") from prompt_slot(cu[s], s) up to the next sequence's: at least as many as it has blocks, without any sum over
-// the sequences before it; the few that are left over are empty.
-constexpr int kPromptRows = 256;
-FQ_HD int64_t prompt_slot(int64_t first_row, int seq) { return (first_row < 0 ? 0 : first_row / kPromptRows) + seq; }
-FQ_HD int64_t prompt_slots(int64_t n_rows, int n_seqs) { return n_rows / kPromptRows + n_seqs; }
+// ---- prompts. An item is a block of `rows` rows of one sequence and one query head. Sequence s has the block numbers ("slots")
+// from prompt_slot(cu[s], s) up to the next sequence's: at least as many as it has blocks, without any sum over the
+// sequences before it; the few that are left over are empty.
+FQ_HD int64_t prompt_slot(int64_t first_row, int seq, int rows) { return (first_row < 0 ? 0 : first_row / rows) + seq; }
+FQ_HD int64_t prompt_slots(int64_t n_rows, int n_seqs, int rows) { return n_rows / rows + n_seqs; }
 struct PromptBlock {
   int64_t first;  // first row of the sequence
   int len;        // its rows; -1: its boundaries are none
   int row;        // first row of the block within the sequence; >= len: empty
 };
 // The block of a slot. The blocks of a sequence come in descending order, the longest first.
-FQ_HD PromptBlock prompt_block(const int* cu, int n_seqs, int64_t n_rows, int64_t slot) {
+FQ_HD PromptBlock prompt_block(const int* cu, int n_seqs, int64_t n_rows, int64_t slot, int rows) {
   int lo = 0, hi = n_seqs;  // the last sequence whose slots begin at or before this one
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (prompt_slot(cu[mid], mid) <= slot) lo = mid; else hi = mid;
+    if (prompt_slot(cu[mid], mid, rows) <= slot) lo = mid; else hi = mid;
   }
   PromptBlock b;
   b.first = cu[lo];
@@ -51,8 +50,8 @@ FQ_HD PromptBlock prompt_block(const int* cu, int n_seqs, int64_t n_rows, int64_
     return b;
   }
   b.len = (int)(end - b.first);
-  const int64_t back = prompt_slot(end, lo + 1) - 1 - slot;  // 0 for the last slot of the sequence
-  const int64_t row = back * kPromptRows;
+  const int64_t back = prompt_slot(end, lo + 1, rows) - 1 - slot;  // 0 for the last slot of the sequence
+  const int64_t row = back * rows;
   b.row = back < 0 || row >= b.len ? b.len : (int)row;
   return b;
 }

@@ -10,8 +10,8 @@
 //   warps 0-3, 4-7  softmax of tile 0, 1: one thread per row. Reads S from tensor memory, writes P over it in the inputs' type,
 //                   which the second product reads from there; at the end divides and stores its rows
 //   warp 8          copies (TMA): Q tiles, and K and V tiles of 128 keys through one ring
-//   warp 9          (10 and 11 only make up its group of four) issues the MMAs: S of the next key tile goes out behind the product of the last, so the tensor cores have
-//                   work whenever one of the tiles is ready
+//   warp 9          issues the MMAs: S of the next key tile goes out behind the product of the last, so the tensor cores have
+//                   work whenever one of the tiles is ready; 10 and 11 only make up the group of four that gives registers away
 // Keys behind a row: the scores of the last key tile are masked. A value of NaN or infinity there would still reach earlier rows
 // as 0 x NaN, so the softmax warps take such values out of the last tile in shared memory and add them to the rows they
 // belong to at the end. Rows of the next sequence, or of nobody, that the last tile touches are taken out the same way.
@@ -31,7 +31,7 @@ struct PromptParams {
   int n_seqs, n_heads, group;
   float c;
 };
-constexpr int kPaThreads = 384, kPaTile = 128;
+constexpr int kPaThreads = 384, kPaTile = 128, kPaRows = 2 * kPaTile;
 // registers of a softmax thread (its row of S is 128 of them) and of the others: 256 x 208 + 128 x 80 of the launch's 384 x 168
 constexpr int kPaSoftmaxRegs = 208, kPaOtherRegs = 80;
 
@@ -73,6 +73,15 @@ __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t* r) {
         "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr)
       : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
@@ -162,7 +171,7 @@ struct PromptItem {
 __device__ __forceinline__ bool prompt_item(const PromptParams& p, int64_t x, PromptItem& it, bool& bad) {
   const int64_t slot = x / p.n_heads;
   it.head = (int)(x - slot * p.n_heads);
-  const PromptBlock b = prompt_block(p.cu, p.n_seqs, p.n_rows, slot);
+  const PromptBlock b = prompt_block(p.cu, p.n_seqs, p.n_rows, slot, kPaRows);
   bad = b.len < 0;
   if (b.row >= b.len) return false;
   it.first = b.first, it.len = b.len, it.row = b.row;
@@ -466,6 +475,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
               *reinterpret_cast<uint4*>(dst + 32 * i + e) = q;
             }
           }
+          __syncwarp();
         }
         tc_fence_before();
         if (t) mbar_arrive(&ctl->taken_free);

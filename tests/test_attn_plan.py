@@ -14,6 +14,12 @@ long long split_begin(long long total, int blocks, int b) { return fq::split_beg
 int split_block(long long total, int blocks, long long tile) { return fq::split_block(total, blocks, tile); }
 int split_slot(long long total, int blocks, int b, long long first) { return fq::split_slot(total, blocks, b, first); }
 int seq_keys(int len, int max_pages, int shift) { return fq::seq_keys(len, max_pages, shift); }
+struct Block { long long first; int len, row; };
+void prompt_block(const int* cu, int n, long long rows, long long slot, int size, Block* out) {
+  const fq::PromptBlock b = fq::prompt_block(cu, n, rows, slot, size);
+  out->first = b.first, out->len = b.len, out->row = b.row;
+}
+long long prompt_slots(long long rows, int n, int size) { return fq::prompt_slots(rows, n, size); }
 int seq_tiles(int len, int max_pages, int shift, int tile) { return fq::seq_tiles(len, max_pages, shift, tile); }
 }
 """
@@ -30,7 +36,47 @@ def plan(tmp_path_factory):
     lib.split_begin.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_int]
     lib.split_block.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_longlong]
     lib.split_slot.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_longlong]
+    lib.prompt_block.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p]
+    lib.prompt_slots.restype = ctypes.c_longlong
+    lib.prompt_slots.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_int]
     return lib
+
+
+class _Block(ctypes.Structure):
+    _fields_ = [("first", ctypes.c_longlong), ("len", ctypes.c_int), ("row", ctypes.c_int)]
+
+
+def _blocks(plan, cu, rows, size):
+    arr, out = (ctypes.c_int * len(cu))(*cu), []
+    for slot in range(plan.prompt_slots(rows, len(cu) - 1, size)):
+        b = _Block()
+        plan.prompt_block(arr, len(cu) - 1, rows, slot, size, ctypes.byref(b))
+        out.append((b.first, b.len, b.row))
+    return out
+
+
+def test_slots_hold_every_block_of_every_prompt_once(plan):
+    rng = random.Random(5)
+    for _ in range(400):
+        lens = [rng.choice((0, rng.randint(0, 4), 128 * rng.randint(0, 6), rng.randint(0, 2000))) for _ in range(rng.randint(1, 9))]
+        cu = [0]
+        for n in lens:
+            cu.append(cu[-1] + n)
+        for size in (128, 256):
+            got = _blocks(plan, cu, cu[-1] + rng.choice((0, 1, 300)), size)
+            full = [(f, r) for f, n, r in got if r < n]
+            assert len(full) == len(set(full)) == sum(-(-n // size) for n in lens)
+            for f in {f for f, _ in full}:                      # the longest block of a prompt first
+                rows = [r for g, r in full if g == f]
+                assert rows == sorted(rows, reverse=True) and rows[-1] == 0 and all(r % size == 0 for r in rows)
+
+
+def test_boundaries_that_are_none_are_seen(plan):
+    for cu in ([0, 20, 40, 90], [0, 20, 40, 30], [0, 20, 40, -3], [0, 20, 40, 2 ** 31 - 1]):
+        got = _blocks(plan, cu, 64, 256)
+        assert any(n == -1 for _, n, _ in got), cu
+        assert {(f, n) for f, n, r in got if n > 0 and r < n} == {(0, 20), (20, 20)}, cu
+    assert all(n == -1 for _, n, _ in _blocks(plan, [-5, 70], 64, 128))
 
 
 def test_runs_cover_the_tiles_and_know_their_block(plan):
