@@ -170,7 +170,7 @@ int32_t launch_prompt_f32(const PromptArgs& r, cudaStream_t stream) {
   CUtensorMap qmap, kmap, vmap;  // both parts in one map, the second behind the first
   if (!make_rows_map(p.qp, 2 * r.n_rows, r.n_heads, kHd, (int64_t)r.n_heads * kHd, kPaTile, &qmap) ||
       !make_rows_map(p.kp, 2 * r.n_rows, r.n_kv, kHd, (int64_t)r.n_kv * kHd, kPaTile, &kmap) ||
-      !make_rows_map(p.vp, 2 * r.n_rows, r.n_kv, kHd, (int64_t)r.n_kv * kHd, kPaTile, &vmap))
+      !make_rows_map(p.vp, 2 * r.n_rows, r.n_kv, kHd, (int64_t)r.n_kv * kHd, Cfg::kUnitKeys, &vmap))
     return kLaunchFailure;
   cudaError_t e = launch(prompt_split_kernel<kHd>, dim3((unsigned)slots, (unsigned)(r.n_heads + 2 * r.n_kv)), dim3(256), 0, stream, p);
   if (e != cudaSuccess) return kLaunchFailure;

@@ -4,20 +4,25 @@
 // f32: hi hi + lo hi + hi lo (lo lo is below 2^-22). f16 at three products is twice as fast as bf16 at the six that it would
 // take for as many bits, or tf32 at its half rate; what f16 lacks in range the powers of two give:
 //   q, k   one for each row and head: S = (Q' K'^T)_ij 2^(eq_i + ek_j)
-//   v      one for each row and head, put into the weight: with f_j the row's power, w_ij = 2^(s_ij + f_j - m'_i), m' the running
-//          maximum of s + f, so that w V' has f16's range whatever the rows' magnitudes; the sum of the softmax keeps p_ij =
-//          2^(s_ij - m_i) and its own running maximum, and out = (O / l) 2^(m' - m)
-// so no row loses bits to a larger one, in front of it or behind it. prompt_split_kernel writes the parts and powers (bound by
-// HBM: 4 bytes in, 4 out); values that are not finite are taken out of v there, and the tiles that had some are marked: the few
-// rows that see one add it again from the original at the end.
+//   v      one for each row and head, put into the weight: with f_j the row's power, w_ij = 2^(s_ij + f_j - m_i), m the maximum of
+//          s + f in the key tile, so that w V' has f16's range whatever the rows' magnitudes. sum_j w_ij 2^-f_j is the softmax's
+//          sum in the same unit as O = sum_j w_ij V'_j, so the result is their quotient
+// so no row loses bits to a larger one, in front of it or behind it, up to 2^100 apart (the powers of a tile of v are held within that of
+// its largest, and above 2^-80, for the sums' range). prompt_split_kernel writes the parts and powers (bound by HBM: 4 bytes in,
+// 4 out); values that are not finite are taken out of v there, and the tiles that had some are marked: the few rows that see
+// one add it again from the original at the end.
 // The tensor cores' f32 sums round towards zero, which over a long row adds up (1.6e-5 of it at 4000 keys). So they sum one
-// key tile at a time, and the tiles' results are added in registers, rounded to nearest.
+// key tile at a time, and the tiles' results are added in registers, rounded to nearest, each with its maximum: the softmax of a
+// tile needs nothing from the tile before, and two warpgroups take the tiles in turn.
 // Bound by the tensor cores: three times the 16-bit kernel's products. One tile of 128 query rows per thread block; S of the next
-// key tile is in tensor memory before the weights of this one are needed, so the softmax (two exponentials a score) and the
-// sums run beside the products.
-//   warps 0-3  softmax: a thread per row        warps 4-7  O: a thread per row adds the tiles' products, finishes and stores it
-//   warp 8     copies: the parts of Q, K and V, 32 KB each, through one ring
-//   warp 9     issues the MMAs                  warp 10    brings the powers of each key tile
+// key tile is in tensor memory before the weights of this one are needed, so softmax and sums run beside the products. K and
+// V come in units of 16 KB through a ring each, a tile long, and a product frees its units one by one: there is no room
+// for a second tile.
+//   warps 0-3, 4-7  softmax of every other key tile: a thread per row
+//   warps 8-11      O: a thread per row adds the tiles' products, finishes and stores it
+//   warps 12, 15    copies: the parts of Q and K, of V
+//   warp 13         issues the MMAs
+//   warp 14         brings the powers of each key tile
 #pragma once
 #include "prompt_attn.cuh"
 
@@ -56,30 +61,52 @@ __global__ void __launch_bounds__(256) prompt_split_kernel(const PromptF32Params
   __half* dst = kind == 0 ? p.qp : kind == 1 ? p.kp : p.vp;
   const int64_t plane = p.n_rows * heads * kHd;
   const int rows = min(kPaTile, b.len - b.row);
+  constexpr int kMine = kPaTile / 8;  // rows of a warp
+  alignas(16) float x[kMine][kPer];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const float* in = src + (b.first + b.row + warp + 8 * i) * stride + head * kHd + lane * kPer;
+    if (warp + 8 * i >= rows) {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) x[i][e] = 0.f;
+    } else if constexpr (kPer == 4) {
+      *reinterpret_cast<float4*>(x[i]) = *reinterpret_cast<const float4*>(in);
+    } else {
+      *reinterpret_cast<float2*>(x[i]) = *reinterpret_cast<const float2*>(in);
+    }
+  }
   bool odd = false;
-#pragma unroll 4
-  for (int i = warp; i < rows; i += 8) {
-    const int64_t row = b.first + b.row + i;
-    alignas(16) float x[kPer];
-    const float* in = src + row * stride + head * kHd + lane * kPer;
-    if constexpr (kPer == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(in);
-    else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(in);
+  int power[kMine], most = -1000;  // the largest value of a row comes to [2^14, 2^15)
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
     float top = 0.f;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      const bool fin = isfinite(x[e]);
-      if (fin) top = fmaxf(top, fabsf(x[e]));
-      if (kind == 2 && !fin) odd = true, x[e] = 0.f;
+      const bool fin = isfinite(x[i][e]);
+      if (fin) top = fmaxf(top, fabsf(x[i][e]));
+      if (kind == 2 && !fin) odd = true, x[i][e] = 0.f;
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    // the largest value comes to [2^14, 2^15); rows of nothing but denormals keep their lower bits out of f16's reach
-    const int e0 = top > 0.f ? max(ilogbf(top) - 14, -112) : 0;
+    power[i] = top > 0.f ? ilogbf(top) - 14 : -1000;
+    most = max(most, power[i]);
+  }
+  __shared__ int most_s[8];
+  if (lane == 0) most_s[warp] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) most = max(most, most_s[w]);
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    if (warp + 8 * i >= rows) break;
+    const int64_t row = b.first + b.row + warp + 8 * i;
+    // q, k: a row of zeros or nothing but denormals keeps a power in f32's range
+    const int e0 = kind == 2 ? max(power[i], max(most - 100, -80)) : max(power[i], -112);
     const float down = exp2f((float)-e0);
     alignas(8) __half hi[kPer], lo[kPer];
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      const float y = x[e] * down;
+      const float y = x[i][e] * down;
       hi[e] = __float2half_rn(y);
       lo[e] = isfinite(y) ? __float2half_rn(y - __half2float(hi[e])) : __ushort_as_half(0);
     }
@@ -95,7 +122,7 @@ __global__ void __launch_bounds__(256) prompt_split_kernel(const PromptF32Params
       const int64_t at = (int64_t)head * p.n_rows + row;
       if (kind == 0) p.q_up[at] = exp2f((float)e0) * p.c;
       else if (kind == 1) p.kv_up[at].x = exp2f((float)e0);
-      else p.kv_up[at].y = top > 0.f ? (float)e0 : -1e30f;  // a row of zeros weighs nothing in O
+      else p.kv_up[at].y = (float)e0;
     }
   }
   if (kind == 2) {
@@ -104,27 +131,29 @@ __global__ void __launch_bounds__(256) prompt_split_kernel(const PromptF32Params
   }
 }
 
-constexpr int kPfaThreads = 384;
-// registers: 128 threads of each, 128 x (240 + 176 + 88) of the launch's 384 x 168
-constexpr int kPfaSoftmaxRegs = 240, kPfaSumRegs = 176, kPfaOtherRegs = 88;
-constexpr int kPfaAhead = 4;  // steps and items that the softmax may be ahead of the sums (two, for the tensor memory; and their own)
+constexpr int kPfaThreads = 512;
+// registers of a softmax thread, of one that holds a row of O, of the others: 128 x (2 x 120 + 184 + 88) of the launch's 512 x 128
+constexpr int kPfaSoftmaxRegs = 120, kPfaSumRegs = 184, kPfaOtherRegs = 88;
+constexpr int kPfaAhead = 4;  // key tiles that the softmax may be ahead of the sums (two, for the tensor memory), and their own
 
-template <int kStages>
+constexpr int kPfaRing = 4;  // units of K, and of V
+
 struct PromptF32Ctl {
-  uint64_t q_full, q_empty, s_full[2], p_full, pv_full[2], pv_empty[2], up_full[2], up_empty[2];
-  uint64_t kv_full[kStages], kv_empty[kStages];
-  float keep[kPfaAhead][kPaTile];    // by step: what the row's reference has moved by
-  float2 finish[kPfaAhead][kPaTile]; // by item: what the row's O is multiplied by at the end
+  float2 stats[kPfaAhead][kPaTile];    // of a row: the maximum of s + f, the sum of w 2^-f
+  float4 up[2][kPaTile / 2];           // of two keys: 2^ek, 2^ek, f, f
+  float2 down[2][kPaTile / 2];         // 2^-f, 2^-f
+  uint64_t q_full, q_empty, s_full[2], p_full[2], pv_full, pv_empty, up_full[2], up_empty[2];
+  uint64_t k_full[kPfaRing], k_empty[kPfaRing], v_full[kPfaRing], v_empty[kPfaRing];
   uint32_t tmem_base;
   int abort_flag;
 };
 
 template <int kHd>
 struct PromptF32Cfg {
-  static constexpr int kStages = kHd == 128 ? 4 : 8;
   static constexpr int kTileBytes = kPaTile * kHd * 2;  // one part of a tile
-  static constexpr int kUpBytes = 2 * kPaTile * 8;
-  static constexpr int kSmem = 1024 + (2 + kStages) * kTileBytes + kUpBytes + (int)sizeof(PromptF32Ctl<kStages>) + 16;
+  static constexpr int kUnitBytes = kPaTile * 128;      // of K: 64 columns of a part; of V: kUnitKeys rows of a part
+  static constexpr int kUnits = kTileBytes / kUnitBytes, kUnitKeys = kPaTile / kUnits;
+  static constexpr int kSmem = 1024 + 2 * kTileBytes + 2 * kPfaRing * kUnitBytes + (int)sizeof(PromptF32Ctl) + 16;
 };
 
 // A row of the result whose key tiles hold values that are not finite: adds those that the row sees
@@ -150,22 +179,24 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
                                                                          const __grid_constant__ CUtensorMap kmap,
                                                                          const __grid_constant__ CUtensorMap vmap) {
   using Cfg = PromptF32Cfg<kHd>;
-  constexpr int kStages = Cfg::kStages, kTileBytes = Cfg::kTileBytes, kBoxes = kHd / 64, kBoxBytes = kPaTile * 128;
+  constexpr int kTileBytes = Cfg::kTileBytes, kUnitBytes = Cfg::kUnitBytes, kUnits = Cfg::kUnits, kUnitKeys = Cfg::kUnitKeys;
   extern __shared__ __align__(1024) uint8_t pfa_smem[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pfa_smem) + 1023) & ~(uintptr_t)1023);
-  const uint32_t q_addr = smem_u32(base), kv_addr = q_addr + 2 * kTileBytes;
-  float4* up_s = reinterpret_cast<float4*>(base + (2 + kStages) * kTileBytes);  // [2][64] pairs of keys: 2^ek, f of each
-  auto* ctl = reinterpret_cast<PromptF32Ctl<kStages>*>(base + (2 + kStages) * kTileBytes + Cfg::kUpBytes);
+  uint8_t* v_ring = base + 2 * kTileBytes + kPfaRing * kUnitBytes;
+  const uint32_t q_addr = smem_u32(base), k_addr = q_addr + 2 * kTileBytes, v_addr = smem_u32(v_ring);
+  auto* ctl = reinterpret_cast<PromptF32Ctl*>(v_ring + kPfaRing * kUnitBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(&ctl->q_full, 1), mbar_init(&ctl->q_empty, 1), mbar_init(&ctl->p_full, 128);
-    for (int i = 0; i < 2; ++i) mbar_init(&ctl->pv_full[i], 1), mbar_init(&ctl->pv_empty[i], 128);
-    for (int i = 0; i < 2; ++i) mbar_init(&ctl->s_full[i], 1), mbar_init(&ctl->up_full[i], 1), mbar_init(&ctl->up_empty[i], 128);
-    for (int s = 0; s < kStages; ++s) mbar_init(&ctl->kv_full[s], 1), mbar_init(&ctl->kv_empty[s], 1);
+    mbar_init(&ctl->q_full, 1), mbar_init(&ctl->q_empty, 1), mbar_init(&ctl->pv_full, 1), mbar_init(&ctl->pv_empty, 128);
+    for (int i = 0; i < 2; ++i) mbar_init(&ctl->s_full[i], 1), mbar_init(&ctl->p_full[i], 128), mbar_init(&ctl->up_full[i], 1), mbar_init(&ctl->up_empty[i], 128);
+    for (int s = 0; s < kPfaRing; ++s) {
+      mbar_init(&ctl->k_full[s], 1), mbar_init(&ctl->k_empty[s], 1);
+      mbar_init(&ctl->v_full[s], 1), mbar_init(&ctl->v_empty[s], 1);
+    }
     ctl->abort_flag = 0;
     mbar_init_fence();
   }
-  if (warp == 9) tmem_alloc(&ctl->tmem_base, 512);  // two S (the weights' two parts over each), two products
+  if (warp == 13) tmem_alloc(&ctl->tmem_base, 512);  // two S (the weights' upper parts over each), their lower parts, O of a tile
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -190,95 +221,108 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
     return true;
   };
 
-  if (warp >= 8) set_regs_down<kPfaOtherRegs>();
-  if (warp == 8) {
-    // ---------------- copies
+  const uint32_t p_low = tmem + 256, pv_acc = tmem + 384;
+
+  if (warp >= 12) set_regs_down<kPfaOtherRegs>();
+  if (warp == 12 || warp == 15) {
+    // ---------------- copies: Q and K, V. Units of a tile: upper part, lower part
     if (lane == 0) {
-      uint32_t unit = 0, items = 0;  // a unit: one part of a key or value tile
+      const bool values = warp == 15;
+      uint64_t* full = values ? ctl->v_full : ctl->k_full;
+      uint64_t* empty = values ? ctl->v_empty : ctl->k_empty;
+      uint32_t unit = 0, items = 0;
       bool ok = true;
       for (int64_t x = blockIdx.x; x < p.n_items && ok && !*abort_flag; x += gridDim.x) {
         Item it;
         if (!item(x, it)) continue;
         const int kvh = it.head / p.group;
-        if (items && !(ok = wait(&ctl->q_empty, items - 1, kErrEmptyWait))) break;
-        mbar_arrive_expect_tx(&ctl->q_full, 2 * kTileBytes);
-        for (int part = 0; part < 2; ++part)
-          for (int b = 0; b < kBoxes; ++b)
-            tma_load_3d(q_addr + part * kTileBytes + b * kBoxBytes, &qmap, 64 * b, it.head, (int)(part * p.n_rows + it.first + it.row), &ctl->q_full);
-        ++items;
+        if (!values) {
+          if (items && !(ok = wait(&ctl->q_empty, items - 1, kErrEmptyWait))) break;
+          mbar_arrive_expect_tx(&ctl->q_full, 2 * kTileBytes);
+          for (int part = 0; part < 2; ++part)
+            for (int b = 0; b < kUnits; ++b)
+              tma_load_3d(q_addr + part * kTileBytes + b * kUnitBytes, &qmap, 64 * b, it.head, (int)(part * p.n_rows + it.first + it.row), &ctl->q_full);
+          ++items;
+        }
         for (int j = 0; j < it.n && ok && !*abort_flag; ++j)
-          for (int u = 0; u < 4 && ok; ++u) {  // K hi, K lo, V hi, V lo
-            const uint32_t s = unit % kStages;
-            if (unit >= kStages && !(ok = wait(&ctl->kv_empty[s], unit / kStages - 1, kErrEmptyWait))) break;
-            mbar_arrive_expect_tx(&ctl->kv_full[s], kTileBytes);
-            for (int b = 0; b < kBoxes; ++b)
-              tma_load_3d(kv_addr + s * kTileBytes + b * kBoxBytes, u < 2 ? &kmap : &vmap, 64 * b, kvh,
-                          (int)((u & 1) * p.n_rows + it.first + j * kPaTile), &ctl->kv_full[s]);
-            ++unit;
+          for (int u = 0; u < 2 * kUnits && ok; ++u, ++unit) {
+            const uint32_t s = unit % kPfaRing;
+            if (unit >= kPfaRing && !(ok = wait(&empty[s], unit / kPfaRing - 1, kErrEmptyWait))) break;
+            mbar_arrive_expect_tx(&full[s], kUnitBytes);
+            const int row = (int)((u / kUnits) * p.n_rows + it.first + j * kPaTile), piece = u % kUnits;
+            if (!values) {
+              tma_load_3d(k_addr + s * kUnitBytes, &kmap, 64 * piece, kvh, row, &full[s]);
+            } else {
+              for (int b = 0; b < kHd / 64; ++b)
+                tma_load_3d(v_addr + s * kUnitBytes + b * kUnitKeys * 128, &vmap, 64 * b, kvh, row + piece * kUnitKeys, &full[s]);
+            }
           }
       }
       pdl_launch_dependents();
       if (*abort_flag) {  // leaving early: let the copies already requested land first
-        for (uint32_t u = unit > kStages ? unit - kStages : 0; u < unit; ++u)
-          if (!mbar_wait_bounded(&ctl->kv_full[u % kStages], (u / kStages) & 1)) record_dev_error(kErrDrainWait);
+        for (uint32_t u = unit > kPfaRing ? unit - kPfaRing : 0; u < unit; ++u)
+          if (!mbar_wait_bounded(&full[u % kPfaRing], (u / kPfaRing) & 1)) record_dev_error(kErrDrainWait);
         if (items && !mbar_wait_bounded(&ctl->q_full, (items - 1) & 1)) record_dev_error(kErrDrainWait);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == 13) {
     // ---------------- MMA issue: one thread
     if (lane == 0) {
       const uint32_t s_desc = umma_idesc_f16(kPaTile, kPaTile), o_desc = umma_idesc_f16(kPaTile, kHd) | kIdescBColumns;
-      uint32_t unit = 0, items = 0, steps = 0;
+      uint32_t items = 0, steps = 0;
       bool ok = true;
       for (int64_t x = blockIdx.x; x < p.n_items && ok && !*abort_flag; x += gridDim.x) {
         Item it;
         if (!item(x, it)) continue;
-        auto ready = [&](uint32_t u) { return wait(&ctl->kv_full[u % kStages], u / kStages, kErrFullWait); };
-        // S of key tile j into its half of tensor memory: hi hi, lo hi, hi lo
+        // S of key tile j into its half of tensor memory: hi hi and lo hi of each unit of the upper part, then hi lo
         auto scores = [&](int j) {
-          const uint32_t u = unit + 4 * j, d = tmem + ((steps + j) & 1) * kPaTile;
-          if (!ready(u)) return false;
-          tc_fence_after();
+          const uint32_t d = tmem + ((steps + j) & 1) * kPaTile;
 #pragma unroll
-          for (int part = 0; part < 3; ++part) {
-            if (part == 2 && !ready(u + 1)) return false;
-            if (part == 2) tc_fence_after();
-            const uint32_t a = q_addr + (part == 1 ? kTileBytes : 0), b = kv_addr + ((u + (part == 2)) % kStages) * kTileBytes;
+          for (int u = 0; u < 2 * kUnits; ++u) {
+            const uint32_t n = (steps + j) * 2 * kUnits + u, st = n % kPfaRing, b = k_addr + st * kUnitBytes;
+            if (!wait(&ctl->k_full[st], n / kPfaRing, kErrFullWait)) return false;
+            tc_fence_after();
 #pragma unroll
-            for (int k = 0; k < kHd / 16; ++k) {
-              const uint32_t off = (k / 4) * kBoxBytes + (k % 4) * 32;
-              umma_bf16(d, umma_desc_sw128(a + off), umma_desc_sw128(b + off), s_desc, (part | k) != 0);
+            for (int part = 0; part < (u < kUnits ? 2 : 1); ++part) {
+              const uint32_t a = q_addr + part * kTileBytes + (u % kUnits) * kUnitBytes;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) umma_bf16(d, umma_desc_sw128(a + k * 32), umma_desc_sw128(b + k * 32), s_desc, (u | part | k) != 0);
             }
-            if (part) umma_commit(&ctl->kv_empty[(u + part - 1) % kStages]);
+            umma_commit(&ctl->k_empty[st]);
           }
           if (j + 1 == it.n) umma_commit(&ctl->q_empty);
           umma_commit(&ctl->s_full[(steps + j) & 1]);
           return true;
         };
         if (!(ok = wait(&ctl->q_full, items++, kErrFullWait))) break;
+        tc_fence_after();
         ok = scores(0);
         for (int j = 0; j < it.n && ok; ++j) {
           if (j + 1 < it.n && !(ok = scores(j + 1))) break;
-          const uint32_t step = steps + j, d = tmem + 256 + (step & 1) * 128;
-          if (!(ok = wait(&ctl->p_full, step, kErrMmaWait))) break;
-          if (step >= 2 && !(ok = wait(&ctl->pv_empty[step & 1], step / 2 - 1, kErrTmemWait))) break;
-          const uint32_t u = unit + 4 * j + 2, w = tmem + ((steps + j) & 1) * kPaTile;
+          const uint32_t step = steps + j, hi = tmem + (step & 1) * kPaTile, lo = p_low + (step & 1) * 64;
+          if (!(ok = wait(&ctl->p_full[step & 1], step / 2, kErrMmaWait))) break;
+          if (step && !(ok = wait(&ctl->pv_empty, step - 1, kErrTmemWait))) break;
+          tc_fence_after();
 #pragma unroll
-          for (int part = 0; part < 3; ++part) {
-            if (part != 1 && !(ok = ready(u + part / 2))) break;
+          for (int u = 0; u < 2 * kUnits; ++u) {
+            const uint32_t n = step * 2 * kUnits + u, st = n % kPfaRing, b = v_addr + st * kUnitBytes;
+            if (!(ok = wait(&ctl->v_full[st], n / kPfaRing, kErrFullWait))) break;
             tc_fence_after();
-            const uint32_t b = kv_addr + ((u + part / 2) % kStages) * kTileBytes;
 #pragma unroll
-            for (int k = 0; k < kPaTile / 16; ++k)
-              umma_f16_ts(d, w + (part == 1 ? 64 : 0) + k * 8, umma_desc_sw128_mn(b + k * 2048, kBoxBytes), o_desc, (part | k) != 0);
-            if (part) umma_commit(&ctl->kv_empty[(u + part - 1) % kStages]);
+            for (int part = 0; part < (u < kUnits ? 2 : 1); ++part) {
+              const uint32_t a = (part ? lo : hi) + (u % kUnits) * (kUnitKeys / 2);
+#pragma unroll
+              for (int k = 0; k < kUnitKeys / 16; ++k)
+                umma_f16_ts(pv_acc, a + k * 8, umma_desc_sw128_mn(b + k * 2048, kUnitKeys * 128), o_desc, (u | part | k) != 0);
+            }
+            umma_commit(&ctl->v_empty[st]);
           }
-          if (ok) umma_commit(&ctl->pv_full[step & 1]);
+          if (ok) umma_commit(&ctl->pv_full);
         }
-        unit += 4 * it.n, steps += it.n;
+        steps += it.n;
       }
     }
-  } else if (warp == 10) {
+  } else if (warp == 14) {
     // ---------------- the powers of each key tile
     uint32_t steps = 0;
     bool ok = true;
@@ -288,139 +332,162 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
       const float2* src = p.kv_up + (int64_t)(it.head / p.group) * p.n_rows + it.first;
       for (int j = 0; j < it.n && ok; ++j, ++steps) {
         if (steps >= 2 && !(ok = __all_sync(0xffffffffu, wait(&ctl->up_empty[steps & 1], steps / 2 - 1, kErrEmptyWait)))) break;
-        float2* dst = reinterpret_cast<float2*>(up_s) + (steps & 1) * kPaTile;
+        float* up = reinterpret_cast<float*>(ctl->up[steps & 1]);
+        float* down = reinterpret_cast<float*>(ctl->down[steps & 1]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int key = j * kPaTile + i * 32 + lane;
-          dst[i * 32 + lane] = key < it.len ? src[key] : make_float2(0.f, 0.f);
+          const int at = i * 32 + lane, key = j * kPaTile + at;
+          const float2 u = key < it.len ? src[key] : make_float2(0.f, 0.f);
+          up[at / 2 * 4 + (at & 1)] = u.x, up[at / 2 * 4 + 2 + (at & 1)] = u.y;
+          down[at] = exp2f(-u.y);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl->up_full[steps & 1]);
       }
     }
-  } else if (warp < 4) {
-    // ---------------- softmax: a thread per row
-    set_regs_up<kPfaSoftmaxRegs>();
-    const int r = threadIdx.x;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    uint32_t unit = 0, steps = 0, items = 0;
+  } else if (warp < 8) {
+    // ---------------- softmax: a thread per row of every other key tile
+    set_regs_down<kPfaSoftmaxRegs>();
+    const uint32_t half = warp >> 2;
+    const int r = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + half * kPaTile, lo_addr = p_low + lanes + half * 64;
+    const uint32_t up = smem_u32(ctl->up[half]), down = smem_u32(ctl->down[half]);
+    uint32_t steps = 0;
     bool ok = true;
     for (int64_t x = blockIdx.x; x < p.n_items && ok; x += gridDim.x) {
       Item it;
       if (!item(x, it)) continue;
       const int row = it.row + r;
       const float cq = row < it.len ? p.q_up[(int64_t)it.head * p.n_rows + it.first + row] : 0.f;
-      float m = -INFINITY, ref = -INFINITY, sum = 0.f;  // running maxima of s and of s + f
-      for (int j = 0; j < it.n; ++j, ++steps) {
-        const uint32_t s_addr = tmem + lanes + (steps & 1) * kPaTile;
-        const float4* up = up_s + (steps & 1) * (kPaTile / 2);
-        ok = wait(&ctl->up_full[steps & 1], steps / 2, kErrFullWait) && wait(&ctl->s_full[steps & 1], steps / 2, kErrMmaWait);
+      const uint64_t cq2 = pair(cq, cq);
+      for (int j = (steps ^ half) & 1; j < it.n; j += 2) {
+        const uint32_t step = steps + j;
+        ok = wait(&ctl->up_full[half], step / 2, kErrFullWait) && wait(&ctl->s_full[half], step / 2, kErrMmaWait);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
-        uint32_t s[kPaTile];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32_nowait(s_addr + 32 * i, s + 32 * i);
-        tmem_wait_ld();
         const bool last = j + 1 == it.n;
-        float top[2] = {-INFINITY, -INFINITY}, topf[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < kPaTile; i += 2) {
-          const float4 u = up[i / 2];
-          float a = __uint_as_float(s[i]) * u.x * cq, b = __uint_as_float(s[i + 1]) * u.z * cq;
-          if (last && i > r) a = -INFINITY;
-          if (last && i + 1 > r) b = -INFINITY;
-          top[0] = fmaxf(top[0], a), top[1] = fmaxf(top[1], b);
-          topf[0] = fmaxf(topf[0], a + u.y), topf[1] = fmaxf(topf[1], b + u.w);
-          s[i] = __float_as_uint(a), s[i + 1] = __float_as_uint(b);
-        }
-        const float most = fmaxf(m, fmaxf(top[0], top[1])), mostf = fmaxf(ref, fmaxf(topf[0], topf[1]));
-        if (most != m) {
-          sum *= exp2f(m - most);
-          m = most;
-        }
-        ctl->keep[steps % kPfaAhead][r] = mostf == ref ? 1.f : exp2f(ref - mostf);
-        ref = mostf;
-        const float mm = m == -INFINITY ? 0.f : m, rr = (ref == -INFINITY ? 0.f : ref) - 14.f;  // weights up to 2^14
-        float part[2] = {0.f, 0.f};
-        uint32_t whi[32], wlo[32];
-#pragma unroll
-        for (int i = 0; i < kPaTile; i += 2) {
-          const float4 u = up[i / 2];
-          const float a = __uint_as_float(s[i]), b = __uint_as_float(s[i + 1]);
-          part[0] += exp2_approx(a - mm), part[1] += exp2_approx(b - mm);
-          const float wa = exp2_approx((a + u.y) - rr), wb = exp2_approx((b + u.w) - rr);
-          const uint32_t hi = cvt2<__half>(wa, wb);
-          const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-          whi[(i / 2) & 31] = hi;
-          wlo[(i / 2) & 31] = cvt2<__half>(wa - h.x, wb - h.y);
-          if (i % 64 == 62) {
-            tmem_st32(s_addr + (i / 64) * 32, whi);
-            tmem_st32(s_addr + 64 + (i / 64) * 32, wlo);
-          }
-        }
-        sum += part[0] + part[1];
-        mbar_arrive(&ctl->up_empty[steps & 1]);
-        if (last) {
-          // out = (O / l) 2^(m' - m); the weights had 2^14 more. In two steps, so that no power leaves f32's range before the
-          // product
-          const float f1 = exp2f(0.5f * ((ref == -INFINITY ? 0.f : ref) - mm - 14.f));
-          ctl->finish[items % kPfaAhead][r] = make_float2(f1, sum == 0.f ? 0.f : f1 / sum);
-          if (it.row + kPaTile > it.len) {
-            // the tile goes on behind the sequence: whatever stands there, 0 times it has to be 0. The products of the tile
-            // before are waited for first: then that tile's values had landed, and the parity below can only mean this one's
-            if (j && !(ok = __all_sync(0xffffffffu, wait(&ctl->pv_full[(steps - 1) & 1], (steps - 1) / 2, kErrMmaWait)))) break;
-            const int from = it.len - it.row;  // rows of the sequence in the tile
+        // the maximum, and again from tensor memory the weights: S is not held in registers. Sixteen columns at a time, the next
+        // sixteen on their way; rolled up, so that the loops stay in the instruction cache
+        uint32_t s[2][16];
+        float top[2] = {-INFINITY, -INFINITY};
+        auto look = [&](auto masked) {
+          tmem_ld16_nowait(s_addr, s[0]);
 #pragma unroll 1
-            for (int part_i = 0; part_i < 2 && ok; ++part_i) {
-              const uint32_t u = unit + 4 * j + 2 + part_i;
-              if (!(ok = __all_sync(0xffffffffu, wait(&ctl->kv_full[u % kStages], u / kStages, kErrFullWait)))) break;
-              uint8_t* v = base + (2 + u % kStages) * kTileBytes;
-              for (int i = from * 8 + r; i < kPaTile * 8; i += 128)
-                for (int b = 0; b < kBoxes; ++b) *reinterpret_cast<uint4*>(v + b * kBoxBytes + i * 16) = make_uint4(0, 0, 0, 0);
+          for (int c0 = 0; c0 < 8; c0 += 2) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = c0 + h;
+              tmem_wait_ld16(s[h]);
+              if (c < 7) tmem_ld16_nowait(s_addr + 16 * (c + 1), s[h ^ 1]);
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                const float4 w = lds_f4(up + (8 * c + i / 2) * 16);
+                float a, b;
+                unpair(fma2(pair(__uint_as_float(s[h][i]), __uint_as_float(s[h][i + 1])), mul2(pair(w.x, w.y), cq2), pair(w.z, w.w)), a, b);
+                if (decltype(masked)::value && c * 16 + i > r) a = -INFINITY;
+                if (decltype(masked)::value && c * 16 + i + 1 > r) b = -INFINITY;
+                top[0] = fmaxf(top[0], a), top[1] = fmaxf(top[1], b);
+              }
             }
-            if (!ok) break;
-            fence_proxy_async();
           }
+        };
+        if (last) look(std::true_type());
+        else look(std::false_type());
+        const float ref = fmaxf(top[0], top[1]), rr = 14.f - (ref == -INFINITY ? 0.f : ref);  // weights up to 2^14
+        const uint64_t rr2 = pair(rr, rr);
+        uint64_t sum2 = pair(0.f, 0.f);
+        auto weigh = [&](auto masked) {
+          tmem_ld16_nowait(s_addr, s[0]);
+#pragma unroll 1
+          for (int c0 = 0; c0 < 8; c0 += 2) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = c0 + h;
+              tmem_wait_ld16(s[h]);
+              if (c < 7) tmem_ld16_nowait(s_addr + 16 * (c + 1), s[h ^ 1]);
+              uint32_t hi[8], lo[8];
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                const float4 w = lds_f4(up + (8 * c + i / 2) * 16);
+                float a, b;
+                unpair(fma2(pair(__uint_as_float(s[h][i]), __uint_as_float(s[h][i + 1])), mul2(pair(w.x, w.y), cq2), add2(pair(w.z, w.w), rr2)), a, b);
+                if (decltype(masked)::value && c * 16 + i > r) a = -INFINITY;
+                if (decltype(masked)::value && c * 16 + i + 1 > r) b = -INFINITY;
+                a = exp2_approx(a), b = exp2_approx(b);
+                sum2 = fma2(pair(a, b), lds_pair(down + (8 * c + i / 2) * 8), sum2);
+                hi[i / 2] = cvt2<__half>(a, b);
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[i / 2]));
+                lo[i / 2] = cvt2<__half>(a - f.x, b - f.y);
+              }
+              // over columns of S that have been read: in front of the ones in flight
+              tmem_st8(s_addr + 8 * c, hi);
+              tmem_st8(lo_addr + 8 * c, lo);
+            }
+          }
+        };
+        if (last) weigh(std::true_type());
+        else weigh(std::false_type());
+        float a, b;
+        unpair(sum2, a, b);
+        ctl->stats[step % kPfaAhead][r] = make_float2(ref, a + b);
+        mbar_arrive(&ctl->up_empty[half]);
+        if (last && it.row + kPaTile > it.len) {
+          // the tile goes on behind the sequence: whatever stands there, 0 times it has to be 0. The products of the tile
+          // before are waited for first: then that tile's values had landed, and the parity below can only mean this one's
+          if (j && !(ok = __all_sync(0xffffffffu, wait(&ctl->pv_full, step - 1, kErrMmaWait)))) break;
+          const int from = it.len - it.row;  // rows of the sequence in the tile
+#pragma unroll 1
+          for (int u = 0; u < 2 * kUnits && ok; ++u) {
+            const uint32_t n = step * 2 * kUnits + u, st = n % kPfaRing;
+            if (!(ok = __all_sync(0xffffffffu, wait(&ctl->v_full[st], n / kPfaRing, kErrFullWait)))) break;
+            uint8_t* v = v_ring + st * kUnitBytes;
+            for (int i = max(from - (u % kUnits) * kUnitKeys, 0) * 8 + r; i < kUnitKeys * 8; i += 128)
+              for (int box = 0; box < kHd / 64; ++box) *reinterpret_cast<uint4*>(v + box * kUnitKeys * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+          }
+          if (!ok) break;
+          fence_proxy_async();
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&ctl->p_full);
+        mbar_arrive(&ctl->p_full[half]);
       }
-      unit += 4 * it.n;
-      ++items;
+      steps += it.n;
     }
-  } else if (warp < 8) {
+  } else if (warp < 12) {
     // ---------------- O: a thread per row
     set_regs_up<kPfaSumRegs>();
     const int r = threadIdx.x & 127;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    uint32_t steps = 0, items = 0;
+    const uint32_t addr = pv_acc + ((uint32_t)((warp & 3) * 32) << 16);
+    uint32_t steps = 0;
     bool ok = true;
     for (int64_t x = blockIdx.x; x < p.n_items && ok; x += gridDim.x) {
       Item it;
       if (!item(x, it)) continue;
-      float o[kHd];
+      float o[kHd], ref = -INFINITY, sum = 0.f;
 #pragma unroll
       for (int e = 0; e < kHd; ++e) o[e] = 0.f;
       for (int j = 0; j < it.n; ++j, ++steps) {
-        if (!(ok = __all_sync(0xffffffffu, wait(&ctl->pv_full[steps & 1], steps / 2, kErrMmaWait)))) break;
+        if (!(ok = __all_sync(0xffffffffu, wait(&ctl->pv_full, steps, kErrMmaWait)))) break;
         tc_fence_after();
-        const float keep = ctl->keep[steps % kPfaAhead][r];
-        const uint32_t addr = tmem + lanes + 256 + (steps & 1) * 128;
+        const float2 st = ctl->stats[steps % kPfaAhead][r];
+        const float to = fmaxf(ref, st.x), keep = ref == to ? 1.f : exp2f(ref - to), take = st.x == to ? 1.f : exp2f(st.x - to);
+        ref = to;
+        sum = sum * keep + st.y * take;
 #pragma unroll
         for (int i = 0; i < kHd / 16; ++i) {
           uint32_t v[16];
           tmem_ld16(addr + 16 * i, v);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[16 * i + e] = fmaf(o[16 * i + e], keep, __uint_as_float(v[e]));
+          for (int e = 0; e < 16; ++e) o[16 * i + e] = fmaf(o[16 * i + e], keep, __uint_as_float(v[e]) * take);
         }
         tc_fence_before();
-        mbar_arrive(&ctl->pv_empty[steps & 1]);
+        mbar_arrive(&ctl->pv_empty);
       }
       if (!ok) break;
       const int row = it.row + r;
       const int64_t rows_at = (int64_t)(it.head / p.group) * p.n_rows + it.first;
-      const float2 f = ctl->finish[items % kPfaAhead][r];
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
       bool odd = false;
       for (int j = lane; j < it.n; j += 32) odd |= p.marked[rows_at + (int64_t)j * kPaTile] != 0;
       odd = __any_sync(0xffffffffu, odd);
@@ -428,16 +495,15 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
         float* dst = p.out + ((it.first + row) * p.n_heads + it.head) * kHd;
 #pragma unroll
         for (int e = 0; e < kHd; e += 4)
-          *reinterpret_cast<float4*>(dst + e) = make_float4(o[e] * f.x * f.y, o[e + 1] * f.x * f.y, o[e + 2] * f.x * f.y, o[e + 3] * f.x * f.y);
+          *reinterpret_cast<float4*>(dst + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
         if (odd) add_not_finite<kHd>(p, it.first, row, it.head, dst);
       }
       __syncwarp();
-      ++items;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == 13) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace fq
