@@ -173,6 +173,14 @@ __device__ __forceinline__ uint32_t cvt2<__nv_bfloat16>(float a, float b) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   return r;
 }
+// one lane of the warp, in a form that lets the compiler keep what the MMAs take (descriptors, addresses) in uniform registers: the
+// whole warp runs the issuing role and only the instructions themselves are this lane's. With the role in a branch of one
+// lane an MMA took 125 cycles to issue, twice what it runs
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0;
+}
 template <int kRegs>
 __device__ __forceinline__ void set_regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 template <int kRegs>
@@ -316,61 +324,68 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
       }
     }
   } else if (warp == 9) {
-    // ---------------- MMA issue: one thread
-    if (lane == 0) {
-      constexpr bool kF16 = std::is_same<T, __half>::value;
-      const uint32_t s_desc = kF16 ? umma_idesc_f16(kPaTile, kPaTile) : umma_idesc_bf16(kPaTile, kPaTile);
-      const uint32_t o_desc = (kF16 ? umma_idesc_f16(kPaTile, kHd) : umma_idesc_bf16(kPaTile, kHd)) | kIdescBColumns;
-      uint32_t unit = 0, tiles[2] = {0, 0}, steps[2] = {0, 0};  // steps: key tiles of each row tile so far
-      bool ok = true;
-      for (int64_t x = blockIdx.x; x < p.n_items && ok && !*abort_flag; x += gridDim.x) {
-        PromptItem it;
-        bool bad;
-        if (!prompt_item(p, x, it, bad)) continue;
-        const int n = it.n1 ? it.n1 : it.n0, nt[2] = {it.n0, it.n1};
-        auto stage = [&](int j, bool value) { return (unit + 2 * j + value) % kStages; };
-        auto kv_ready = [&](int j, bool value) {
-          return wait(&ctl->kv_full[stage(j, value)], (unit + 2 * j + value) / kStages, kErrFullWait);
-        };
-        auto scores = [&](int t, int j) {
+    // ---------------- MMA issue
+    constexpr bool kF16 = std::is_same<T, __half>::value;
+    constexpr uint32_t s_desc = kF16 ? umma_idesc_f16(kPaTile, kPaTile) : umma_idesc_bf16(kPaTile, kPaTile);
+    constexpr uint32_t o_desc = (kF16 ? umma_idesc_f16(kPaTile, kHd) : umma_idesc_bf16(kPaTile, kHd)) | kIdescBColumns;
+    const uint32_t acc = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t q_desc = umma_desc_sw128(q_addr), k_desc = umma_desc_sw128(kv_addr), v_desc = umma_desc_sw128_mn(kv_addr, kBoxBytes);
+    const bool leader = elect_one();
+    auto ready = [&](uint64_t* bar, uint32_t parity, int code) { return (bool)__all_sync(0xffffffffu, wait(bar, parity, code)); };
+    uint32_t unit = 0, tiles[2] = {0, 0}, steps[2] = {0, 0};  // steps: key tiles of each row tile so far
+    bool ok = true;
+    for (int64_t x = blockIdx.x; x < p.n_items && ok; x += gridDim.x) {
+      PromptItem it;
+      bool bad;
+      if (!prompt_item(p, x, it, bad)) continue;
+      const int n = it.n1 ? it.n1 : it.n0, nt[2] = {it.n0, it.n1};
+      auto stage = [&](int j, bool value) { return (unit + 2 * j + value) % kStages; };
+      auto kv_ready = [&](int j, bool value) { return ready(&ctl->kv_full[stage(j, value)], (unit + 2 * j + value) / kStages, kErrFullWait); };
+      auto scores = [&](int t, int j) {
+        const uint64_t a = q_desc + (uint64_t)(t * kTileBytes >> 4), b = k_desc + (uint64_t)(stage(j, false) * kTileBytes >> 4);
+        if (leader) {
           tc_fence_after();
-          const uint32_t a = q_addr + t * kTileBytes, b = kv_addr + stage(j, false) * kTileBytes;
 #pragma unroll
           for (int k = 0; k < kHd / 16; ++k) {
-            const uint32_t off = (k / 4) * kBoxBytes + (k % 4) * 32;
-            umma_bf16(tmem + t * kPaTile, umma_desc_sw128(a + off), umma_desc_sw128(b + off), s_desc, k != 0);
+            const uint64_t off = ((k / 4) * kBoxBytes + (k % 4) * 32) >> 4;
+            umma_bf16(acc + t * kPaTile, a + off, b + off, s_desc, k != 0);
           }
           umma_commit(&ctl->s_full[t]);
           if (j + 1 == nt[t]) umma_commit(&ctl->q_empty[t]);
-        };
-        ok = kv_ready(0, false);
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (!nt[t]) continue;
-          ok = wait(&ctl->q_full[t], tiles[t]++, kErrFullWait);
-          if (ok) scores(t, 0);
         }
-        if (ok) umma_commit(&ctl->kv_empty[stage(0, false)]);
-        for (int j = 0; j < n && ok; ++j) {
-          if (!(ok = kv_ready(j, true))) break;
-          if (j + 1 < n && !(ok = kv_ready(j + 1, false))) break;
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (j >= nt[t]) continue;
-            if (!(ok = wait(&ctl->p_full[t], steps[t]++, kErrMmaWait))) break;
+      };
+      ok = kv_ready(0, false);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (!ok || !nt[t]) continue;
+        ok = ready(&ctl->q_full[t], tiles[t]++, kErrFullWait);
+        if (ok) scores(t, 0);
+      }
+      if (ok && leader) umma_commit(&ctl->kv_empty[stage(0, false)]);
+      for (int j = 0; j < n && ok; ++j) {
+        if (!(ok = kv_ready(j, true))) break;
+        if (j + 1 < n && !(ok = kv_ready(j + 1, false))) break;
+        const uint64_t b = v_desc + (uint64_t)(stage(j, true) * kTileBytes >> 4);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!ok || j >= nt[t]) continue;
+          if (!(ok = ready(&ctl->p_full[t], steps[t]++, kErrMmaWait))) continue;
+          if (leader) {
             tc_fence_after();
-            const uint32_t b = kv_addr + stage(j, true) * kTileBytes;
 #pragma unroll
             for (int k = 0; k < kPaTile / 16; ++k)
-              umma_f16_ts(tmem + 256 + t * 128, tmem + t * kPaTile + k * 8, umma_desc_sw128_mn(b + k * 2048, kBoxBytes), o_desc, (j | k) != 0);
-            if (j + 1 < nt[t]) scores(t, j + 1);
-            else if (j + 1 < n) umma_commit(&ctl->o_full[t]);
+              umma_f16_ts(acc + 256 + t * 128, acc + t * kPaTile + k * 8, b + (uint64_t)(k * 2048 >> 4), o_desc, (j | k) != 0);
           }
-          if (!ok) break;
+          if (j + 1 < nt[t]) scores(t, j + 1);
+          else if (j + 1 < n && leader) umma_commit(&ctl->o_full[t]);
+        }
+        if (ok && leader) {
           umma_commit(&ctl->kv_empty[stage(j, true)]);
           if (j + 1 < n) umma_commit(&ctl->kv_empty[stage(j + 1, false)]);
           else umma_commit(&ctl->o_full[it.n1 ? 1 : 0]);  // last of all: nothing of this block arrives after its results are read
         }
-        unit += 2 * n;
       }
+      unit += 2 * n;
     }
   } else if (warp < 8) {
     // ---------------- softmax: a thread per row of tile t

@@ -266,61 +266,66 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
       }
     }
   } else if (warp == 13) {
-    // ---------------- MMA issue: one thread
-    if (lane == 0) {
-      const uint32_t s_desc = umma_idesc_f16(kPaTile, kPaTile), o_desc = umma_idesc_f16(kPaTile, kHd) | kIdescBColumns;
-      uint32_t items = 0, steps = 0;
-      bool ok = true;
-      for (int64_t x = blockIdx.x; x < p.n_items && ok && !*abort_flag; x += gridDim.x) {
-        Item it;
-        if (!item(x, it)) continue;
-        // S of key tile j into its half of tensor memory: hi hi and lo hi of each unit of the upper part, then hi lo
-        auto scores = [&](int j) {
-          const uint32_t d = tmem + ((steps + j) & 1) * kPaTile;
+    // ---------------- MMA issue
+    constexpr uint32_t s_desc = umma_idesc_f16(kPaTile, kPaTile), o_desc = umma_idesc_f16(kPaTile, kHd) | kIdescBColumns;
+    const uint32_t acc = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t q_desc = umma_desc_sw128(q_addr), k_desc = umma_desc_sw128(k_addr), v_desc = umma_desc_sw128_mn(v_addr, kUnitKeys * 128);
+    const bool leader = elect_one();
+    auto ready = [&](uint64_t* bar, uint32_t parity, int code) { return (bool)__all_sync(0xffffffffu, wait(bar, parity, code)); };
+    uint32_t items = 0, steps = 0;
+    bool ok = true;
+    for (int64_t x = blockIdx.x; x < p.n_items && ok; x += gridDim.x) {
+      Item it;
+      if (!item(x, it)) continue;
+      // S of key tile j into its half of tensor memory: hi hi and lo hi of each unit of the upper part, then hi lo
+      auto scores = [&](int j) {
+        const uint32_t d = acc + ((steps + j) & 1) * kPaTile;
 #pragma unroll
-          for (int u = 0; u < 2 * kUnits; ++u) {
-            const uint32_t n = (steps + j) * 2 * kUnits + u, st = n % kPfaRing, b = k_addr + st * kUnitBytes;
-            if (!wait(&ctl->k_full[st], n / kPfaRing, kErrFullWait)) return false;
+        for (int u = 0; u < 2 * kUnits; ++u) {
+          const uint32_t n = (steps + j) * 2 * kUnits + u, st = n % kPfaRing;
+          if (!ready(&ctl->k_full[st], n / kPfaRing, kErrFullWait)) return false;
+          const uint64_t b = k_desc + (uint64_t)(st * kUnitBytes >> 4);
+          if (leader) {
             tc_fence_after();
 #pragma unroll
-            for (int part = 0; part < (u < kUnits ? 2 : 1); ++part) {
-              const uint32_t a = q_addr + part * kTileBytes + (u % kUnits) * kUnitBytes;
+            for (int part = 0; part < (u < kUnits ? 2 : 1); ++part)
 #pragma unroll
-              for (int k = 0; k < 4; ++k) umma_bf16(d, umma_desc_sw128(a + k * 32), umma_desc_sw128(b + k * 32), s_desc, (u | part | k) != 0);
-            }
+              for (int k = 0; k < 4; ++k)
+                umma_bf16(d, q_desc + (uint64_t)((part * kTileBytes + (u % kUnits) * kUnitBytes + k * 32) >> 4), b + 2 * k, s_desc, (u | part | k) != 0);
             umma_commit(&ctl->k_empty[st]);
           }
+        }
+        if (leader) {
           if (j + 1 == it.n) umma_commit(&ctl->q_empty);
           umma_commit(&ctl->s_full[(steps + j) & 1]);
-          return true;
-        };
-        if (!(ok = wait(&ctl->q_full, items++, kErrFullWait))) break;
-        tc_fence_after();
-        ok = scores(0);
-        for (int j = 0; j < it.n && ok; ++j) {
-          if (j + 1 < it.n && !(ok = scores(j + 1))) break;
-          const uint32_t step = steps + j, hi = tmem + (step & 1) * kPaTile, lo = p_low + (step & 1) * 64;
-          if (!(ok = wait(&ctl->p_full[step & 1], step / 2, kErrMmaWait))) break;
-          if (step && !(ok = wait(&ctl->pv_empty, step - 1, kErrTmemWait))) break;
-          tc_fence_after();
+        }
+        return true;
+      };
+      if (!(ok = ready(&ctl->q_full, items++, kErrFullWait))) break;
+      ok = scores(0);
+      for (int j = 0; j < it.n && ok; ++j) {
+        if (j + 1 < it.n && !(ok = scores(j + 1))) break;
+        const uint32_t step = steps + j, hi = acc + (step & 1) * kPaTile, lo = acc + 256 + (step & 1) * 64, d = acc + 384;
+        if (!(ok = ready(&ctl->p_full[step & 1], step / 2, kErrMmaWait))) break;
+        if (step && !(ok = ready(&ctl->pv_empty, step - 1, kErrTmemWait))) break;
 #pragma unroll
-          for (int u = 0; u < 2 * kUnits; ++u) {
-            const uint32_t n = step * 2 * kUnits + u, st = n % kPfaRing, b = v_addr + st * kUnitBytes;
-            if (!(ok = wait(&ctl->v_full[st], n / kPfaRing, kErrFullWait))) break;
+        for (int u = 0; u < 2 * kUnits; ++u) {
+          const uint32_t n = step * 2 * kUnits + u, st = n % kPfaRing;
+          if (ok) ok = ready(&ctl->v_full[st], n / kPfaRing, kErrFullWait);
+          const uint64_t b = v_desc + (uint64_t)(st * kUnitBytes >> 4);
+          if (ok && leader) {
             tc_fence_after();
 #pragma unroll
-            for (int part = 0; part < (u < kUnits ? 2 : 1); ++part) {
-              const uint32_t a = (part ? lo : hi) + (u % kUnits) * (kUnitKeys / 2);
+            for (int part = 0; part < (u < kUnits ? 2 : 1); ++part)
 #pragma unroll
               for (int k = 0; k < kUnitKeys / 16; ++k)
-                umma_f16_ts(pv_acc, a + k * 8, umma_desc_sw128_mn(b + k * 2048, kUnitKeys * 128), o_desc, (u | part | k) != 0);
-            }
+                umma_f16_ts(d, (part ? lo : hi) + (u % kUnits) * (kUnitKeys / 2) + k * 8, b + (uint64_t)(k * 2048 >> 4), o_desc, (u | part | k) != 0);
             umma_commit(&ctl->v_empty[st]);
           }
-          if (ok) umma_commit(&ctl->pv_full);
         }
-        steps += it.n;
+        if (ok && leader) umma_commit(&ctl->pv_full);
       }
+      steps += it.n;
     }
   } else if (warp == 14) {
     // ---------------- the powers of each key tile
