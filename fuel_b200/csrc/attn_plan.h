@@ -35,25 +35,29 @@ struct PromptBlock {
   int len;        // its rows; -1: its boundaries are none
   int row;        // first row of the block within the sequence; >= len: empty
 };
-// The block of a slot. The blocks of a sequence come in descending order, the longest first.
-FQ_HD PromptBlock prompt_block(const int* cu, int n_seqs, int64_t n_rows, int64_t slot, int rows) {
-  int lo = 0, hi = n_seqs;  // the last sequence whose slots begin at or before this one
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (prompt_slot(cu[mid], mid, rows) <= slot) lo = mid; else hi = mid;
-  }
+// The block of a slot that is one of sequence s. The blocks of a sequence come in descending order, the longest first.
+FQ_HD PromptBlock prompt_block_of(const int* cu, int s, int64_t n_rows, int64_t slot, int rows) {
   PromptBlock b;
-  b.first = cu[lo];
-  const int64_t end = cu[lo + 1];
+  b.first = cu[s];
+  const int64_t end = cu[s + 1];
   if (b.first < 0 || end < b.first || end > n_rows) {
     b.len = -1, b.row = 0;
     return b;
   }
   b.len = (int)(end - b.first);
-  const int64_t back = prompt_slot(end, lo + 1, rows) - 1 - slot;  // 0 for the last slot of the sequence
+  const int64_t back = prompt_slot(end, s + 1, rows) - 1 - slot;  // 0 for the last slot of the sequence
   const int64_t row = back * rows;
   b.row = back < 0 || row >= b.len ? b.len : (int)row;
   return b;
+}
+// The same, the sequence (the last whose slots begin at or before this one) looked for
+FQ_HD PromptBlock prompt_block(const int* cu, int n_seqs, int64_t n_rows, int64_t slot, int rows) {
+  int lo = 0, hi = n_seqs;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prompt_slot(cu[mid], mid, rows) <= slot) lo = mid; else hi = mid;
+  }
+  return prompt_block_of(cu, lo, n_rows, slot, rows);
 }
 
 }  // namespace fq

@@ -11,7 +11,8 @@
 //                   which the second product reads from there; at the end divides and stores its rows
 //   warp 8          copies (TMA): Q tiles, and K and V tiles of 128 keys through one ring
 //   warp 9          issues the MMAs: S of the next key tile goes out behind the product of the last, so the tensor cores have
-//                   work whenever one of the tiles is ready; 10 and 11 only make up the group of four that gives registers away
+//                   work whenever one of the tiles is ready
+//   warp 10         finds the block's items ahead of the others (11 only makes up the group of four that gives registers away)
 // Keys behind a row: the scores of the last key tile are masked. A value of NaN or infinity there would still reach earlier rows
 // as 0 x NaN, so the softmax warps take such values out of the last tile in shared memory and add them to the rows they
 // belong to at the end. Rows of the next sequence, or of nobody, that the last tile touches are taken out the same way.
@@ -137,6 +138,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// the largest of three, NaN if one is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // two f32 at a time
 __device__ __forceinline__ uint64_t pair(float a, float b) {
   uint64_t r;
@@ -158,6 +165,24 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+// 2^x of two values on the multiply-add pipes: x = n + f with n the nearest integer, found by adding 1.5 2^23, 2^f by a polynomial of
+// degree four (fitted to the least relative error over [-1/2, 1/2]: 2.6e-6), n added to its exponent. Below 2^-126: some
+// denormal. NaN does not pass
+__device__ __forceinline__ void exp2_poly2(uint64_t x, float& a, float& b) {
+  unpair(x, a, b);
+  x = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const uint64_t magic = pair(12582912.f, 12582912.f), t = add2(x, magic);
+  const uint64_t f = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), x);
+  uint64_t y = fma2(f, pair(0x1.3997d4p-7f, 0x1.3997d4p-7f), pair(0x1.ca1442p-5f, 0x1.ca1442p-5f));
+  y = fma2(y, f, pair(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+  y = fma2(y, f, pair(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+  y = fma2(y, f, pair(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  float ta, tb;
+  unpair(t, ta, tb);
+  unpair(y, a, b);
+  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23));
+  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
 }
 template <typename T>
 __device__ __forceinline__ uint32_t cvt2(float a, float b);
@@ -185,11 +210,36 @@ template <int kRegs>
 __device__ __forceinline__ void set_regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 template <int kRegs>
 __device__ __forceinline__ void set_regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
-// is one of the two 16-bit values an infinity or NaN?
+// bit 15 or 31 of the result: the value below it is an infinity or NaN (its exponent, all ones, overflows by one more)
 template <typename T>
-__device__ __forceinline__ bool not_finite2(uint32_t w) {
-  const uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  return (w & e) == e || ((w >> 16) & e) == e;
+__device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
+  return (w & 0x7fff7fffu) + (std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u);
+}
+__device__ __forceinline__ uint4 lds_u4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts_u4(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// A warp's 32 rows, 64 bytes of each in its lane's registers, to memory: turned round in shared memory so that four lanes write a
+// row's 64 bytes together (a lane by itself would touch 32 lines with every store: the epilogue was 6000 cycles long). rows: how
+// many of them there are
+constexpr int kStageRow = 80, kStageBytes = 32 * kStageRow;  // 80: eight rows in eight different 16-byte columns of the banks
+__device__ __forceinline__ void store_rows64(uint32_t stage, int lane, const uint4 (&v)[4], uint8_t* dst, int64_t row_bytes, int rows) {
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sts_u4(stage + lane * kStageRow + 16 * i, v[i]);
+  __syncwarp();
+  dst += (lane >> 2) * row_bytes + 16 * (lane & 3);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 8 * i + (lane >> 2);
+    const uint4 q = lds_u4(stage + row * kStageRow + 16 * (lane & 3));
+    if (row < rows) *reinterpret_cast<uint4*>(dst + 8 * i * row_bytes) = q;
+  }
 }
 
 // Values taken out of a tile of values, by column: the first of its rows that holds +inf, -inf, NaN. Records carry the number of
@@ -203,39 +253,88 @@ __device__ __forceinline__ uint32_t taken_word(uint32_t item, int row) { return 
 // the row of a record, or a row behind all others if it is not of this item
 __device__ __forceinline__ int taken_row(uint32_t word, uint32_t item) { return word >> 8 == 0xffffffu - item ? (int)(word & 0xff) : 0x100; }
 
+// The items of a thread block are found by a warp of their own and handed to the others through a ring: the search (dependent loads,
+// a division) is 2700 cycles long, which every role had between two items before
+struct PromptItem {
+  int64_t first;  // first row of the sequence
+  int len;        // its rows; -1: there are no more items
+  int row, head;  // first row of the block within the sequence
+  int n;          // key tiles of the block's first 128 rows
+};
+constexpr int kItemRing = 4;
+struct ItemRing {
+  uint64_t full[kItemRing], empty[kItemRing];
+  PromptItem item[kItemRing];
+};
+// The next item from x on (in steps of the grid) whose block has rows; the whole warp looks
+__device__ __forceinline__ PromptItem find_item(const int* cu, int n_seqs, int64_t n_rows, int n_heads, int64_t n_items, int rows, int64_t& x, int lane) {
+  PromptItem it;
+  for (; x < n_items; x += gridDim.x) {
+    const int64_t slot = x / n_heads;
+    int lo = 0, hi = n_seqs;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+      const uint32_t before = __ballot_sync(0xffffffffu, at < hi && prompt_slot(cu[at], at, rows) <= slot);
+      lo += max(__popc(before) - 1, 0) * step;
+      hi = min(lo + step, hi);
+    }
+    const PromptBlock b = prompt_block_of(cu, lo, n_rows, slot, rows);
+    if (b.len < 0 && lane == 0) record_dev_error(kErrIndex);
+    if (b.row >= b.len) continue;
+    it.first = b.first, it.len = b.len, it.row = b.row, it.head = (int)(x - slot * n_heads), it.n = b.row / kPaTile + 1;
+    x += gridDim.x;
+    return it;
+  }
+  it.first = 0, it.len = -1, it.row = it.head = it.n = 0;
+  return it;
+}
+// the n-th item into the ring; false if its place was not free in time
+template <typename Wait>
+__device__ __forceinline__ bool put_item(ItemRing& ring, uint32_t n, const PromptItem& it, int lane, Wait& wait) {
+  const uint32_t s = n % kItemRing;
+  if (n >= kItemRing && !__all_sync(0xffffffffu, wait(&ring.empty[s], n / kItemRing - 1, kErrEmptyWait))) return false;
+  if (lane == 0) {
+    ring.item[s] = it;
+    mbar_arrive(&ring.full[s]);
+  }
+  return true;
+}
+// the n-th item, for the whole warp or for the one lane that runs a role; false if there is none, or none in time
+template <bool kWarp, typename Wait>
+__device__ __forceinline__ bool get_item(ItemRing& ring, uint32_t n, PromptItem& it, Wait& wait) {
+  const uint32_t s = n % kItemRing;
+  bool ok = wait(&ring.full[s], n / kItemRing, kErrFullWait);
+  if constexpr (kWarp) ok = __all_sync(0xffffffffu, ok);
+  if (!ok) return false;
+  it = ring.item[s];
+  if constexpr (kWarp) __syncwarp();
+  if (!kWarp || (threadIdx.x & 31) == 0) mbar_arrive(&ring.empty[s]);
+  return it.len >= 0;
+}
+
 template <int kHd, int kStages>
 struct PromptCtl {
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];
   uint64_t kv_full[kStages], kv_empty[kStages];
   uint64_t taken_free;  // tile 1 has read the record of tile 0 (once per item with a tile 1)
   TakenOut<kHd> taken[2];
+  ItemRing items;
   uint32_t tmem_base;
   int abort_flag;
 };
 
-// What an item holds for the two tiles
-struct PromptItem {
-  int64_t first;  // first row of the sequence
-  int len, row, head;
-  int n0, n1;  // key tiles of each tile of rows; 0: it has no rows
-};
-__device__ __forceinline__ bool prompt_item(const PromptParams& p, int64_t x, PromptItem& it, bool& bad) {
-  const int64_t slot = x / p.n_heads;
-  it.head = (int)(x - slot * p.n_heads);
-  const PromptBlock b = prompt_block(p.cu, p.n_seqs, p.n_rows, slot, kPaRows);
-  bad = b.len < 0;
-  if (b.row >= b.len) return false;
-  it.first = b.first, it.len = b.len, it.row = b.row;
-  it.n0 = b.row / kPaTile + 1;
-  it.n1 = b.row + kPaTile < b.len ? it.n0 + 1 : 0;
-  return true;
-}
+// key tiles of the second 128 rows of a block, 0 if it has none
+__device__ __forceinline__ int second_tiles(const PromptItem& it) { return it.row + kPaTile < it.len ? it.n + 1 : 0; }
 
 template <typename T, int kHd>
 struct PromptCfg {
   static constexpr int kStages = kHd == 128 ? 4 : 8;
+  // one pair of scores in so many has its exponentials on the multiply-add pipes (the exponential unit does 16 a clock and SM).
+  // 24 prompts up to 2048, head_dim 128: none 393, one in eight 392, six 389, four 395 us; 8192 tokens, head_dim 64, where half the
+  // products meet as many exponentials: 452, 461, 450, 433 us
+  static constexpr int kPolyEvery = kHd == 128 ? 6 : 4;
   static constexpr int kTileBytes = kPaTile * kHd * 2;
-  static constexpr int kSmem = 1024 + (2 + kStages) * kTileBytes + (int)sizeof(PromptCtl<kHd, kStages>) + 16;
+  static constexpr int kSmem = 1024 + (2 + kStages) * kTileBytes + 8 * kStageBytes + (int)sizeof(PromptCtl<kHd, kStages>) + 16;
 };
 
 template <typename T, int kHd>
@@ -247,7 +346,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
   extern __shared__ __align__(1024) uint8_t pa_smem[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pa_smem) + 1023) & ~(uintptr_t)1023);
   const uint32_t q_addr = smem_u32(base), kv_addr = q_addr + 2 * kTileBytes;
-  auto* ctl = reinterpret_cast<PromptCtl<kHd, kStages>*>(base + (2 + kStages) * kTileBytes);
+  uint8_t* stages = base + (2 + kStages) * kTileBytes;  // of the rows on their way out, a warp each
+  auto* ctl = reinterpret_cast<PromptCtl<kHd, kStages>*>(stages + 8 * kStageBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int x = 0; x < 2; ++x) {
@@ -257,6 +357,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
     }
     for (int s = 0; s < kStages; ++s) mbar_init(&ctl->kv_full[s], 1), mbar_init(&ctl->kv_empty[s], 1);
     mbar_init(&ctl->taken_free, 128);
+    for (int s = 0; s < kItemRing; ++s) mbar_init(&ctl->items.full[s], 1), mbar_init(&ctl->items.empty[s], 10);  // warps 0 to 9
     ctl->abort_flag = 0;
     mbar_init_fence();
   }
@@ -282,14 +383,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
     if (lane == 0) {
       uint32_t unit = 0, tiles[2] = {0, 0};  // key and value tiles requested; items of each row tile
       bool ok = true;
-      for (int64_t x = blockIdx.x; x < p.n_items && ok && !*abort_flag; x += gridDim.x) {
-        PromptItem it;
-        bool bad;
-        if (!prompt_item(p, x, it, bad)) {
-          if (bad) record_dev_error(kErrIndex);
-          continue;
-        }
-        const int kvh = it.head / p.group, row0 = (int)it.first + it.row;
+      PromptItem it;
+      for (uint32_t items = 0; ok && !*abort_flag && get_item<false>(ctl->items, items, it, wait); ++items) {
+        const int n1 = second_tiles(it), kvh = it.head / p.group, row0 = (int)it.first + it.row;
         auto load_q = [&](int t) {
           if (tiles[t] && !wait(&ctl->q_empty[t], tiles[t] - 1, kErrEmptyWait)) return false;
           mbar_arrive_expect_tx(&ctl->q_full[t], kTileBytes);
@@ -308,10 +404,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
           return true;
         };
         ok = load_q(0);
-        const int n = it.n1 ? it.n1 : it.n0;
+        const int n = n1 ? n1 : it.n;
         for (int j = 0; j < n && ok && !*abort_flag; ++j) {
           ok = load_kv(&kmap, j);
-          if (ok && j == 0 && it.n1) ok = load_q(1);
+          if (ok && j == 0 && n1) ok = load_q(1);
           if (ok) ok = load_kv(&vmap, j);
         }
       }
@@ -334,11 +430,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
     auto ready = [&](uint64_t* bar, uint32_t parity, int code) { return (bool)__all_sync(0xffffffffu, wait(bar, parity, code)); };
     uint32_t unit = 0, tiles[2] = {0, 0}, steps[2] = {0, 0};  // steps: key tiles of each row tile so far
     bool ok = true;
-    for (int64_t x = blockIdx.x; x < p.n_items && ok; x += gridDim.x) {
-      PromptItem it;
-      bool bad;
-      if (!prompt_item(p, x, it, bad)) continue;
-      const int n = it.n1 ? it.n1 : it.n0, nt[2] = {it.n0, it.n1};
+    PromptItem it;
+    for (uint32_t items = 0; ok && get_item<true>(ctl->items, items, it, wait); ++items) {
+      const int n1 = second_tiles(it), n = n1 ? n1 : it.n, nt[2] = {it.n, n1};
       auto stage = [&](int j, bool value) { return (unit + 2 * j + value) % kStages; };
       auto kv_ready = [&](int j, bool value) { return ready(&ctl->kv_full[stage(j, value)], (unit + 2 * j + value) / kStages, kErrFullWait); };
       auto scores = [&](int t, int j) {
@@ -382,11 +476,19 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
         if (ok && leader) {
           umma_commit(&ctl->kv_empty[stage(j, true)]);
           if (j + 1 < n) umma_commit(&ctl->kv_empty[stage(j + 1, false)]);
-          else umma_commit(&ctl->o_full[it.n1 ? 1 : 0]);  // last of all: nothing of this block arrives after its results are read
+          else umma_commit(&ctl->o_full[n1 ? 1 : 0]);  // last of all: nothing of this block arrives after its results are read
         }
       }
       unit += 2 * n;
     }
+  } else if (warp == 10) {
+    // ---------------- the items
+    int64_t x = blockIdx.x;
+    PromptItem it;
+    uint32_t items = 0;
+    do {
+      it = find_item(p.cu, p.n_seqs, p.n_rows, p.n_heads, p.n_items, kPaRows, x, lane);
+    } while (put_item(ctl->items, items++, it, lane, wait) && it.len >= 0);
   } else if (warp < 8) {
     // ---------------- softmax: a thread per row of tile t
     set_regs_up<kPaSoftmaxRegs>();
@@ -395,38 +497,39 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
     const uint32_t s_addr = tmem + lanes + t * kPaTile, o_addr = tmem + lanes + 256 + t * 128;
     uint32_t unit = 0, steps = 0, done = 0, done1 = 0;  // items so far; those with a tile 1
     bool ok = true;
-    for (int64_t x = blockIdx.x; x < p.n_items && ok; x += gridDim.x) {
-      PromptItem it;
-      bool bad;
-      if (!prompt_item(p, x, it, bad)) continue;
-      const int n = it.n1 ? it.n1 : it.n0, mine = t ? it.n1 : it.n0;
+    PromptItem it;
+    for (; ok && get_item<true>(ctl->items, done, it, wait);) {
+      const int n1 = second_tiles(it), n = n1 ? n1 : it.n, mine = t ? n1 : it.n;
       float ref = -INFINITY, mc = 0.f;  // the reference; c times it
       uint64_t sum2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
       for (int j = 0; j < mine && ok; ++j) {
         if (!(ok = __all_sync(0xffffffffu, wait(&ctl->s_full[t], steps++, kErrMmaWait)))) break;
         tc_fence_after();
         uint32_t s[kPaTile];
+        const bool last = j + 1 == mine;
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // NaN where a visible score is: then the whole row is
 #pragma unroll
         for (int i = 0; i < 4; ++i) tmem_ld32_nowait(s_addr + 32 * i, s + 32 * i);
 #pragma unroll
         for (int i = 0; i < 4; ++i) tmem_wait_ld(s + 32 * i);
-        const bool last = j + 1 == mine;
-        if (last) {  // keys behind the row
+        if (last) {  // keys behind the row: some of the 32 that are its warp's own, and all behind those
 #pragma unroll
-          for (int i = 0; i < kPaTile; ++i)
-            if (i > r) s[i] = 0xff800000u;
+          for (int c = 0; c < 4; ++c) {
+            if (c < (warp & 3)) continue;
+            const int seen = c == (warp & 3) ? lane : -1;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i > seen) s[32 * c + i] = 0xff800000u;
+          }
         }
-        float top[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top[i] = __uint_as_float(s[i]);
-#pragma unroll
-        for (int i = 4; i < kPaTile; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[i]));
-        const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        for (int i = 0; i < kPaTile; i += 2) top[(i >> 1) & 3] = max3_nan(top[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+        const float most = max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3]));
         if (j == 0) {
           ref = most;
           mc = ref == -INFINITY ? 0.f : ref * p.c;
         } else {
-          const bool move = (most - ref) * p.c > 8.f;
+          const bool move = !((most - ref) * p.c <= 8.f);
           if (__any_sync(0xffffffffu, move)) {  // O is complete up to the tile before: S of this one came after it
             // each row by its own scores alone: its bits do not depend on what else is in the warp
             const float keep = move ? exp2_approx((ref - most) * p.c) : 1.f;
@@ -454,8 +557,13 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
 #pragma unroll
         for (int i = 0; i < kPaTile; i += 2) {
           float a, b;
-          unpair(fma2(pair(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, m2), a, b);
-          a = exp2_approx(a), b = exp2_approx(b);
+          const uint64_t x = fma2(pair(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, m2);
+          if (i / 2 % Cfg::kPolyEvery == Cfg::kPolyEvery - 1) {
+            exp2_poly2(x, a, b);
+          } else {
+            unpair(x, a, b);
+            a = exp2_approx(a), b = exp2_approx(b);
+          }
           sum2[(i >> 1) & 1] = add2(sum2[(i >> 1) & 1], pair(a, b));
           w[i >> 1] = cvt2<T>(a, b);
           if (i % 64 == 62) tmem_st32(s_addr + (i / 64) * 32, w + (i / 64) * 32);
@@ -466,22 +574,26 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
           if (!(ok = __all_sync(0xffffffffu, wait(&ctl->kv_full[st], u / kStages, kErrFullWait)))) break;
           uint8_t* v = base + (2 + st) * kTileBytes;
           TakenOut<kHd>* rec = &ctl->taken[t];
-          bool found = false;
-#pragma unroll 4
+          const uint32_t v_mine = smem_u32(v) + r * 16;
+          uint32_t odd = 0;
+#pragma unroll
           for (int i = 0; i < kTileBytes / 16 / 128; ++i) {
-            const int at = (i * 128 + r) * 16;
-            const uint4 q = *reinterpret_cast<const uint4*>(v + at);
-            if (!(not_finite2<T>(q.x) || not_finite2<T>(q.y) || not_finite2<T>(q.z) || not_finite2<T>(q.w))) continue;
-            // tile 0's record is read by tile 1 too, perhaps still for the last item that had one
-            if (t == 0 && !found && done1 && !wait(&ctl->taken_free, done1 - 1, kErrMmaWait)) break;
-            found = true;
-            const int box = at / kBoxBytes, key = (at % kBoxBytes) / 128, chunk = ((at % 128) / 16) ^ (key & 7);
-            T* e = reinterpret_cast<T*>(v + at);
-            for (int k = 0; k < 8; ++k) {
-              const float f = to_f32(e[k]);
-              if (isfinite(f)) continue;
-              atomicMin(&rec->row[f != f ? 2 : f < 0.f ? 1 : 0][box * 64 + chunk * 8 + k], taken_word(done, key));
-              e[k] = from_f32<T>(0.f);
+            const uint4 q = lds_u4(v_mine + i * 2048);
+            odd |= not_finite2<T>(q.x) | not_finite2<T>(q.y) | not_finite2<T>(q.z) | not_finite2<T>(q.w);
+          }
+          const bool found = (odd & 0x80008000u) != 0;
+          // tile 0's record is read by tile 1 too, perhaps still for the last item that had one
+          if (found && (t || !done1 || wait(&ctl->taken_free, done1 - 1, kErrMmaWait))) {
+#pragma unroll 1
+            for (int i = 0; i < kTileBytes / 16 / 128; ++i) {
+              const int at = (i * 128 + r) * 16, box = at / kBoxBytes, key = (at % kBoxBytes) / 128, chunk = ((at % 128) / 16) ^ (key & 7);
+              T* e = reinterpret_cast<T*>(v + at);
+              for (int k = 0; k < 8; ++k) {
+                const float f = to_f32(e[k]);
+                if (isfinite(f)) continue;
+                atomicMin(&rec->row[f != f ? 2 : f < 0.f ? 1 : 0][box * 64 + chunk * 8 + k], taken_word(done, key));
+                e[k] = from_f32<T>(0.f);
+              }
             }
           }
           if (found) {
@@ -501,47 +613,44 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
         const float total = (a + b) + (a1 + b1), inv = total == 0.f ? 0.f : 1.f / total;
         const int row = it.row + t * kPaTile + r;
         const bool rec0 = ctl->taken[0].last == done + 1, rec1 = t && ctl->taken[1].last == done + 1;
-        T* dst = reinterpret_cast<T*>(p.out) + ((it.first + row) * p.n_heads + it.head) * kHd;
+        const int row0 = row - lane;  // of the warp
+        uint8_t* dst = reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(p.out) + ((it.first + row0) * p.n_heads + it.head) * kHd);
+        const int64_t row_bytes = (int64_t)p.n_heads * kHd * sizeof(T);
+        uint32_t all[kHd];
+#pragma unroll
+        for (int i = 0; i < kHd / 32; ++i) tmem_ld32_nowait(o_addr + 32 * i, all + 32 * i);
 #pragma unroll
         for (int i = 0; i < kHd / 32; ++i) {
-          uint32_t o[32];
-          tmem_ld32_nowait(o_addr + 32 * i, o);
+          uint32_t* o = all + 32 * i;
           tmem_wait_ld(o);
-          if (row < it.len) {
-            if (rec0 || rec1) {
+          if (rec0 || rec1) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                float f = __uint_as_float(o[e]);
+            for (int e = 0; e < 32; ++e) {
+              float f = __uint_as_float(o[e]);
 #pragma unroll 1
-                for (int k = 0; k < 1 + t; ++k) {
-                  if (!(k ? rec1 : rec0)) continue;
-                  const int upto = k == t ? r : kPaTile - 1;  // tile 1 sees all of tile 0's keys
-                  const volatile uint32_t* q = &ctl->taken[k].row[0][32 * i + e];
-                  if (taken_row(q[0], done) <= upto) f += INFINITY;
-                  if (taken_row(q[kHd], done) <= upto) f -= INFINITY;
-                  if (taken_row(q[2 * kHd], done) <= upto) f += __int_as_float(0x7fc00000);
-                }
-                o[e] = __float_as_uint(f);
+              for (int k = 0; k < 1 + t; ++k) {
+                if (!(k ? rec1 : rec0)) continue;
+                const int upto = k == t ? r : kPaTile - 1;  // tile 1 sees all of tile 0's keys
+                const volatile uint32_t* q = &ctl->taken[k].row[0][32 * i + e];
+                if (taken_row(q[0], done) <= upto) f += INFINITY;
+                if (taken_row(q[kHd], done) <= upto) f -= INFINITY;
+                if (taken_row(q[2 * kHd], done) <= upto) f += __int_as_float(0x7fc00000);
               }
-            }
-#pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint4 q;
-              q.x = cvt2<T>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-              q.y = cvt2<T>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-              q.z = cvt2<T>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-              q.w = cvt2<T>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-              *reinterpret_cast<uint4*>(dst + 32 * i + e) = q;
+              o[e] = __float_as_uint(f);
             }
           }
-          __syncwarp();
+          uint4 v[4];
+          uint32_t* w = reinterpret_cast<uint32_t*>(v);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = cvt2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+          store_rows64(smem_u32(stages) + warp * kStageBytes, lane, v, dst + 64 * i, row_bytes, it.len - row0);
         }
         tc_fence_before();
         if (t) mbar_arrive(&ctl->taken_free);
       }
       unit += 2 * n;
       ++done;
-      done1 += it.n1 != 0;
+      done1 += n1 != 0;
     }
   }
   tc_fence_before();

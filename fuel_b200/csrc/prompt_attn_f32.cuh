@@ -22,7 +22,7 @@
 //   warps 8-11      O: a thread per row adds the tiles' products, finishes and stores it
 //   warps 12, 15    copies: the parts of Q and K, of V
 //   warp 13         issues the MMAs
-//   warp 14         brings the powers of each key tile
+//   warp 14         finds the block's items and brings the powers of each key tile
 #pragma once
 #include "prompt_attn.cuh"
 
@@ -143,6 +143,7 @@ struct PromptF32Ctl {
   float4 up[2][kPaTile / 2];           // of two keys: 2^ek, 2^ek, f, f
   float2 down[2][kPaTile / 2];         // 2^-f, 2^-f
   uint64_t q_full, q_empty, s_full[2], p_full[2], pv_full, pv_empty, up_full[2], up_empty[2];
+  ItemRing items;
   uint64_t k_full[kPfaRing], k_empty[kPfaRing], v_full[kPfaRing], v_empty[kPfaRing];
   uint32_t tmem_base;
   int abort_flag;
@@ -153,7 +154,7 @@ struct PromptF32Cfg {
   static constexpr int kTileBytes = kPaTile * kHd * 2;  // one part of a tile
   static constexpr int kUnitBytes = kPaTile * 128;      // of K: 64 columns of a part; of V: kUnitKeys rows of a part
   static constexpr int kUnits = kTileBytes / kUnitBytes, kUnitKeys = kPaTile / kUnits;
-  static constexpr int kSmem = 1024 + 2 * kTileBytes + 2 * kPfaRing * kUnitBytes + (int)sizeof(PromptF32Ctl) + 16;
+  static constexpr int kSmem = 1024 + 2 * kTileBytes + 2 * kPfaRing * kUnitBytes + 4 * kStageBytes + (int)sizeof(PromptF32Ctl) + 16;
 };
 
 // A row of the result whose key tiles hold values that are not finite: adds those that the row sees
@@ -184,11 +185,13 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pfa_smem) + 1023) & ~(uintptr_t)1023);
   uint8_t* v_ring = base + 2 * kTileBytes + kPfaRing * kUnitBytes;
   const uint32_t q_addr = smem_u32(base), k_addr = q_addr + 2 * kTileBytes, v_addr = smem_u32(v_ring);
-  auto* ctl = reinterpret_cast<PromptF32Ctl*>(v_ring + kPfaRing * kUnitBytes);
+  uint8_t* stages = v_ring + kPfaRing * kUnitBytes;  // of the rows on their way out, a warp each
+  auto* ctl = reinterpret_cast<PromptF32Ctl*>(stages + 4 * kStageBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(&ctl->q_full, 1), mbar_init(&ctl->q_empty, 1), mbar_init(&ctl->pv_full, 1), mbar_init(&ctl->pv_empty, 128);
     for (int i = 0; i < 2; ++i) mbar_init(&ctl->s_full[i], 1), mbar_init(&ctl->p_full[i], 128), mbar_init(&ctl->up_full[i], 1), mbar_init(&ctl->up_empty[i], 128);
+    for (int s = 0; s < kItemRing; ++s) mbar_init(&ctl->items.full[s], 1), mbar_init(&ctl->items.empty[s], 16);  // every warp
     for (int s = 0; s < kPfaRing; ++s) {
       mbar_init(&ctl->k_full[s], 1), mbar_init(&ctl->k_empty[s], 1);
       mbar_init(&ctl->v_full[s], 1), mbar_init(&ctl->v_empty[s], 1);
@@ -209,18 +212,6 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
     *abort_flag = 1;
     return false;
   };
-  struct Item {
-    int64_t first;
-    int len, row, head, n;
-  };
-  auto item = [&](int64_t x, Item& it) {
-    const int64_t slot = x / p.n_heads;
-    const PromptBlock b = prompt_block(p.cu, p.n_seqs, p.n_rows, slot, kPaTile);
-    if (b.row >= b.len) return false;
-    it.first = b.first, it.len = b.len, it.row = b.row, it.head = (int)(x - slot * p.n_heads), it.n = b.row / kPaTile + 1;
-    return true;
-  };
-
   const uint32_t p_low = tmem + 256, pv_acc = tmem + 384;
 
   if (warp >= 12) set_regs_down<kPfaOtherRegs>();
@@ -232,9 +223,8 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
       uint64_t* empty = values ? ctl->v_empty : ctl->k_empty;
       uint32_t unit = 0, items = 0;
       bool ok = true;
-      for (int64_t x = blockIdx.x; x < p.n_items && ok && !*abort_flag; x += gridDim.x) {
-        Item it;
-        if (!item(x, it)) continue;
+      PromptItem it;
+      for (; ok && !*abort_flag && get_item<false>(ctl->items, items, it, wait); ++items) {
         const int kvh = it.head / p.group;
         if (!values) {
           if (items && !(ok = wait(&ctl->q_empty, items - 1, kErrEmptyWait))) break;
@@ -242,7 +232,6 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
           for (int part = 0; part < 2; ++part)
             for (int b = 0; b < kUnits; ++b)
               tma_load_3d(q_addr + part * kTileBytes + b * kUnitBytes, &qmap, 64 * b, it.head, (int)(part * p.n_rows + it.first + it.row), &ctl->q_full);
-          ++items;
         }
         for (int j = 0; j < it.n && ok && !*abort_flag; ++j)
           for (int u = 0; u < 2 * kUnits && ok; ++u, ++unit) {
@@ -262,7 +251,7 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
       if (*abort_flag) {  // leaving early: let the copies already requested land first
         for (uint32_t u = unit > kPfaRing ? unit - kPfaRing : 0; u < unit; ++u)
           if (!mbar_wait_bounded(&full[u % kPfaRing], (u / kPfaRing) & 1)) record_dev_error(kErrDrainWait);
-        if (items && !mbar_wait_bounded(&ctl->q_full, (items - 1) & 1)) record_dev_error(kErrDrainWait);
+        if (!values && items && !mbar_wait_bounded(&ctl->q_full, (items - 1) & 1)) record_dev_error(kErrDrainWait);
       }
     }
   } else if (warp == 13) {
@@ -274,9 +263,8 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
     auto ready = [&](uint64_t* bar, uint32_t parity, int code) { return (bool)__all_sync(0xffffffffu, wait(bar, parity, code)); };
     uint32_t items = 0, steps = 0;
     bool ok = true;
-    for (int64_t x = blockIdx.x; x < p.n_items && ok; x += gridDim.x) {
-      Item it;
-      if (!item(x, it)) continue;
+    PromptItem it;
+    for (; ok && get_item<true>(ctl->items, items, it, wait); ++items) {
       // S of key tile j into its half of tensor memory: hi hi and lo hi of each unit of the upper part, then hi lo
       auto scores = [&](int j) {
         const uint32_t d = acc + ((steps + j) & 1) * kPaTile;
@@ -301,7 +289,7 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
         }
         return true;
       };
-      if (!(ok = ready(&ctl->q_full, items++, kErrFullWait))) break;
+      if (!(ok = ready(&ctl->q_full, items, kErrFullWait))) break;
       ok = scores(0);
       for (int j = 0; j < it.n && ok; ++j) {
         if (j + 1 < it.n && !(ok = scores(j + 1))) break;
@@ -328,12 +316,15 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
       steps += it.n;
     }
   } else if (warp == 14) {
-    // ---------------- the powers of each key tile
-    uint32_t steps = 0;
-    bool ok = true;
-    for (int64_t x = blockIdx.x; x < p.n_items && ok && !*abort_flag; x += gridDim.x) {
-      Item it;
-      if (!item(x, it)) continue;
+    // ---------------- the items, one ahead, and the powers of each key tile
+    uint32_t steps = 0, items = 0;
+    int64_t x = blockIdx.x;
+    auto next = [&]() { return find_item(p.cu, p.n_seqs, p.n_rows, p.n_heads, p.n_items, kPaTile, x, lane); };
+    PromptItem ahead = next(), it;
+    bool ok = put_item(ctl->items, 0, ahead, lane, wait);
+    for (; ok && get_item<true>(ctl->items, items, it, wait); ++items) {
+      ahead = next();
+      if (!(ok = put_item(ctl->items, items + 1, ahead, lane, wait))) break;
       const float2* src = p.kv_up + (int64_t)(it.head / p.group) * p.n_rows + it.first;
       for (int j = 0; j < it.n && ok; ++j, ++steps) {
         if (steps >= 2 && !(ok = __all_sync(0xffffffffu, wait(&ctl->up_empty[steps & 1], steps / 2 - 1, kErrEmptyWait)))) break;
@@ -360,9 +351,8 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
     const uint32_t up = smem_u32(ctl->up[half]), down = smem_u32(ctl->down[half]);
     uint32_t steps = 0;
     bool ok = true;
-    for (int64_t x = blockIdx.x; x < p.n_items && ok; x += gridDim.x) {
-      Item it;
-      if (!item(x, it)) continue;
+    PromptItem it;
+    for (uint32_t items = 0; ok && get_item<true>(ctl->items, items, it, wait); ++items) {
       const int row = it.row + r;
       const float cq = row < it.len ? p.q_up[(int64_t)it.head * p.n_rows + it.first + row] : 0.f;
       const uint64_t cq2 = pair(cq, cq);
@@ -466,9 +456,8 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
     const uint32_t addr = pv_acc + ((uint32_t)((warp & 3) * 32) << 16);
     uint32_t steps = 0;
     bool ok = true;
-    for (int64_t x = blockIdx.x; x < p.n_items && ok; x += gridDim.x) {
-      Item it;
-      if (!item(x, it)) continue;
+    PromptItem it;
+    for (uint32_t items = 0; ok && get_item<true>(ctl->items, items, it, wait); ++items) {
       float o[kHd], ref = -INFINITY, sum = 0.f;
 #pragma unroll
       for (int e = 0; e < kHd; ++e) o[e] = 0.f;
@@ -496,12 +485,19 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
       bool odd = false;
       for (int j = lane; j < it.n; j += 32) odd |= p.marked[rows_at + (int64_t)j * kPaTile] != 0;
       odd = __any_sync(0xffffffffu, odd);
-      if (row < it.len) {
-        float* dst = p.out + ((it.first + row) * p.n_heads + it.head) * kHd;
+      const int row0 = row - lane;  // of the warp
+      float* dst = p.out + ((it.first + row0) * p.n_heads + it.head) * kHd;
 #pragma unroll
-        for (int e = 0; e < kHd; e += 4)
-          *reinterpret_cast<float4*>(dst + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
-        if (odd) add_not_finite<kHd>(p, it.first, row, it.head, dst);
+      for (int i = 0; i < kHd / 16; ++i) {
+        uint4 v[4];
+        float* w = reinterpret_cast<float*>(v);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = o[16 * i + e] * inv;
+        store_rows64(smem_u32(stages) + (warp & 3) * kStageBytes, lane, v, reinterpret_cast<uint8_t*>(dst + 16 * i), (int64_t)p.n_heads * kHd * 4, it.len - row0);
+      }
+      if (odd) {
+        __syncwarp();  // the rows are written: each lane completes its own
+        if (row < it.len) add_not_finite<kHd>(p, it.first, row, it.head, dst + (int64_t)lane * p.n_heads * kHd);
       }
       __syncwarp();
     }
