@@ -117,6 +117,27 @@ __device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
                :
                : "memory");
 }
+__device__ __forceinline__ void tmem_ld8_nowait(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld8(uint32_t (&r)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%4], {%0,%1,%2,%3};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+               "r"(r[15]), "r"(taddr)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
                "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
@@ -142,6 +163,11 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float d;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 // two f32 at a time
@@ -505,68 +531,99 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
       for (int j = 0; j < mine && ok; ++j) {
         if (!(ok = __all_sync(0xffffffffu, wait(&ctl->s_full[t], steps++, kErrMmaWait)))) break;
         tc_fence_after();
-        uint32_t s[kPaTile];
         const bool last = j + 1 == mine;
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // NaN where a visible score is: then the whole row is
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32_nowait(s_addr + 32 * i, s + 32 * i);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_wait_ld(s + 32 * i);
-        if (last) {  // keys behind the row: some of the 32 that are its warp's own, and all behind those
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (c < (warp & 3)) continue;
-            const int seen = c == (warp & 3) ? lane : -1;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i > seen) s[32 * c + i] = 0xff800000u;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kPaTile; i += 2) top[(i >> 1) & 3] = max3_nan(top[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-        const float most = max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3]));
-        if (j == 0) {
-          ref = most;
-          mc = ref == -INFINITY ? 0.f : ref * p.c;
-        } else {
-          const bool move = !((most - ref) * p.c <= 8.f);
-          if (__any_sync(0xffffffffu, move)) {  // O is complete up to the tile before: S of this one came after it
-            // each row by its own scores alone: its bits do not depend on what else is in the warp
-            const float keep = move ? exp2_approx((ref - most) * p.c) : 1.f;
-            if (move) ref = most;
+        uint64_t c2, m2;
+        // the row's reference, once its maximum is in top[]
+        auto refer = [&]() {
+          const float most = max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3]));
+          if (j == 0) {
+            ref = most;
             mc = ref == -INFINITY ? 0.f : ref * p.c;
+          } else {
+            const bool move = !((most - ref) * p.c <= 8.f);
+            if (__any_sync(0xffffffffu, move)) {  // O is complete up to the tile before: S of this one came after it
+              // each row by its own scores alone: its bits do not depend on what else is in the warp
+              const float keep = move ? exp2_approx((ref - most) * p.c) : 1.f;
+              if (move) ref = most;
+              mc = ref == -INFINITY ? 0.f : ref * p.c;
+#pragma unroll 1
+              for (int i = 0; i < kHd / 16; ++i) {
+                uint32_t o[16];
+                tmem_ld16(o_addr + 16 * i, o);
 #pragma unroll
-            for (int i = 0; i < kHd / 32; ++i) {
-              uint32_t o[32];
-              tmem_ld32_nowait(o_addr + 32 * i, o);
-              tmem_wait_ld(o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                tmem_st16(o_addr + 16 * i, o);
+              }
+              float a, b;
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-              tmem_st32(o_addr + 32 * i, o);
-            }
-            float a, b;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              unpair(sum2[i], a, b);
-              sum2[i] = pair(a * keep, b * keep);
+              for (int i = 0; i < 2; ++i) {
+                unpair(sum2[i], a, b);
+                sum2[i] = pair(a * keep, b * keep);
+              }
             }
           }
-        }
-        const uint64_t c2 = pair(p.c, p.c), m2 = pair(-mc, -mc);
-        uint32_t w[kPaTile / 2];
-#pragma unroll
-        for (int i = 0; i < kPaTile; i += 2) {
+          c2 = pair(p.c, p.c), m2 = pair(-mc, -mc);
+        };
+        auto weight2 = [&](int i, uint32_t s0, uint32_t s1) {  // of pair i of the tile
           float a, b;
-          const uint64_t x = fma2(pair(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, m2);
-          if (i / 2 % Cfg::kPolyEvery == Cfg::kPolyEvery - 1) {
+          const uint64_t x = fma2(pair(__uint_as_float(s0), __uint_as_float(s1)), c2, m2);
+          if (i % Cfg::kPolyEvery == Cfg::kPolyEvery - 1) {
             exp2_poly2(x, a, b);
           } else {
             unpair(x, a, b);
             a = exp2_approx(a), b = exp2_approx(b);
           }
-          sum2[(i >> 1) & 1] = add2(sum2[(i >> 1) & 1], pair(a, b));
-          w[i >> 1] = cvt2<T>(a, b);
-          if (i % 64 == 62) tmem_st32(s_addr + (i / 64) * 32, w + (i / 64) * 32);
+          sum2[i & 1] = add2(sum2[i & 1], pair(a, b));
+          return cvt2<T>(a, b);
+        };
+        if (!last) {
+          uint32_t s[kPaTile];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmem_ld32_nowait(s_addr + 32 * i, s + 32 * i);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmem_wait_ld(s + 32 * i);
+#pragma unroll
+          for (int i = 0; i < kPaTile; i += 2) top[(i >> 1) & 3] = max3_nan(top[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+          refer();
+          uint32_t w[kPaTile / 2];
+#pragma unroll
+          for (int i = 0; i < kPaTile / 2; ++i) {
+            w[i] = weight2(i, s[2 * i], s[2 * i + 1]);
+            if (i % 32 == 31) tmem_st32(s_addr + i - 31, w + i - 31);
+          }
+        } else {
+          // The last tile of an item, with keys behind the row: short loops that read the scores from tensor memory twice. Code that is
+          // run through once comes at some four cycles an instruction, and this is run once an item: 64 prompts of 256 tokens take
+          // 116 us this way, 143 with the lines above; 4096 tokens 181 us if every tile is taken this way, 158 otherwise
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t s[32];
+            tmem_ld32_nowait(s_addr + 32 * c, s);
+            tmem_wait_ld(s);
+            const int seen = r - 32 * c;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i > seen) s[i] = 0xff800000u;
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) top[(i >> 1) & 3] = max3_nan(top[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+          }
+          refer();
+          uint32_t s[2][16];
+          tmem_ld16_nowait(s_addr, s[0]);
+#pragma unroll 1
+          for (int c0 = 0; c0 < 8; c0 += 2) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = c0 + h, seen = r - 16 * c;
+              tmem_wait_ld16(s[h]);
+              if (c < 7) tmem_ld16_nowait(s_addr + 16 * (c + 1), s[h ^ 1]);
+              uint32_t w[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) w[i] = weight2(i, 2 * i > seen ? 0xff800000u : s[h][2 * i], 2 * i + 1 > seen ? 0xff800000u : s[h][2 * i + 1]);
+              tmem_st8(s_addr + 8 * c, w);  // over scores that have been read: in front of the ones in flight
+            }
+          }
         }
         if (last) {
           // values of the last key tile that are not finite: out of the tile, into the record
@@ -576,7 +633,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
           TakenOut<kHd>* rec = &ctl->taken[t];
           const uint32_t v_mine = smem_u32(v) + r * 16;
           uint32_t odd = 0;
-#pragma unroll
+#pragma unroll 4
           for (int i = 0; i < kTileBytes / 16 / 128; ++i) {
             const uint4 q = lds_u4(v_mine + i * 2048);
             odd |= not_finite2<T>(q.x) | not_finite2<T>(q.y) | not_finite2<T>(q.z) | not_finite2<T>(q.w);
@@ -616,12 +673,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
         const int row0 = row - lane;  // of the warp
         uint8_t* dst = reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(p.out) + ((it.first + row0) * p.n_heads + it.head) * kHd);
         const int64_t row_bytes = (int64_t)p.n_heads * kHd * sizeof(T);
-        uint32_t all[kHd];
-#pragma unroll
-        for (int i = 0; i < kHd / 32; ++i) tmem_ld32_nowait(o_addr + 32 * i, all + 32 * i);
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < kHd / 32; ++i) {
-          uint32_t* o = all + 32 * i;
+          uint32_t o[32];
+          tmem_ld32_nowait(o_addr + 32 * i, o);
           tmem_wait_ld(o);
           if (rec0 || rec1) {
 #pragma unroll

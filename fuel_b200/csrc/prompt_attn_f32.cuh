@@ -362,11 +362,11 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
         const bool last = j + 1 == it.n;
-        // the maximum, and again from tensor memory the weights: S is not held in registers. Sixteen columns at a time, the next
-        // sixteen on their way; rolled up, so that the loops stay in the instruction cache
-        uint32_t s[2][16];
+        // the maximum, and again from tensor memory the weights, in short loops with the next columns on their way (code that is run
+        // through once per key tile comes at some four cycles an instruction)
         float top[2] = {-INFINITY, -INFINITY};
         auto look = [&](auto masked) {
+          uint32_t s[2][16];
           tmem_ld16_nowait(s_addr, s[0]);
 #pragma unroll 1
           for (int c0 = 0; c0 < 8; c0 += 2) {
@@ -375,14 +375,15 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
               const int c = c0 + h;
               tmem_wait_ld16(s[h]);
               if (c < 7) tmem_ld16_nowait(s_addr + 16 * (c + 1), s[h ^ 1]);
+              const int seen = r - 16 * c;  // the last of the sixteen keys that this row sees
 #pragma unroll
               for (int i = 0; i < 16; i += 2) {
                 const float4 w = lds_f4(up + (8 * c + i / 2) * 16);
                 float a, b;
                 unpair(fma2(pair(__uint_as_float(s[h][i]), __uint_as_float(s[h][i + 1])), mul2(pair(w.x, w.y), cq2), pair(w.z, w.w)), a, b);
-                if (decltype(masked)::value && c * 16 + i > r) a = -INFINITY;
-                if (decltype(masked)::value && c * 16 + i + 1 > r) b = -INFINITY;
-                top[0] = fmaxf(top[0], a), top[1] = fmaxf(top[1], b);
+                if (decltype(masked)::value && i > seen) a = -INFINITY;
+                if (decltype(masked)::value && i + 1 > seen) b = -INFINITY;
+                top[i / 2 & 1] = max3(top[i / 2 & 1], a, b);
               }
             }
           }
@@ -393,31 +394,33 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
         const uint64_t rr2 = pair(rr, rr);
         uint64_t sum2 = pair(0.f, 0.f);
         auto weigh = [&](auto masked) {
-          tmem_ld16_nowait(s_addr, s[0]);
+          uint32_t s[2][8];
+          tmem_ld8_nowait(s_addr, s[0]);
 #pragma unroll 1
-          for (int c0 = 0; c0 < 8; c0 += 2) {
+          for (int c0 = 0; c0 < 16; c0 += 2) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int c = c0 + h;
-              tmem_wait_ld16(s[h]);
-              if (c < 7) tmem_ld16_nowait(s_addr + 16 * (c + 1), s[h ^ 1]);
-              uint32_t hi[8], lo[8];
+              tmem_wait_ld8(s[h]);
+              if (c < 15) tmem_ld8_nowait(s_addr + 8 * (c + 1), s[h ^ 1]);
+              const int seen = r - 8 * c;
+              uint32_t hi[4], lo[4];
 #pragma unroll
-              for (int i = 0; i < 16; i += 2) {
-                const float4 w = lds_f4(up + (8 * c + i / 2) * 16);
+              for (int i = 0; i < 8; i += 2) {
+                const float4 w = lds_f4(up + (4 * c + i / 2) * 16);
                 float a, b;
                 unpair(fma2(pair(__uint_as_float(s[h][i]), __uint_as_float(s[h][i + 1])), mul2(pair(w.x, w.y), cq2), add2(pair(w.z, w.w), rr2)), a, b);
-                if (decltype(masked)::value && c * 16 + i > r) a = -INFINITY;
-                if (decltype(masked)::value && c * 16 + i + 1 > r) b = -INFINITY;
+                if (decltype(masked)::value && i > seen) a = -INFINITY;
+                if (decltype(masked)::value && i + 1 > seen) b = -INFINITY;
                 a = exp2_approx(a), b = exp2_approx(b);
-                sum2 = fma2(pair(a, b), lds_pair(down + (8 * c + i / 2) * 8), sum2);
+                sum2 = fma2(pair(a, b), lds_pair(down + (4 * c + i / 2) * 8), sum2);
                 hi[i / 2] = cvt2<__half>(a, b);
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[i / 2]));
                 lo[i / 2] = cvt2<__half>(a - f.x, b - f.y);
               }
               // over columns of S that have been read: in front of the ones in flight
-              tmem_st8(s_addr + 8 * c, hi);
-              tmem_st8(lo_addr + 8 * c, lo);
+              tmem_st4(s_addr + 4 * c, hi);
+              tmem_st4(lo_addr + 4 * c, lo);
             }
           }
         };
