@@ -10,13 +10,17 @@
 
 namespace fq {
 
-// ---- decode. The keys of a sequence are cut into tiles, a unit of work ("item") is one sequence and one kv head, and the
-// tiles of all items, laid end to end, are dealt out in equal runs to the thread blocks: block b has tiles
-// [split_begin(b), split_begin(b + 1)). An item that lies in several runs is joined from its pieces.
-FQ_HD int64_t split_begin(int64_t total, int blocks, int b) { return total * b / blocks; }
-// the block whose run holds `tile`: the largest b with split_begin(b) <= tile
-FQ_HD int split_block(int64_t total, int blocks, int64_t tile) { return (int)(((tile + 1) * blocks - 1) / total); }
-// where block b leaves its piece of an item that begins at tile `first`: its first slot if the piece begins with its run
+// ---- decode. The keys of a sequence are cut into tiles, a unit of work ("item") is one sequence and one kv head. The tiles of
+// all items, laid end to end with kItemUnits places behind each item for what an item costs besides its tiles, are dealt out in
+// equal runs to the thread blocks: block b has places [split_begin(b), split_begin(b + 1)). An item whose tiles lie in several
+// runs is joined from its pieces.
+constexpr int kItemUnits = 2;
+// quotients of numbers that hardly ever pass 32 bits, where the long division is a hundred instructions
+FQ_HD int64_t quotient(int64_t a, int64_t b) { return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b; }
+FQ_HD int64_t split_begin(int64_t total, int blocks, int b) { return quotient(total * b, blocks); }
+// the block whose run holds place x: the largest b with split_begin(b) <= x
+FQ_HD int split_block(int64_t total, int blocks, int64_t x) { return (int)quotient((x + 1) * blocks - 1, total); }
+// where block b leaves its piece of an item that begins at place `first`: its first slot if the piece begins with its run
 FQ_HD int split_slot(int64_t total, int blocks, int b, int64_t first) { return 2 * b + (split_begin(total, blocks, b) < first ? 1 : 0); }
 // tiles of a sequence: lengths below zero count as zero, lengths behind the end of its page table row as that end
 FQ_HD int seq_keys(int len, int max_pages, int page_shift) {
@@ -24,6 +28,8 @@ FQ_HD int seq_keys(int len, int max_pages, int page_shift) {
   return len < 0 ? 0 : len > room ? (int)room : len;
 }
 FQ_HD int seq_tiles(int len, int max_pages, int page_shift, int tile) { return (int)(((int64_t)seq_keys(len, max_pages, page_shift) + tile - 1) / tile); }
+
+FQ_HD int item_units(int tiles) { return tiles ? tiles + kItemUnits : 0; }
 
 // ---- prompts. An item is a block of `rows` rows of one sequence and one query head. Sequence s has the block numbers ("slots")
 // from prompt_slot(cu[s], s) up to the next sequence's: at least as many as it has blocks, without any sum over the

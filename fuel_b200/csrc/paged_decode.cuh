@@ -14,7 +14,7 @@
 // Work: tiles of kTile keys of all (sequence, kv head) items, laid end to end and dealt out evenly (attn_plan.h), so that one
 // long sequence, many short ones and any mixture fill the device alike. A warp owns 16 (head_dim 64: 32) keys of each
 // tile and runs by itself: its own ring of cp.async copies that runs on across items, its own running maximum and sums; the
-// block's four warps are joined in shared memory at the end of an item, pieces of an item in other blocks by
+// block's four warps join their results in shared memory at the end of an item, a quarter of the columns each, pieces of an item in other blocks by
 // paged_join_kernel in a fixed order.
 #pragma once
 #include <type_traits>
@@ -92,8 +92,10 @@ struct DecodeCfg {
   static constexpr int kParts = !kWideAct ? 1 : kF32 ? 2 : sizeof(C) == 2 && std::is_same<C, __nv_bfloat16>::value ? 3 : 2;
   static constexpr int kKs = kF32 ? kHd / 8 : kHd / 16, kMt = kHd / 16;
   static constexpr int kQBytes = kNT * kParts * kKs * 256;             // q in the order of the instruction's operand
-  static constexpr int kMergeBytes = 32 * (kNT * kMt * 16 + kNT * 16);  // one warp's sums and statistics
-  static constexpr int kShared = kQBytes > 3 * kMergeBytes ? kQBytes : 3 * kMergeBytes;
+  // at the end of an item: a warp's statistics, and three quarters of its sums, for the other warps to join
+  static constexpr int kStatBytes = 32 * kNT * 16, kQuarter = kMt / kDecodeWarps, kQuarterBytes = 32 * kNT * kQuarter * 16;
+  static constexpr int kMergeBytes = kDecodeWarps * (kStatBytes + 3 * kQuarterBytes);
+  static constexpr int kShared = kQBytes > kMergeBytes ? kQBytes : kMergeBytes;
   // two thread blocks an SM need 113 KB each at most; the widest form runs alone with a deeper ring
   static constexpr int kRing = kF32 ? (kNT == 2 ? 6 : 3) : (kNT == 2 ? 5 : 6);
   static constexpr int kPerSm = kF32 && kNT == 2 ? 1 : 2;
@@ -101,19 +103,23 @@ struct DecodeCfg {
   static constexpr int kSlot = kHeads * (kHd + 2);  // floats of a piece: [heads][hd], then maxima, then sums
 };
 
-// A place in the list of tiles
+// A tile in the list
 struct TilePos {
+  int64_t x;                           // its place
   int seq, chunk, tile, tiles, keys;  // chunk: kv head and piece of its group; tiles, keys: of the sequence
 };
 
 template <typename Cfg>
 __device__ __forceinline__ void next_tile(TilePos& t, const DecodeParams& p) {
+  ++t.x;
   if (++t.tile < t.tiles) return;
+  t.x += kItemUnits;
   t.tile = 0;
   if (++t.chunk < p.n_kv * p.chunks) return;
   t.chunk = 0;
-  do {  // the caller stops before the last sequence with keys ends
-    if (++t.seq >= p.n_seqs) {
+  do {
+    if (++t.seq >= p.n_seqs) {  // behind the last item: nobody's tile
+      t.seq = p.n_seqs - 1;
       t.tiles = t.keys = 0;
       return;
     }
@@ -148,7 +154,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
   for (int s = s0; s < s1; ++s) {
     const int len = p.lens[s];
     bad |= len > ((int64_t)p.max_pages << p.page_shift);
-    mine += seq_tiles(len, p.max_pages, p.page_shift, Cfg::kTile);
+    mine += item_units(seq_tiles(len, p.max_pages, p.page_shift, Cfg::kTile));
   }
   int incl = mine;
 #pragma unroll
@@ -173,7 +179,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     if (active && at <= x0 && x0 < at + (int64_t)mine * items) {
       int s = s0;
       for (;; ++s) {
-        const int64_t n = (int64_t)seq_tiles(p.lens[s], p.max_pages, p.page_shift, Cfg::kTile) * items;
+        const int64_t n = (int64_t)item_units(seq_tiles(p.lens[s], p.max_pages, p.page_shift, Cfg::kTile)) * items;
         if (x0 < at + n) break;
         at += n;
       }
@@ -189,27 +195,34 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
   }
   if (bad && blockIdx.x == 0) record_dev_error(kErrIndex);
   __syncthreads();
-  if (!active) {
+  TilePos use;
+  use.x = x1;
+  if (active) {
+    use.seq = (int)start_s[0];
+    use.keys = seq_keys(p.lens[use.seq], p.max_pages, p.page_shift);
+    use.tiles = (use.keys + Cfg::kTile - 1) / Cfg::kTile;
+    const int64_t rest = x0 - start_s[1];
+    use.chunk = (int)quotient(rest, item_units(use.tiles));
+    use.tile = (int)(rest - (int64_t)use.chunk * item_units(use.tiles));
+    use.x = x0;
+    if (use.tile >= use.tiles) {  // the run begins with places behind an item
+      use.x = x0 - use.tile + use.tiles - 1;
+      use.tile = use.tiles - 1;
+      next_tile<Cfg>(use, p);
+    }
+  }
+  if (use.x >= x1) {
     if (threadIdx.x == 0) p.meta[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
     return;
   }
-  TilePos use;
-  use.seq = (int)start_s[0];
-  use.keys = seq_keys(p.lens[use.seq], p.max_pages, p.page_shift);
-  use.tiles = (use.keys + Cfg::kTile - 1) / Cfg::kTile;
-  {
-    const int64_t rest = x0 - start_s[1];
-    use.chunk = (int)(rest / use.tiles);
-    use.tile = (int)(rest - (int64_t)use.chunk * use.tiles);
-  }
   TilePos get = use;
-  const int n_tiles = (int)(x1 - x0);
 
   // ---- copies. Lane r holds the place of key r of the tile to be fetched: its row in the cache, or -1
   const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.k);
   const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.v);
   constexpr int kLanesPerRow = kRow / 16, kRowsPerCopy = 32 / kLanesPerRow, kCopies = kKeys / kRowsPerCopy;
-  int fetched = 0;        // tiles whose keys have been requested
+  uint32_t fetched = 0;   // tiles whose keys have been requested
+  bool values_due = false;
   int64_t place = -1;     // of this lane's key, of the tile being fetched
   int next_page = -1;     // page of this lane's key in the tile after it, looked up ahead of its use
   auto look_up = [&](const TilePos& t) {
@@ -235,24 +248,22 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     cp_async_commit();
   };
   auto fetch_keys = [&](int slot) {
-    if (fetched < n_tiles) {
+    values_due = get.x < x1;
+    if (values_due) {
       const int key = get.tile * Cfg::kTile + warp * kKeys + (lane & (kKeys - 1));
       place = next_page < 0 ? -1 : (((int64_t)next_page * p.n_kv + get.chunk / p.chunks) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
       const uint32_t seen = __ballot_sync(0xffffffffu, place >= 0);
       if (lane == 0) seen_s[fetched & 7] = seen;
-      copy_unit(kc, slot, false);
       ++fetched;
-      if (fetched < n_tiles) {
-        next_tile<Cfg>(get, p);
-        next_page = look_up(get);
-      }
+      next_tile<Cfg>(get, p);
+      next_page = get.x < x1 ? look_up(get) : -1;
+      copy_unit(kc, slot, false);
     } else {
       cp_async_commit();
-      ++fetched;
     }
   };
   auto fetch_values = [&](int slot) {  // of the tile whose keys were fetched last
-    if (fetched <= n_tiles) copy_unit(vc, slot, true);
+    if (values_due) copy_unit(vc, slot, true);
     else cp_async_commit();
   };
   next_page = look_up(get);
@@ -264,22 +275,31 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     keys_next = !keys_next;
     in = in + 1 == kRing ? 0 : in + 1;
   };
-  for (int i = 0; i < kRing; ++i) request();
 
   // ---- one item after the other
   float m[kNT][2], l[kNT][2], o[kNT][kMt][4];
   float factor[kNT][2];
   int nh = 0;
-  int64_t item_first = x0 - use.tile;  // first tile of the item in the list
-  auto begin_item = [&]() {
-    const int kvh = use.chunk / p.chunks, part = use.chunk % p.chunks;
+  int64_t item_first = use.x - use.tile;  // first place of the item in the list
+  // the query heads of an item, two (or four) for each warp: read ahead, put into the order of the instruction's operand later
+  constexpr int kPer = kHd / 32, kMine = kHeads / kDecodeWarps;
+  float qx[kMine][kPer];
+  auto load_q = [&]() {
+    const int kvh = use.chunk / p.chunks, part = use.chunk - kvh * p.chunks;
     nh = min(kHeads, p.group - part * kHeads);
-    const A* q = reinterpret_cast<const A*>(p.q) + use.seq * p.q_stride + (int64_t)(kvh * p.group + part * kHeads) * kHd;
-    constexpr int kPer = kHd / 32;
-    for (int h = warp; h < kHeads; h += kDecodeWarps) {
-      float x[kPer];
+    const A* q = reinterpret_cast<const A*>(p.q) + use.seq * p.q_stride + (int64_t)(kvh * p.group + part * kHeads) * kHd + lane * kPer;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) x[i] = h < nh ? to_f32(q[h * kHd + lane * kPer + i]) : 0.f;
+    for (int j = 0; j < kMine; ++j) {
+      const int h = warp + j * kDecodeWarps;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) qx[j][i] = h < nh ? to_f32(q[h * kHd + i]) : 0.f;
+    }
+  };
+  auto begin_item = [&]() {
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      const int h = warp + j * kDecodeWarps;
+      float(&x)[kPer] = qx[j];
       float f = p.scale * 1.4426950408889634f;
       if constexpr (Cfg::kWideAct && std::is_same<C, __half>::value) {  // a power of two that brings the row into f16's range
         float top = 0.f;
@@ -297,18 +317,17 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
 #pragma unroll
       for (int i = 0; i < kPer; i += 2) {
         const int d = lane * kPer + i;
+        uint32_t* w = reinterpret_cast<uint32_t*>(shared);
         if constexpr (kF32) {
-          uint32_t* w = reinterpret_cast<uint32_t*>(shared);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int dd = d + j, at = ((nt * kParts * kKs + dd / 8) * 32 + n * 4 + (dd & 3)) * 2 + ((dd >> 2) & 1);
+          for (int k = 0; k < 2; ++k) {
+            const int dd = d + k, at = ((nt * kParts * kKs + dd / 8) * 32 + n * 4 + (dd & 3)) * 2 + ((dd >> 2) & 1);
             uint32_t hi, lo;
-            split_tf32(__float_as_uint(x[i + j]), hi, lo);
+            split_tf32(__float_as_uint(x[i + k]), hi, lo);
             w[at] = hi;
             w[at + kKs * 64] = lo;
           }
         } else {
-          uint32_t* w = reinterpret_cast<uint32_t*>(shared);
           const int at = ((nt * kParts * kKs + d / 16) * 32 + n * 4 + ((d & 7) >> 1)) * 2 + ((d >> 3) & 1);
           float a = x[i], b = x[i + 1];
 #pragma unroll
@@ -337,8 +356,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     for (int nt = 0; nt < kNT; ++nt) factor[nt][0] = factor_s[nt * 8 + 2 * tq], factor[nt][1] = factor_s[nt * 8 + 2 * tq + 1];
   };
 
-  // the four warps' results, added up by the first; whole items are finished, pieces are left for paged_join_kernel
-  auto end_item = [&](int64_t x_end, bool item_done) {
+  // The four warps' results joined, each warp a quarter of the columns; whole items are finished, pieces are left for
+  // paged_join_kernel. done: the item ends here; last: so does this block's run
+  auto end_item = [&](const TilePos& at, int heads, bool done, bool last) {
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
@@ -346,78 +366,81 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], off);
     __syncthreads();  // nobody reads q any more
-    float4* box = reinterpret_cast<float4*>(shared);
-    constexpr int kBox = 32 * kNT * (kMt + 1);
-    if (warp) {
-      float4* b = box + (warp - 1) * kBox;
+    constexpr int kQ = Cfg::kQuarter;
+    float4* stats = reinterpret_cast<float4*>(shared) + lane;                                 // [warp][nt][lane]
+    float4* box = reinterpret_cast<float4*>(shared + kDecodeWarps * Cfg::kStatBytes) + lane;  // [to][from][nt][tile of the quarter][lane]
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
-        b[nt * (kMt + 1) * 32 + lane] = make_float4(m[nt][0], m[nt][1], l[nt][0], l[nt][1]);
+    for (int nt = 0; nt < kNT; ++nt) {
+      stats[(warp * kNT + nt) * 32] = make_float4(m[nt][0], m[nt][1], l[nt][0], l[nt][1]);
 #pragma unroll
-        for (int t = 0; t < kMt; ++t) b[(nt * (kMt + 1) + 1 + t) * 32 + lane] = make_float4(o[nt][t][0], o[nt][t][1], o[nt][t][2], o[nt][t][3]);
+      for (int t = 0; t < kMt; ++t) {
+        const int to = t / kQ, from = warp - (warp > to ? 1 : 0);
+        if (to != warp) box[(((to * 3 + from) * kNT + nt) * kQ + t % kQ) * 32] = make_float4(o[nt][t][0], o[nt][t][1], o[nt][t][2], o[nt][t][3]);
       }
     }
     __syncthreads();
-    if (warp == 0) {
-      const int kvh = use.chunk / p.chunks, part = use.chunk % p.chunks;
-      const bool whole = item_done && item_first >= x0;
-      float* slot = p.slots + (int64_t)split_slot(total, blocks, blockIdx.x, item_first) * Cfg::kSlot;
-      A* dst = reinterpret_cast<A*>(p.out) + ((int64_t)use.seq * p.n_heads + kvh * p.group + part * kHeads) * kHd;
+    const int kvh = at.chunk / p.chunks, part = at.chunk - kvh * p.chunks;
+    const bool whole = done && item_first >= x0;
+    float* slot = p.slots + (int64_t)split_slot(total, blocks, blockIdx.x, item_first) * Cfg::kSlot;
+    A* dst = reinterpret_cast<A*>(p.out) + ((int64_t)at.seq * p.n_heads + kvh * p.group + part * kHeads) * kHd;
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
-        float4 st[3];
-        float top[2] = {m[nt][0], m[nt][1]};
+    for (int nt = 0; nt < kNT; ++nt) {
+      float4 st[kDecodeWarps];
+      float top[2] = {-INFINITY, -INFINITY}, f[kDecodeWarps][2], sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < 3; ++w) {
-          st[w] = box[w * kBox + nt * (kMt + 1) * 32 + lane];
-          top[0] = fmaxf(top[0], st[w].x), top[1] = fmaxf(top[1], st[w].y);
+      for (int w = 0; w < kDecodeWarps; ++w) {
+        st[w] = stats[(w * kNT + nt) * 32];
+        top[0] = fmaxf(top[0], st[w].x), top[1] = fmaxf(top[1], st[w].y);
+      }
+      const float ref[2] = {top[0] == -INFINITY ? 0.f : top[0], top[1] == -INFINITY ? 0.f : top[1]};
+#pragma unroll
+      for (int w = 0; w < kDecodeWarps; ++w) {
+        f[w][0] = exp2f(st[w].x - ref[0]), f[w][1] = exp2f(st[w].y - ref[1]);
+        sum[0] += st[w].z * f[w][0], sum[1] += st[w].w * f[w][1];
+      }
+      const float inv[2] = {sum[0] == 0.f ? 0.f : 1.f / sum[0], sum[1] == 0.f ? 0.f : 1.f / sum[1]};
+      const float own[2] = {exp2f(m[nt][0] - ref[0]), exp2f(m[nt][1] - ref[1])};
+#pragma unroll
+      for (int q = 0; q < kQ; ++q) {
+        float r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float lower = warp & 1 ? o[nt][kQ + q][i] : o[nt][q][i], upper = warp & 1 ? o[nt][3 * kQ + q][i] : o[nt][2 * kQ + q][i];
+          r[i] = (warp & 2 ? upper : lower) * own[i & 1];
         }
-        float own[2], f[3][2], sum[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float ref = top[j] == -INFINITY ? 0.f : top[j];
-          own[j] = exp2f(m[nt][j] - ref);
-          sum[j] = l[nt][j] * own[j];
-#pragma unroll
-          for (int w = 0; w < 3; ++w) {
-            f[w][j] = exp2f((j ? st[w].y : st[w].x) - ref);
-            sum[j] += (j ? st[w].w : st[w].z) * f[w][j];
-          }
+        for (int w = 0; w < kDecodeWarps; ++w) {
+          if (w == warp) continue;
+          const float4 b = box[(((warp * 3 + w - (w > warp ? 1 : 0)) * kNT + nt) * kQ + q) * 32];
+          r[0] += b.x * f[w][0], r[1] += b.y * f[w][1], r[2] += b.z * f[w][0], r[3] += b.w * f[w][1];
         }
-        const float inv[2] = {sum[0] == 0.f ? 0.f : 1.f / sum[0], sum[1] == 0.f ? 0.f : 1.f / sum[1]};
 #pragma unroll
-        for (int t = 0; t < kMt; ++t) {
-          float r[4] = {o[nt][t][0] * own[0], o[nt][t][1] * own[1], o[nt][t][2] * own[0], o[nt][t][3] * own[1]};
-#pragma unroll
-          for (int w = 0; w < 3; ++w) {
-            const float4 b = box[w * kBox + (nt * (kMt + 1) + 1 + t) * 32 + lane];
-            r[0] += b.x * f[w][0], r[1] += b.y * f[w][1], r[2] += b.z * f[w][0], r[3] += b.w * f[w][1];
+        for (int i = 0; i < 4; ++i) {
+          const int h = nt * 8 + 2 * tq + (i & 1), d = 16 * (warp * kQ + q) + g + 8 * (i >> 1);
+          if (h < heads) {
+            if (whole) dst[h * kHd + d] = from_f32<A>(r[i] * inv[i & 1]);
+            else slot[h * kHd + d] = r[i];
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int h = nt * 8 + 2 * tq + (i & 1), d = 16 * t + g + 8 * (i >> 1);
-            if (h < nh) {
-              if (whole) dst[h * kHd + d] = from_f32<A>(r[i] * inv[i & 1]);
-              else slot[h * kHd + d] = r[i];
-            }
-          }
-        }
-        if (!whole && g == 0) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) slot[kHeads * kHd + nt * 8 + 2 * tq + j] = top[j], slot[kHeads * (kHd + 1) + nt * 8 + 2 * tq + j] = sum[j];
         }
       }
-      if (x_end == x1 && lane == 0) {  // the end of this block's run: does an item go on from here that began here?
-        const bool first_piece = !item_done && item_first >= x0;
-        p.meta[2 * blockIdx.x] = make_int4(first_piece ? use.seq : -1, use.chunk, use.tiles, blocks);
-        p.meta[2 * blockIdx.x + 1] = make_int4((int)(item_first & 0xffffffff), (int)(item_first >> 32), (int)(total & 0xffffffff), (int)(total >> 32));
+      if (!whole && warp == 0 && g == 0) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) slot[kHeads * kHd + nt * 8 + 2 * tq + j] = top[j], slot[kHeads * (kHd + 1) + nt * 8 + 2 * tq + j] = sum[j];
       }
+    }
+    if (last && threadIdx.x == 0) {  // the end of this block's run: does an item go on from here that began here?
+      const bool first_piece = !done && item_first >= x0;
+      p.meta[2 * blockIdx.x] = make_int4(first_piece ? at.seq : -1, at.chunk, at.tiles, blocks);
+      p.meta[2 * blockIdx.x + 1] = make_int4((int)(item_first & 0xffffffff), (int)(item_first >> 32), (int)(total & 0xffffffff), (int)(total >> 32));
     }
     __syncthreads();
   };
 
+  load_q();
+#pragma unroll 1
+  for (int i = 0; i < kRing; ++i) request();
   begin_item();
-  for (int i = 0; i < n_tiles; ++i) {
+  for (uint32_t i = 0;; ++i) {
     // scores
     cp_async_wait<kRing - 1>();
     __syncwarp();
@@ -577,17 +600,17 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     out_slot = out_slot + 1 == kRing ? 0 : out_slot + 1;
 
     // the end of the item, or of this block's run
-    const int64_t x = x0 + i + 1;
-    const bool item_done = use.tile + 1 == use.tiles;
-    if (item_done || x == x1) {
-      end_item(x, item_done);
-      if (x < x1) {
-        next_tile<Cfg>(use, p);
-        item_first = x;
-        begin_item();
-      }
-    } else {
-      ++use.tile;
+    const bool done = use.tile + 1 == use.tiles;
+    const TilePos at = use;
+    next_tile<Cfg>(use, p);
+    if (done || use.x >= x1) {
+      const bool last = use.x >= x1;
+      const int heads = nh;
+      if (!last) load_q();
+      end_item(at, heads, done, last);
+      if (last) break;
+      item_first = use.x;
+      begin_item();
     }
   }
   cp_async_wait<0>();

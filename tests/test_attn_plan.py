@@ -20,6 +20,7 @@ void prompt_block(const int* cu, int n, long long rows, long long slot, int size
   out->first = b.first, out->len = b.len, out->row = b.row;
 }
 long long prompt_slots(long long rows, int n, int size) { return fq::prompt_slots(rows, n, size); }
+int item_units(int tiles) { return fq::item_units(tiles); }
 int seq_tiles(int len, int max_pages, int shift, int tile) { return fq::seq_tiles(len, max_pages, shift, tile); }
 }
 """
@@ -115,10 +116,11 @@ def test_every_piece_has_a_slot_of_its_own_and_is_joined_once(plan):
         for n in lens:
             for _ in range(items if n else 0):
                 spans.append((at, at + n))
-                at += n
+                at += plan.item_units(n)
         total = at
         if not total:
             continue
+        assert plan.item_units(0) == 0 and plan.item_units(5) > 5
         blocks = min(total, rng.choice((1, 2, 3, 8, 40)))
         whole, slots, meta = set(), {}, {}
         for b in range(blocks):
@@ -134,7 +136,7 @@ def test_every_piece_has_a_slot_of_its_own_and_is_joined_once(plan):
                     slot = plan.split_slot(total, blocks, b, i0)
                     assert slot not in slots and slot // 2 == b
                     slots[slot] = (k, a, z)
-                    if z == x1 and not done and i0 >= x0:
+                    if not done and i0 >= x0:
                         meta[b] = k
         joined = set()
         for b, k in meta.items():
