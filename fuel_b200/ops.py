@@ -6,8 +6,6 @@ the reference's quantized storage API (fuel-backend-contract/src/quantized.rs:29
 """
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import _lib
@@ -18,16 +16,11 @@ _raw_stream = torch._C._cuda_getCurrentRawStream   # the handle alone: a Stream 
 _OUT_TYPES = {torch.float32: GgmlDType.F32, torch.float16: GgmlDType.F16, torch.bfloat16: GgmlDType.BF16}
 _TYPE_IDS = {t: int(g) for t, g in _OUT_TYPES.items()}
 _current_device = torch._C._cuda_getDevice
-_HERE = contextlib.nullcontext()
+_I32, _F32 = torch.int32, torch.float32
 
 
 def _stream() -> int:
     return _raw_stream(torch.cuda.current_device())
-
-
-def _on(dev: int):
-    """The device of the operands made current, which costs microseconds only where it is not."""
-    return _HERE if dev == _current_device() else torch.cuda.device(dev)
 
 
 def _need_cuda(t: torch.Tensor, name: str) -> None:
@@ -155,13 +148,13 @@ def _heads(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int) -> int:
         raise ValueError(f"{name} must be a {dtype} tensor of [rows, heads, head_dim]")
     rows, heads, hd = t.shape
     row, head, one = t.stride()
-    if (one != 1 and hd > 1) or (head != hd and heads > 1):
+    if one != 1 or (head != hd and heads > 1):
         raise ValueError(f"the heads of a row of {name} must be contiguous")
     return row if rows > 1 else heads * hd
 
 
 def _indices(t: torch.Tensor, name: str, dims: int, dev: int) -> None:
-    if t.dtype is not torch.int32 or t.dim() != dims or t.get_device() != dev or not t.is_contiguous():
+    if t.dtype is not _I32 or t.get_device() != dev or t.dim() != dims or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of {dims} dimension(s) on the device of the other operands")
 
 
@@ -201,6 +194,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, kcache: torch.Tensor, vcache:
     queries (q_out, or a new tensor) if q is given; k_out, if given, receives the rotated keys. The rows of q, k and v may be
     column ranges of one stacked projection."""
     dev, dtype = k.get_device(), k.dtype
+    if dev >= 0 and dev != _current_device():
+        with torch.cuda.device(dev):
+            return paged_append(k, v, kcache, vcache, page_table, positions, cos, sin, seq_ids=seq_ids, q=q, q_out=q_out, k_out=k_out)
     ks, vs = _heads(k, "k", dtype, dev), _heads(v, "v", dtype, dev)
     shape = k.shape
     if dtype not in _TYPE_IDS or v.shape != shape:
@@ -215,8 +211,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, kcache: torch.Tensor, vcache:
         _indices(seq_ids, "seq_ids", 1, dev)
     if positions.shape[0] != rows or (seq_ids is not None and seq_ids.shape[0] != rows):
         raise ValueError("positions and seq_ids need one entry per row")
-    for t, name in ((cos, "cos"), (sin, "sin")):
-        if t.dtype is not torch.float32 or t.dim() != 2 or t.shape[1] != hd or t.get_device() != dev or not t.is_contiguous():
+    for t, name in (cos, "cos"), (sin, "sin"):
+        if t.dtype is not _F32 or t.dim() != 2 or t.shape[1] != hd or t.get_device() != dev or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous f32 table of [positions, head_dim]")
     heads = qs = 0
     if q is not None:
@@ -228,13 +224,12 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, kcache: torch.Tensor, vcache:
     if k_out is not None:
         _result(k_out, k, "k_out")
     seqs, width = page_table.shape
-    with _on(dev):
-        status = _L.fuelq_paged_append(_TYPE_IDS[dtype], _TYPE_IDS[kcache.dtype], k.data_ptr(), ks, v.data_ptr(), vs,
-                                       None if q is None else q.data_ptr(), qs, None if q is None else q_out.data_ptr(),
-                                       None if k_out is None else k_out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(),
-                                       page_table.data_ptr(), None if seq_ids is None else seq_ids.data_ptr(), positions.data_ptr(),
-                                       cos.data_ptr(), sin.data_ptr(), rows, seqs, heads, kv, hd, page, pages, width,
-                                       min(cos.shape[0], sin.shape[0]), _raw_stream(dev))
+    status = _L.fuelq_paged_append(_TYPE_IDS[dtype], _TYPE_IDS[kcache.dtype], k.data_ptr(), ks, v.data_ptr(), vs,
+                                   None if q is None else q.data_ptr(), qs, None if q is None else q_out.data_ptr(),
+                                   None if k_out is None else k_out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(),
+                                   page_table.data_ptr(), None if seq_ids is None else seq_ids.data_ptr(), positions.data_ptr(),
+                                   cos.data_ptr(), sin.data_ptr(), rows, seqs, heads, kv, hd, page, pages, width,
+                                   min(cos.shape[0], sin.shape[0]), _raw_stream(dev))
     if status:
         _lib.check(status, "fuelq_paged_append")
     return None if q is None else q_out
@@ -252,6 +247,9 @@ def paged_attn_decode(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tenso
     """Attention of one new token per sequence, q [sequences, heads, head_dim] already rotated, over the first seq_lens[s]
     positions of its pages. A length of zero, a free slot of the batch, gives zeros. Default scale: 1 / sqrt(head_dim)."""
     dev, dtype = q.get_device(), q.dtype
+    if dev >= 0 and dev != _current_device():
+        with torch.cuda.device(dev):
+            return paged_attn_decode(q, kcache, vcache, page_table, seq_lens, scale, out, workspace)
     qs = _heads(q, "q", dtype, dev)
     n, heads, hd = q.shape
     pages, kv, page, chd = _paged(kcache, vcache, dev)
@@ -264,11 +262,10 @@ def paged_attn_decode(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tenso
         raise ValueError("page_table and seq_lens need one row per sequence")
     out = _result(out, q, "out")
     workspace = _scratch(workspace, _L.fuelq_paged_attn_workspace_bytes(n, heads, kv, hd) if workspace is None else 0, q)
-    with _on(dev):
-        status = _L.fuelq_paged_attn_decode(_TYPE_IDS[dtype], _TYPE_IDS[kcache.dtype], q.data_ptr(), qs, kcache.data_ptr(),
-                                            vcache.data_ptr(), out.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), n, heads,
-                                            kv, hd, page, pages, width, hd ** -0.5 if scale is None else scale,
-                                            workspace.data_ptr(), workspace.nbytes, _raw_stream(dev))
+    status = _L.fuelq_paged_attn_decode(_TYPE_IDS[dtype], _TYPE_IDS[kcache.dtype], q.data_ptr(), qs, kcache.data_ptr(),
+                                        vcache.data_ptr(), out.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), n, heads,
+                                        kv, hd, page, pages, width, hd ** -0.5 if scale is None else scale,
+                                        workspace.data_ptr(), workspace.nbytes, _raw_stream(dev))
     if status:
         _lib.check(status, "fuelq_paged_attn_decode")
     return out
@@ -286,6 +283,9 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: t
     and of k, v [rows, kv_heads, head_dim] are sequence s. Rows behind the last sequence are padding: not read, and left as
     they were in `out`. Default scale: 1 / sqrt(head_dim)."""
     dev, dtype = q.get_device(), q.dtype
+    if dev >= 0 and dev != _current_device():
+        with torch.cuda.device(dev):
+            return prompt_attn(q, k, v, cu_seqlens, scale, out, workspace)
     qs, ks, vs = _heads(q, "q", dtype, dev), _heads(k, "k", dtype, dev), _heads(v, "v", dtype, dev)
     rows, heads, hd = q.shape
     shape = k.shape
@@ -298,10 +298,9 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: t
         raise ValueError("cu_seqlens needs n_seqs + 1 entries")
     out = _result(out, q, "out")
     workspace = _scratch(workspace, _L.fuelq_prompt_attn_workspace_bytes(_TYPE_IDS[dtype], rows, heads, kv, hd) if workspace is None else 0, q)
-    with _on(dev):
-        status = _L.fuelq_prompt_attn(_TYPE_IDS[dtype], q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(),
-                                      cu_seqlens.data_ptr(), seqs, rows, heads, kv, hd, hd ** -0.5 if scale is None else scale,
-                                      workspace.data_ptr(), workspace.nbytes, _raw_stream(dev))
+    status = _L.fuelq_prompt_attn(_TYPE_IDS[dtype], q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(),
+                                  cu_seqlens.data_ptr(), seqs, rows, heads, kv, hd, hd ** -0.5 if scale is None else scale,
+                                  workspace.data_ptr(), workspace.nbytes, _raw_stream(dev))
     if status:
         _lib.check(status, "fuelq_prompt_attn")
     return out
