@@ -9,8 +9,8 @@
 // The 5th-generation instruction has no use here: its 128-row tile would hold 8 of 128 rows of work.
 // Accuracy: 32-bit activations are split into parts that the cache's type holds exactly and multiplied part by part into one
 // f32 sum: f16 caches take q and p as two f16 parts (22 bits; q scaled by a power of two into range), bf16 caches as three bf16
-// parts (24 bits), f32 caches everything as two tf32 parts, low times low left out (21 bits). 16-bit activations are their
-// own single part; p is then rounded once to their type, half a step of the result's own rounding.
+// parts (24 bits), f32 caches everything as two tf32 parts (22 bits). The instruction's f32 sums round towards zero, which shows
+// over a long row, so they are kept short and joined by additions that round to nearest. 16-bit activations are their own single part; p is then rounded once to their type, half a step of the result's own rounding.
 // Work: tiles of kTile keys of all (sequence, kv head) items, laid end to end and dealt out evenly (attn_plan.h), so that one
 // long sequence, many short ones and any mixture fill the device alike. A warp owns 16 (head_dim 64: 32) keys of each
 // tile and runs by itself: its own ring of cp.async copies that runs on across items, its own running maximum and sums; the
@@ -67,10 +67,11 @@ __device__ __forceinline__ void mma8_tf32(float (&d)[4], const uint32_t (&a)[4],
   asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// two tf32 parts of a float: the upper 10 mantissa bits, and what they leave (exact; the instruction takes its upper bits)
+// two tf32 parts of a float: the upper 10 mantissa bits, and what they leave (exact in f32) rounded to as many: half of the last
+// place that the instruction reads is added, and it ignores the rest
 __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
   hi = x & 0xffffe000u;
-  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
+  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi)) + 0x1000u;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     float s[kSub][kNT][4];
 #pragma unroll
     for (int sub = 0; sub < kSub; ++sub) {
-      float acc[2][kNT][4] = {};
+      float acc[4][kNT][4] = {};  // the instruction's sums round towards zero: four short ones, low parts before high ones
       const int row = sub * 16 + (lane & 15);
 #pragma unroll
       for (int ks = 0; ks < kKs; ++ks) {
@@ -462,9 +463,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
           for (int nt = 0; nt < kNT; ++nt) {
             const uint2 qh = reinterpret_cast<const uint2*>(shared)[(nt * 2 * kKs + ks) * 32 + lane];
             const uint2 ql = reinterpret_cast<const uint2*>(shared)[((nt * 2 + 1) * kKs + ks) * 32 + lane];
-            mma8_tf32(acc[ks & 1][nt], lo, qh.x, qh.y);
-            mma8_tf32(acc[ks & 1][nt], hi, ql.x, ql.y);
-            mma8_tf32(acc[ks & 1][nt], hi, qh.x, qh.y);
+            mma8_tf32(acc[ks & 3][nt], lo, ql.x, ql.y);
+            mma8_tf32(acc[ks & 3][nt], lo, qh.x, qh.y);
+            mma8_tf32(acc[ks & 3][nt], hi, ql.x, ql.y);
+            mma8_tf32(acc[ks & 3][nt], hi, qh.x, qh.y);
           }
         } else {
 #pragma unroll
@@ -472,14 +474,14 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
 #pragma unroll
             for (int part = kParts - 1; part >= 0; --part) {
               const uint2 b = reinterpret_cast<const uint2*>(shared)[((nt * kParts + part) * kKs + ks) * 32 + lane];
-              mma16(acc[ks & 1][nt], a, b.x, b.y, C());
+              mma16(acc[ks & 3][nt], a, b.x, b.y, C());
             }
         }
       }
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[sub][nt][j] = acc[0][nt][j] + acc[1][nt][j];
+        for (int j = 0; j < 4; ++j) s[sub][nt][j] = (acc[0][nt][j] + acc[1][nt][j]) + (acc[2][nt][j] + acc[3][nt][j]);
     }
     const uint32_t seen = seen_s[i & 7];
     __syncwarp();  // the slot and the word above are free
@@ -561,11 +563,13 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     __syncwarp();
     uint8_t* vunit = ring + out_slot * kUnit;
     const uint32_t vbase = smem_u32(vunit);
+    // a tile's products by themselves, then added to O with a sum that rounds to nearest
 #pragma unroll
-    for (int sub = 0; sub < kSub; ++sub) {
-      if constexpr (kF32) {
+    for (int t = 0; t < kMt; ++t) {
+      float tile[kNT][4] = {};
 #pragma unroll
-        for (int t = 0; t < kMt; ++t)
+      for (int sub = 0; sub < kSub; ++sub) {
+        if constexpr (kF32) {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {  // keys 8 * half ..
             uint32_t hi[4], lo[4];
@@ -577,23 +581,26 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
             }
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt) {
-              mma8_tf32(o[nt][t], lo, pf[sub][nt][0][2 * half], pf[sub][nt][0][2 * half + 1]);
-              mma8_tf32(o[nt][t], hi, pf[sub][nt][1][2 * half], pf[sub][nt][1][2 * half + 1]);
-              mma8_tf32(o[nt][t], hi, pf[sub][nt][0][2 * half], pf[sub][nt][0][2 * half + 1]);
+              mma8_tf32(tile[nt], lo, pf[sub][nt][1][2 * half], pf[sub][nt][1][2 * half + 1]);
+              mma8_tf32(tile[nt], lo, pf[sub][nt][0][2 * half], pf[sub][nt][0][2 * half + 1]);
+              mma8_tf32(tile[nt], hi, pf[sub][nt][1][2 * half], pf[sub][nt][1][2 * half + 1]);
+              mma8_tf32(tile[nt], hi, pf[sub][nt][0][2 * half], pf[sub][nt][0][2 * half + 1]);
             }
           }
-      } else {
-        const int row = sub * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
-#pragma unroll
-        for (int t = 0; t < kMt; ++t) {
+        } else {
+          const int row = sub * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
           uint32_t a[4];
           ldsm4_t(vbase + row * kRow + (((t * 2 + ((lane >> 3) & 1)) ^ (row & 7)) * 16), a);
 #pragma unroll
           for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-            for (int part = kParts - 1; part >= 0; --part) mma16(o[nt][t], a, pf[sub][nt][part][0], pf[sub][nt][part][1], C());
+            for (int part = kParts - 1; part >= 0; --part) mma16(tile[nt], a, pf[sub][nt][part][0], pf[sub][nt][part][1], C());
         }
       }
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nt][t][i] += tile[nt][i];
     }
     __syncwarp();
     request();

@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
 
   if (warp >= 12) set_regs_down<kPfaOtherRegs>();
   if (warp == 12 || warp == 15) {
-    // ---------------- copies: Q and K, V. Units of a tile: upper part, lower part
+    // ---------------- copies: Q and K, V. Units of a tile: lower part, upper part
     if (lane == 0) {
       const bool values = warp == 15;
       uint64_t* full = values ? ctl->v_full : ctl->k_full;
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
             const uint32_t s = unit % kPfaRing;
             if (unit >= kPfaRing && !(ok = wait(&empty[s], unit / kPfaRing - 1, kErrEmptyWait))) break;
             mbar_arrive_expect_tx(&full[s], kUnitBytes);
-            const int row = (int)((u / kUnits) * p.n_rows + it.first + j * kPaTile), piece = u % kUnits;
+            const int row = (int)((1 - u / kUnits) * p.n_rows + it.first + j * kPaTile), piece = u % kUnits;
             if (!values) {
               tma_load_3d(k_addr + s * kUnitBytes, &kmap, 64 * piece, kvh, row, &full[s]);
             } else {
@@ -265,22 +265,21 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
     bool ok = true;
     PromptItem it;
     for (; ok && get_item<true>(ctl->items, items, it, wait); ++items) {
-      // S of key tile j into its half of tensor memory: hi hi and lo hi of each unit of the upper part, then hi lo
+      // S of key tile j into its half of tensor memory. The small products come first, hi lo of each unit of the lower part, lo hi of
+      // the upper part's, then hi hi: sums that round towards zero do so eight times at their full size, not 24
       auto scores = [&](int j) {
         const uint32_t d = acc + ((steps + j) & 1) * kPaTile;
 #pragma unroll
-        for (int u = 0; u < 2 * kUnits; ++u) {
-          const uint32_t n = (steps + j) * 2 * kUnits + u, st = n % kPfaRing;
-          if (!ready(&ctl->k_full[st], n / kPfaRing, kErrFullWait)) return false;
-          const uint64_t b = k_desc + (uint64_t)(st * kUnitBytes >> 4);
+        for (int u = 0; u < 3 * kUnits; ++u) {
+          const int piece = u % kUnits;
+          const uint32_t n = (steps + j) * 2 * kUnits + (u < 2 * kUnits ? u : u - kUnits), st = n % kPfaRing;
+          if (u < 2 * kUnits && !ready(&ctl->k_full[st], n / kPfaRing, kErrFullWait)) return false;
+          const uint64_t a = q_desc + (uint64_t)(((u / kUnits == 1 ? kTileBytes : 0) + piece * kUnitBytes) >> 4), b = k_desc + (uint64_t)(st * kUnitBytes >> 4);
           if (leader) {
             tc_fence_after();
 #pragma unroll
-            for (int part = 0; part < (u < kUnits ? 2 : 1); ++part)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_bf16(d, q_desc + (uint64_t)((part * kTileBytes + (u % kUnits) * kUnitBytes + k * 32) >> 4), b + 2 * k, s_desc, (u | part | k) != 0);
-            umma_commit(&ctl->k_empty[st]);
+            for (int k = 0; k < 4; ++k) umma_bf16(d, a + 2 * k, b + 2 * k, s_desc, (u | k) != 0);
+            if (u / kUnits != 1) umma_commit(&ctl->k_empty[st]);
           }
         }
         if (leader) {
@@ -297,18 +296,17 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
         if (!(ok = ready(&ctl->p_full[step & 1], step / 2, kErrMmaWait))) break;
         if (step && !(ok = ready(&ctl->pv_empty, step - 1, kErrTmemWait))) break;
 #pragma unroll
-        for (int u = 0; u < 2 * kUnits; ++u) {
-          const uint32_t n = step * 2 * kUnits + u, st = n % kPfaRing;
-          if (ok) ok = ready(&ctl->v_full[st], n / kPfaRing, kErrFullWait);
+        for (int u = 0; u < 3 * kUnits; ++u) {  // in the same order
+          const int piece = u % kUnits;
+          const uint32_t n = step * 2 * kUnits + (u < 2 * kUnits ? u : u - kUnits), st = n % kPfaRing;
+          if (ok && u < 2 * kUnits) ok = ready(&ctl->v_full[st], n / kPfaRing, kErrFullWait);
+          const uint32_t a = (u / kUnits == 1 ? lo : hi) + piece * (kUnitKeys / 2);
           const uint64_t b = v_desc + (uint64_t)(st * kUnitBytes >> 4);
           if (ok && leader) {
             tc_fence_after();
 #pragma unroll
-            for (int part = 0; part < (u < kUnits ? 2 : 1); ++part)
-#pragma unroll
-              for (int k = 0; k < kUnitKeys / 16; ++k)
-                umma_f16_ts(d, (part ? lo : hi) + (u % kUnits) * (kUnitKeys / 2) + k * 8, b + (uint64_t)(k * 2048 >> 4), o_desc, (u | part | k) != 0);
-            umma_commit(&ctl->v_empty[st]);
+            for (int k = 0; k < kUnitKeys / 16; ++k) umma_f16_ts(d, a + k * 8, b + (uint64_t)(k * 2048 >> 4), o_desc, (u | k) != 0);
+            if (u / kUnits != 1) umma_commit(&ctl->v_empty[st]);
           }
         }
         if (ok && leader) umma_commit(&ctl->pv_full);
