@@ -172,7 +172,8 @@ int32_t launch_prompt_f32(const PromptArgs& r, cudaStream_t stream) {
       !make_rows_map(p.kp, 2 * r.n_rows, r.n_kv, kHd, (int64_t)r.n_kv * kHd, kPaTile, &kmap) ||
       !make_rows_map(p.vp, 2 * r.n_rows, r.n_kv, kHd, (int64_t)r.n_kv * kHd, Cfg::kUnitKeys, &vmap))
     return kLaunchFailure;
-  cudaError_t e = launch(prompt_split_kernel<kHd>, dim3((unsigned)slots, (unsigned)(r.n_heads + 2 * r.n_kv)), dim3(256), 0, stream, p);
+  cudaError_t e = launch(prompt_split_kernel<kHd>, dim3((unsigned)slots, (unsigned)(r.n_heads + 2 * r.n_kv)), dim3(32 * kSplitWarps), 0,
+                         stream, p);
   if (e != cudaSuccess) return kLaunchFailure;
   const dim3 grid((unsigned)(p.n_items < sms ? p.n_items : sms));
   return launch(kernel, grid, dim3(kPfaThreads), Cfg::kSmem, stream, p, qmap, kmap, vmap) == cudaSuccess ? kOk : kLaunchFailure;

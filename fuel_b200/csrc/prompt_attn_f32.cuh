@@ -43,8 +43,11 @@ struct PromptF32Params {
   int* marked;           // [n_kv][n_rows]     at the first row of a tile: does it hold a value that is not finite?
 };
 
+// one tile of 128 rows of one head; 64 registers, so that two blocks an SM have 64 KB each in flight (512 rows, 96 heads: one block of 256
+// threads an SM took 26 us)
+constexpr int kSplitWarps = 16;
 template <int kHd>
-__global__ void __launch_bounds__(256) prompt_split_kernel(const PromptF32Params p) {
+__global__ void __launch_bounds__(32 * kSplitWarps, 2) prompt_split_kernel(const PromptF32Params p) {
   constexpr int kPer = kHd / 32;
   pdl_launch_dependents();
   pdl_wait();
@@ -61,12 +64,12 @@ __global__ void __launch_bounds__(256) prompt_split_kernel(const PromptF32Params
   __half* dst = kind == 0 ? p.qp : kind == 1 ? p.kp : p.vp;
   const int64_t plane = p.n_rows * heads * kHd;
   const int rows = min(kPaTile, b.len - b.row);
-  constexpr int kMine = kPaTile / 8;  // rows of a warp
+  constexpr int kMine = kPaTile / kSplitWarps;  // rows of a warp
   alignas(16) float x[kMine][kPer];
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
-    const float* in = src + (b.first + b.row + warp + 8 * i) * stride + head * kHd + lane * kPer;
-    if (warp + 8 * i >= rows) {
+    const float* in = src + (b.first + b.row + warp + kSplitWarps * i) * stride + head * kHd + lane * kPer;
+    if (warp + kSplitWarps * i >= rows) {
 #pragma unroll
       for (int e = 0; e < kPer; ++e) x[i][e] = 0.f;
     } else if constexpr (kPer == 4) {
@@ -91,15 +94,15 @@ __global__ void __launch_bounds__(256) prompt_split_kernel(const PromptF32Params
     power[i] = top > 0.f ? ilogbf(top) - 14 : -1000;
     most = max(most, power[i]);
   }
-  __shared__ int most_s[8];
+  __shared__ int most_s[kSplitWarps];
   if (lane == 0) most_s[warp] = most;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; ++w) most = max(most, most_s[w]);
+  for (int w = 0; w < kSplitWarps; ++w) most = max(most, most_s[w]);
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
-    if (warp + 8 * i >= rows) break;
-    const int64_t row = b.first + b.row + warp + 8 * i;
+    if (warp + kSplitWarps * i >= rows) break;
+    const int64_t row = b.first + b.row + warp + kSplitWarps * i;
     // q, k: a row of zeros or nothing but denormals keeps a power in f32's range
     const int e0 = kind == 2 ? max(power[i], max(most - 100, -80)) : max(power[i], -112);
     const float down = exp2f((float)-e0);
