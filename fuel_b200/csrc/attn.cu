@@ -27,8 +27,9 @@ inline int page_shift_of(int page_size) {
 inline bool stride_ok(int64_t stride, int heads, int head_dim, int act) {
   return stride >= (int64_t)heads * head_dim && stride * type_bytes(act) % 16 == 0;
 }
-constexpr int64_t kMaxRows = 0x7fffffff, kMaxPromptRows = 1 << 30;
-constexpr int kMaxHeads = 32767;  // q, k and v heads together are a grid dimension
+constexpr int64_t kMaxRows = 0x7fffffff, kMaxPromptRows = (1 << 30) - 256;  // prompts: twice as many are a coordinate of a copy
+constexpr int64_t kMaxSlots = 1 << 26;  // empty sequences times heads, which a warp looks through while the others' waits run
+constexpr int kMaxHeads = 16383;  // q, k and v heads together are a grid dimension
 
 // f(activation type, cache type, head size) for one of the pairs the entries take
 template <typename A, typename C, typename F>
@@ -285,6 +286,7 @@ int32_t fuelq_prompt_attn(int32_t act_type, const void* q, int64_t q_stride, con
                           size_t workspace_bytes, void* stream) {
   if (!type_bytes(act_type) || (head_dim != 64 && head_dim != 128)) return kNotSupported;
   if (n_seqs < 0 || n_rows < 0 || n_rows > kMaxPromptRows || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !(scale >= 0.f) || std::isinf(scale)) return kInvalidProblem;
+  if ((int64_t)n_seqs * n_heads > kMaxSlots) return kNotSupported;
   if (n_seqs == 0 || n_rows == 0) return kOk;
   if (!q || !k || !v || !out || !cu_seqlens) return kInvalidProblem;
   if (!stride_ok(q_stride, n_heads, head_dim, act_type) || !stride_ok(k_stride, n_kv, head_dim, act_type) ||

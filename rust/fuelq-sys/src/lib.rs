@@ -102,6 +102,28 @@ unsafe extern "C" {
         out: *mut f32, stream: *mut c_void,
     ) -> i32;
 
+    // batches of sequences: paged key-value cache, attention over it, attention inside packed prompts
+    pub fn fuelq_paged_append(
+        act_type: i32, cache_type: i32, k: *const c_void, k_stride: i64, v: *const c_void, v_stride: i64, q: *const c_void,
+        q_stride: i64, q_out: *mut c_void, k_out: *mut c_void, kcache: *mut c_void, vcache: *mut c_void,
+        page_table: *const i32, seq_ids: *const i32, positions: *const i32, cos_table: *const f32, sin_table: *const f32,
+        n_rows: i64, n_seqs: i32, n_heads: i32, n_kv: i32, head_dim: i32, page_size: i32, n_pages: i32, max_pages: i32,
+        max_pos: i32, stream: *mut c_void,
+    ) -> i32;
+    pub fn fuelq_paged_attn_workspace_bytes(n_seqs: i32, n_heads: i32, n_kv: i32, head_dim: i32) -> usize;
+    pub fn fuelq_paged_attn_decode(
+        act_type: i32, cache_type: i32, q: *const c_void, q_stride: i64, kcache: *const c_void, vcache: *const c_void,
+        out: *mut c_void, page_table: *const i32, seq_lens: *const i32, n_seqs: i32, n_heads: i32, n_kv: i32, head_dim: i32,
+        page_size: i32, n_pages: i32, max_pages: i32, scale: f32, workspace: *mut c_void, workspace_bytes: usize,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn fuelq_prompt_attn_workspace_bytes(act_type: i32, n_rows: i64, n_heads: i32, n_kv: i32, head_dim: i32) -> usize;
+    pub fn fuelq_prompt_attn(
+        act_type: i32, q: *const c_void, q_stride: i64, k: *const c_void, k_stride: i64, v: *const c_void, v_stride: i64,
+        out: *mut c_void, cu_seqlens: *const i32, n_seqs: i32, n_rows: i64, n_heads: i32, n_kv: i32, head_dim: i32, scale: f32,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void,
+    ) -> i32;
+
     // GGUF reader
     pub fn fuelq_last_error() -> *const c_char;
     pub fn fuelq_gguf_open(path: *const c_char, out: *mut *mut FuelqGguf) -> i32;

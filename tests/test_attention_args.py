@@ -75,6 +75,8 @@ def test_prompt_refusals():
     assert prompt(act=Q4K) == L.NOT_SUPPORTED and prompt(hd=96) == L.NOT_SUPPORTED
     assert prompt(heads=30) == L.INVALID_PROBLEM and prompt(kv=0) == L.INVALID_PROBLEM
     assert prompt(seqs=-1) == L.INVALID_PROBLEM and prompt(rows=-1) == L.INVALID_PROBLEM and prompt(rows=1 << 31) == L.INVALID_PROBLEM
+    assert prompt(seqs=(1 << 21) + 1) == L.NOT_SUPPORTED and prompt(rows=(1 << 30) - 255) == L.INVALID_PROBLEM
+    assert prompt(heads=16384, kv=8, qs=16384 * 128) == L.INVALID_PROBLEM and decode(heads=16384, kv=8, qs=16384 * 128) == L.INVALID_PROBLEM
     for name in ("q", "k", "v", "out", "cu"):
         assert prompt(**{name: None}) == L.INVALID_PROBLEM, name
     for name in ("q", "k", "v", "out", "ws"):

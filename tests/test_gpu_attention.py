@@ -390,6 +390,44 @@ def test_prompt_boundaries_that_are_none():
         assert (out[40:] == 9.0).all(), cu
 
 
+@pytest.mark.parametrize("act", [F32, F16])
+def test_thousands_of_short_prompts(act):
+    """More sequences than rows of most of them: the search for a block's sequence takes several rounds, many slots are empty."""
+    from fuel_b200 import ops
+    lens = [(i * 7) % 5 for i in range(1500)] + [0] * 700 + [130]
+    h, kv, d, rows = 2, 1, 64, sum(lens)
+    q, k, v = _stacked(rows, h, kv, d, 3, act)
+    starts = [0]
+    for n in lens:
+        starts.append(starts[-1] + n)
+    out = ops.prompt_attn(q, k, v, _ints(starts))
+    # all at once: rows of one sequence see each other and nothing else
+    seq = torch.repeat_interleave(torch.arange(len(lens), device="cuda"), _ints(lens).long())
+    idx = torch.arange(rows, device="cuda")
+    hidden = (seq[:, None] != seq[None, :]) | (idx[None, :] > idx[:, None])
+    want, mag = [], []
+    for j in range(h):
+        p = torch.softmax((q[:, j].double() @ k[:, 0].double().T * d ** -0.5).masked_fill(hidden, float("-inf")), -1)
+        want.append(p @ v[:, 0].double()), mag.append(p @ v[:, 0].double().abs())
+    _check(out, torch.stack(want, 1), torch.stack(mag, 1), act)
+
+
+def test_decode_of_thousands_of_sequences():
+    from fuel_b200 import ops
+    lens = [(i * 13) % 40 for i in range(3000)]
+    h, kv, d, page = 2, 1, 64, 8
+    table, pages = _table(lens, page, 1)
+    kc, vc = _randn((pages, kv, page, d), 1, F16), _randn((pages, kv, page, d), 2, F16)
+    q = _randn((len(lens), h, d), 3, F16)
+    out = ops.paged_attn_decode(q, kc, vc, table, _ints(lens))
+    ids = table.clamp(min=0).long()
+    kk, vv = (c[ids].transpose(1, 2).reshape(len(lens), -1, d).double() for c in (kc, vc))     # [sequences, keys, d]
+    s = q.double() @ kk.transpose(1, 2) * d ** -0.5
+    seen = torch.arange(kk.shape[1], device="cuda") < _ints(lens)[:, None]
+    p = torch.softmax(s.masked_fill(~seen[:, None], float("-inf")), -1).nan_to_num(0.0)
+    _check(out, p @ vv, p @ vv.abs(), "many")
+
+
 # ---- together
 
 @pytest.mark.parametrize("act,cache", _PAIRS)
