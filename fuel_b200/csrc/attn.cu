@@ -252,7 +252,7 @@ int32_t fuelq_paged_attn_decode(int32_t act_type, int32_t cache_type, const void
   if (!type_pair(act_type, cache_type) || (head_dim != 64 && head_dim != 128)) return kNotSupported;
   const int shift = page_shift_of(page_size);
   if (shift < 0) return kNotSupported;
-  if (n_seqs < 0 || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !(scale >= 0.f) || std::isinf(scale) || n_pages < 0 || max_pages < 0) return kInvalidProblem;
+  if (n_seqs < 0 || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !(scale > 0.f) || std::isinf(scale) || n_pages < 0 || max_pages < 0) return kInvalidProblem;
   if (n_seqs == 0) return kOk;
   if (!q || !kcache || !vcache || !out || !page_table || !seq_lens) return kInvalidProblem;
   if (!stride_ok(q_stride, n_heads, head_dim, act_type)) return kInvalidProblem;
@@ -285,7 +285,7 @@ int32_t fuelq_prompt_attn(int32_t act_type, const void* q, int64_t q_stride, con
                           int32_t n_heads, int32_t n_kv, int32_t head_dim, float scale, void* workspace,
                           size_t workspace_bytes, void* stream) {
   if (!type_bytes(act_type) || (head_dim != 64 && head_dim != 128)) return kNotSupported;
-  if (n_seqs < 0 || n_rows < 0 || n_rows > kMaxPromptRows || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !(scale >= 0.f) || std::isinf(scale)) return kInvalidProblem;
+  if (n_seqs < 0 || n_rows < 0 || n_rows > kMaxPromptRows || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !(scale > 0.f) || std::isinf(scale)) return kInvalidProblem;
   if ((int64_t)n_seqs * n_heads > kMaxSlots) return kNotSupported;
   if (n_seqs == 0 || n_rows == 0) return kOk;
   if (!q || !k || !v || !out || !cu_seqlens) return kInvalidProblem;

@@ -273,7 +273,9 @@ def paged_attn_decode(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tenso
 
 def prompt_attn_workspace(q: torch.Tensor, k: torch.Tensor) -> torch.Tensor:
     """Scratch for prompt_attn on tensors of these shapes; calls on one stream may share it."""
-    nbytes = _L.fuelq_prompt_attn_workspace_bytes(int(_OUT_TYPES[q.dtype]), q.shape[0], q.shape[1], k.shape[1], q.shape[2])
+    if q.dtype not in _TYPE_IDS:
+        raise ValueError("q must be f32, f16 or bf16")
+    nbytes = _L.fuelq_prompt_attn_workspace_bytes(_TYPE_IDS[q.dtype], q.shape[0], q.shape[1], k.shape[1], q.shape[2])
     return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
 
 

@@ -14,15 +14,15 @@ def append(act=F32, cache=F32, k=A, ks=1024, v=A, vs=1024, q=A, qs=4096, q_out=2
                                     kv, hd, page, pages, width, max_pos, None)
 
 
-def decode(act=F32, cache=F32, q=A, qs=4096, kc=A, vc=A, out=A, table=A, lens=A, seqs=4, heads=32, kv=8, hd=128, page=16, pages=8,
+def decode(scale=0.1, act=F32, cache=F32, q=A, qs=4096, kc=A, vc=A, out=A, table=A, lens=A, seqs=4, heads=32, kv=8, hd=128, page=16, pages=8,
            width=2, ws=A, ws_bytes=1 << 40):
-    return L.lib.fuelq_paged_attn_decode(act, cache, q, qs, kc, vc, out, table, lens, seqs, heads, kv, hd, page, pages, width, 0.1, ws,
+    return L.lib.fuelq_paged_attn_decode(act, cache, q, qs, kc, vc, out, table, lens, seqs, heads, kv, hd, page, pages, width, scale, ws,
                                          ws_bytes, None)
 
 
-def prompt(act=F32, q=A, qs=4096, k=A, ks=1024, v=A, vs=1024, out=A, cu=A, seqs=4, rows=64, heads=32, kv=8, hd=128, ws=A,
+def prompt(scale=0.1, act=F32, q=A, qs=4096, k=A, ks=1024, v=A, vs=1024, out=A, cu=A, seqs=4, rows=64, heads=32, kv=8, hd=128, ws=A,
            ws_bytes=1 << 40):
-    return L.lib.fuelq_prompt_attn(act, q, qs, k, ks, v, vs, out, cu, seqs, rows, heads, kv, hd, 0.1, ws, ws_bytes, None)
+    return L.lib.fuelq_prompt_attn(act, q, qs, k, ks, v, vs, out, cu, seqs, rows, heads, kv, hd, scale, ws, ws_bytes, None)
 
 
 @pytest.mark.parametrize("call", [append, decode])
@@ -85,6 +85,13 @@ def test_prompt_refusals():
     need = L.lib.fuelq_prompt_attn_workspace_bytes(F32, 64, 32, 8, 128)
     if need:
         assert prompt(ws=None) == L.WORKSPACE and prompt(ws_bytes=need - 1) == L.WORKSPACE
+
+
+@pytest.mark.parametrize("call", [decode, prompt])
+def test_scales(call):
+    """Masked scores are -inf times the scale: it has to be a positive number."""
+    for scale in (0.0, -0.1, float("inf"), float("nan")):
+        assert call(scale=scale) == L.INVALID_PROBLEM
 
 
 def test_there_is_no_cpu_path():

@@ -529,6 +529,32 @@ def test_captured_step_with_other_lengths():
         _check(outs[0], torch.cat(want), torch.cat(mag), now)
 
 
+@pytest.mark.parametrize("act", [F32, F16])
+def test_captured_prompts_with_other_boundaries(act):
+    """Captured once, replayed with other sequences in the same rows; the result in place of the queries."""
+    from fuel_b200 import ops
+    rows, h, kv, d = 700, 4, 2, 128
+    q, k, v = (_randn((rows, n, d), s, act) for n, s in ((h, 1), (kv, 2), (kv, 3)))
+    q0, cu, ws = q.clone(), _ints([0, 1, 2, 3]), ops.prompt_attn_workspace(q, k)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        ops.prompt_attn(q, k, v, cu, out=q, workspace=ws)
+    stream.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        ops.prompt_attn(q, k, v, cu, out=q, workspace=ws)
+    for starts in ([0, 300, 300, 700], [0, 1, 129, 400], [0, 0, 0, 700]):
+        cu.copy_(_ints(starts))
+        q.copy_(q0)
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(starts, starts[1:]):
+            want, mag = _reference(q0[a:b].double(), k[a:b].double(), v[a:b].double(), d ** -0.5, 0)
+            if b > a:
+                _check(q[a:b], want, mag, (act, starts))
+        assert torch.equal(q[starts[-1]:], q0[starts[-1]:])
+
+
 def test_two_streams_with_a_workspace_each():
     from fuel_b200 import ops
     h, kv, d, page = 16, 4, 128, 16
