@@ -140,39 +140,45 @@ def dequantize(dtype: GgmlDType, blocks: torch.Tensor, elem_count: int,
 
 # ---- attention for batches of sequences: a paged key-value cache, whole packed prompts
 
-def _heads(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int) -> int:
-    """Checks a [rows, heads, head_dim] tensor on device `dev` whose rows may lie apart; its row stride in elements."""
+# (these run at every call of a decode step, where a look at a tensor's shape or type is a tenth of a microsecond: each is
+# looked at once and handed on)
+def _heads(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int):
+    """Checks a [rows, heads, head_dim] tensor on device `dev` whose rows may lie apart; its row stride in elements, its shape."""
+    shape = t.shape
     if dev < 0 or t.get_device() != dev:
         raise ValueError(f"{name} must be a CUDA tensor on the device of the other operands (there is no CPU path)")
-    if t.dtype is not dtype or t.dim() != 3:
+    if t.dtype is not dtype or len(shape) != 3:
         raise ValueError(f"{name} must be a {dtype} tensor of [rows, heads, head_dim]")
-    rows, heads, hd = t.shape
+    rows, heads, hd = shape
     row, head, one = t.stride()
     if one != 1 or (head != hd and heads > 1):
         raise ValueError(f"the heads of a row of {name} must be contiguous")
-    return row if rows > 1 else heads * hd
+    return row if rows > 1 else heads * hd, shape
 
 
-def _indices(t: torch.Tensor, name: str, dims: int, dev: int) -> None:
-    if t.dtype is not _I32 or t.get_device() != dev or t.dim() != dims or not t.is_contiguous():
+def _indices(t: torch.Tensor, name: str, dims: int, dev: int):
+    """Checks an int32 tensor of indices; its shape."""
+    shape = t.shape
+    if t.dtype is not _I32 or t.get_device() != dev or len(shape) != dims or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of {dims} dimension(s) on the device of the other operands")
-
-
-def _paged(kcache: torch.Tensor, vcache: torch.Tensor, dev: int):
-    """Checks a paged cache; (pages, kv heads, page size, head_dim)."""
-    shape = kcache.shape
-    if len(shape) != 4 or shape != vcache.shape or kcache.dtype is not vcache.dtype or kcache.dtype not in _TYPE_IDS:
-        raise ValueError("the caches must be two f32, f16 or bf16 tensors of [pages, kv_heads, page_size, head_dim]")
-    if kcache.get_device() != dev or vcache.get_device() != dev or not kcache.is_contiguous() or not vcache.is_contiguous():
-        raise ValueError("the caches must be contiguous, on the device of the other operands")
     return shape
 
 
-def _result(out: torch.Tensor | None, like: torch.Tensor, name: str) -> torch.Tensor:
+def _paged(kcache: torch.Tensor, vcache: torch.Tensor, dev: int):
+    """Checks a paged cache; (pages, kv heads, page size, head_dim), the type's number."""
+    shape, dtype = kcache.shape, kcache.dtype
+    if len(shape) != 4 or shape != vcache.shape or vcache.dtype is not dtype or dtype not in _TYPE_IDS:
+        raise ValueError("the caches must be two f32, f16 or bf16 tensors of [pages, kv_heads, page_size, head_dim]")
+    if kcache.get_device() != dev or vcache.get_device() != dev or not kcache.is_contiguous() or not vcache.is_contiguous():
+        raise ValueError("the caches must be contiguous, on the device of the other operands")
+    return shape, _TYPE_IDS[dtype]
+
+
+def _result(out: torch.Tensor | None, shape, dtype: torch.dtype, dev: int, name: str) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    if out.shape != like.shape or out.dtype is not like.dtype or out.get_device() != like.get_device() or not out.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {like.dtype} tensor of {tuple(like.shape)} on the device of the operands")
+        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", dev))
+    if out.shape != shape or out.dtype is not dtype or out.get_device() != dev or not out.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {tuple(shape)} on the device of the operands")
     return out
 
 
@@ -197,39 +203,38 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, kcache: torch.Tensor, vcache:
     if dev >= 0 and dev != _current_device():
         with torch.cuda.device(dev):
             return paged_append(k, v, kcache, vcache, page_table, positions, cos, sin, seq_ids=seq_ids, q=q, q_out=q_out, k_out=k_out)
-    ks, vs = _heads(k, "k", dtype, dev), _heads(v, "v", dtype, dev)
-    shape = k.shape
-    if dtype not in _TYPE_IDS or v.shape != shape:
+    (ks, shape), (vs, v_shape) = _heads(k, "k", dtype, dev), _heads(v, "v", dtype, dev)
+    if dtype not in _TYPE_IDS or v_shape != shape:
         raise ValueError("k and v must be f32, f16 or bf16 and of one shape")
     rows, kv, hd = shape
-    pages, ckv, page, chd = _paged(kcache, vcache, dev)
+    (pages, ckv, page, chd), cache_type = _paged(kcache, vcache, dev)
     if ckv != kv or chd != hd:
         raise ValueError(f"the caches hold {ckv} heads of {chd}, k has {kv} of {hd}")
-    _indices(page_table, "page_table", 2, dev)
-    _indices(positions, "positions", 1, dev)
-    if seq_ids is not None:
-        _indices(seq_ids, "seq_ids", 1, dev)
-    if positions.shape[0] != rows or (seq_ids is not None and seq_ids.shape[0] != rows):
+    seqs, width = _indices(page_table, "page_table", 2, dev)
+    if (_indices(positions, "positions", 1, dev)[0] != rows
+            or (seq_ids is not None and _indices(seq_ids, "seq_ids", 1, dev)[0] != rows)):
         raise ValueError("positions and seq_ids need one entry per row")
-    for t, name in (cos, "cos"), (sin, "sin"):
-        if t.dtype is not _F32 or t.dim() != 2 or t.shape[1] != hd or t.get_device() != dev or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous f32 table of [positions, head_dim]")
+    table = cos.shape
+    if len(table) != 2 or table[1] != hd or sin.shape != table:
+        raise ValueError("cos and sin must be f32 tables of [positions, head_dim], of one shape")
+    for t in cos, sin:
+        if t.dtype is not _F32 or t.get_device() != dev or not t.is_contiguous():
+            raise ValueError("cos and sin must be contiguous f32 tables on the device of the other operands")
     heads = qs = 0
     if q is not None:
-        qs = _heads(q, "q", dtype, dev)
-        if q.shape[0] != rows or q.shape[2] != hd:
+        qs, q_shape = _heads(q, "q", dtype, dev)
+        q_rows, heads, q_hd = q_shape
+        if q_rows != rows or q_hd != hd:
             raise ValueError("q must have the rows and the head_dim of k")
-        heads = q.shape[1]
-        q_out = _result(q_out, q, "q_out")
+        q_out = _result(q_out, q_shape, dtype, dev, "q_out")
     if k_out is not None:
-        _result(k_out, k, "k_out")
-    seqs, width = page_table.shape
-    status = _L.fuelq_paged_append(_TYPE_IDS[dtype], _TYPE_IDS[kcache.dtype], k.data_ptr(), ks, v.data_ptr(), vs,
+        _result(k_out, shape, dtype, dev, "k_out")
+    status = _L.fuelq_paged_append(_TYPE_IDS[dtype], cache_type, k.data_ptr(), ks, v.data_ptr(), vs,
                                    None if q is None else q.data_ptr(), qs, None if q is None else q_out.data_ptr(),
                                    None if k_out is None else k_out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(),
                                    page_table.data_ptr(), None if seq_ids is None else seq_ids.data_ptr(), positions.data_ptr(),
                                    cos.data_ptr(), sin.data_ptr(), rows, seqs, heads, kv, hd, page, pages, width,
-                                   min(cos.shape[0], sin.shape[0]), _raw_stream(dev))
+                                   table[0], _raw_stream(dev))
     if status:
         _lib.check(status, "fuelq_paged_append")
     return None if q is None else q_out
@@ -250,19 +255,17 @@ def paged_attn_decode(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tenso
     if dev >= 0 and dev != _current_device():
         with torch.cuda.device(dev):
             return paged_attn_decode(q, kcache, vcache, page_table, seq_lens, scale, out, workspace)
-    qs = _heads(q, "q", dtype, dev)
-    n, heads, hd = q.shape
-    pages, kv, page, chd = _paged(kcache, vcache, dev)
+    qs, shape = _heads(q, "q", dtype, dev)
+    n, heads, hd = shape
+    (pages, kv, page, chd), cache_type = _paged(kcache, vcache, dev)
     if dtype not in _TYPE_IDS or chd != hd:
         raise ValueError("q must be f32, f16 or bf16 with the head_dim of the caches")
-    _indices(page_table, "page_table", 2, dev)
-    _indices(seq_lens, "seq_lens", 1, dev)
-    seqs, width = page_table.shape
-    if seqs != n or seq_lens.shape[0] != n:
+    seqs, width = _indices(page_table, "page_table", 2, dev)
+    if seqs != n or _indices(seq_lens, "seq_lens", 1, dev)[0] != n:
         raise ValueError("page_table and seq_lens need one row per sequence")
-    out = _result(out, q, "out")
+    out = _result(out, shape, dtype, dev, "out")
     workspace = _scratch(workspace, _L.fuelq_paged_attn_workspace_bytes(n, heads, kv, hd) if workspace is None else 0, q)
-    status = _L.fuelq_paged_attn_decode(_TYPE_IDS[dtype], _TYPE_IDS[kcache.dtype], q.data_ptr(), qs, kcache.data_ptr(),
+    status = _L.fuelq_paged_attn_decode(_TYPE_IDS[dtype], cache_type, q.data_ptr(), qs, kcache.data_ptr(),
                                         vcache.data_ptr(), out.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), n, heads,
                                         kv, hd, page, pages, width, hd ** -0.5 if scale is None else scale,
                                         workspace.data_ptr(), workspace.nbytes, _raw_stream(dev))
@@ -288,17 +291,15 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: t
     if dev >= 0 and dev != _current_device():
         with torch.cuda.device(dev):
             return prompt_attn(q, k, v, cu_seqlens, scale, out, workspace)
-    qs, ks, vs = _heads(q, "q", dtype, dev), _heads(k, "k", dtype, dev), _heads(v, "v", dtype, dev)
-    rows, heads, hd = q.shape
-    shape = k.shape
-    if dtype not in _TYPE_IDS or shape != v.shape or shape[0] != rows or shape[2] != hd:
+    (qs, shape), (ks, k_shape), (vs, v_shape) = _heads(q, "q", dtype, dev), _heads(k, "k", dtype, dev), _heads(v, "v", dtype, dev)
+    rows, heads, hd = shape
+    k_rows, kv, k_hd = k_shape
+    if dtype not in _TYPE_IDS or k_shape != v_shape or k_rows != rows or k_hd != hd:
         raise ValueError("q, k and v must be f32, f16 or bf16 with the same rows and head_dim")
-    kv = shape[1]
-    _indices(cu_seqlens, "cu_seqlens", 1, dev)
-    seqs = cu_seqlens.shape[0] - 1
+    seqs = _indices(cu_seqlens, "cu_seqlens", 1, dev)[0] - 1
     if seqs < 0:
         raise ValueError("cu_seqlens needs n_seqs + 1 entries")
-    out = _result(out, q, "out")
+    out = _result(out, shape, dtype, dev, "out")
     workspace = _scratch(workspace, _L.fuelq_prompt_attn_workspace_bytes(_TYPE_IDS[dtype], rows, heads, kv, hd) if workspace is None else 0, q)
     status = _L.fuelq_prompt_attn(_TYPE_IDS[dtype], q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(),
                                   cu_seqlens.data_ptr(), seqs, rows, heads, kv, hd, hd ** -0.5 if scale is None else scale,
