@@ -16,8 +16,8 @@
 // tile and runs by itself: its own ring of cp.async copies that runs on across items, its own running maximum and sums; the
 // block's four warps join their results in shared memory at the end of an item, a quarter of the columns each, pieces of an item in other blocks by
 // paged_join_kernel in a fixed order.
-// Measured: 100003 keys, 32/8 heads of 128, f16 cache, f32 activations 74 us (5.5 TB/s, 0.84 of a copy); 64 sequences up to 8192, bf16, 91
-// us (5.8 TB/s); 256 up to 2047, 32/4 heads of 64, f16, 36 us (3.9 TB/s: two or three short items a block, whose beginnings and
+// Measured: 100003 keys, 32/8 heads of 128, f16 cache, f32 activations 70 to 79 us by card (5.2 to 5.8 TB/s); 64 sequences up to 8192, bf16, 91 to 95
+// us (5.6 to 5.8 TB/s); 256 up to 2047, 32/4 heads of 64, f16, 36 to 38 us (3.7 to 3.9 TB/s: two or three short items a block, whose beginnings and
 // ends are latency; without places for them in the split 64 us); 513 keys, 32 heads, f32, 15 us, nearly all latency.
 #pragma once
 #include <type_traits>

@@ -16,8 +16,8 @@
 // Keys behind a row: the scores of the last key tile are masked. A value of NaN or infinity there would still reach earlier rows
 // as 0 x NaN, so the softmax warps take such values out of the last tile in shared memory and add them to the rows they
 // belong to at the end. Rows of the next sequence, or of nobody, that the last tile touches are taken out the same way.
-// Measured, 32/8 heads of 128: one prompt of 16384 tokens, f16, 1.92 to 2.16 ms (1020 to 1145 TFLOP/s of the scores that are seen, the
-// card under its power limit), 4096 tokens 158 us; 24 prompts up to 2048, bf16, 326 us (539). A row tile's softmax (ld 250,
+// Measured, 32/8 heads of 128: one prompt of 16384 tokens, f16, 1.87 to 2.26 ms by card (970 to 1175 TFLOP/s of the scores that are seen, the
+// card under its power limit), 4096 tokens 158 us; 24 prompts up to 2048, bf16, 326 to 337 us (522 to 539). A row tile's softmax (ld 250,
 // maximum 450, exponentials 1370 cycles) and its own products (1380 from the last weight to the next scores) follow one
 // another, so with two tiles in turn the tensor cores wait a quarter of the time; tensor memory has no room for a third.
 #pragma once

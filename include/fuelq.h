@@ -404,7 +404,7 @@ int32_t fuelq_swiglu(const float* gate, const float* up, float* out, int64_t n, 
 int32_t fuelq_argmax_last(const float* x, int64_t n, int32_t* out_index, void* stream);
 
 /* ---- Attention for batches of sequences: a paged key-value cache, and whole prompts.
- * The reference keeps paged attention and flash decoding as ops of its CUDA backend (fuel-core/tests/paged_attn_oracle.rs,
+ * The reference keeps paged attention and flash decoding as ops of its CUDA backend (paged_attn_oracle.rs,
  * fuel-dispatch/src/baracuda_dispatch.rs:3421-3453); the arithmetic here is that of fuelq_attn_decode: scores in f32, softmax
  * with the maximum taken off, f32 sums.
  * Types: act_type is the type of q, k, v and the outputs, cache_type that of the pages: F32, F16 or BF16. f32 activations go
