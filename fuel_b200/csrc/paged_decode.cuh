@@ -10,7 +10,11 @@
 // Accuracy: 32-bit activations are split into parts that the cache's type holds exactly and multiplied part by part into one
 // f32 sum: f16 caches take q and p as two f16 parts (22 bits; q scaled by a power of two into range), bf16 caches as three bf16
 // parts (24 bits), f32 caches everything as two tf32 parts (22 bits). The instruction's f32 sums round towards zero, which shows
-// over a long row, so they are kept short and joined by additions that round to nearest. 16-bit activations are their own single part; p is then rounded once to their type, half a step of the result's own rounding.
+// over a long row, so they are kept short and joined by additions that round to nearest. 16-bit activations are their own single
+// part; p is then rounded once to their type. f16 ends at 2^-24, and one key of e^12 times the others' weight is common: relative to
+// the running maximum their weights had six bits left. So f16 weights are relative to the largest of their own tile's 16 or 32 keys,
+// 2^14 for it, and second parts are 2^11 times too large, in a sum of their own: 22 bits for weights down to 2^-27 of the tile's
+// largest, 11 in a single part down to 2^-28.
 // Work: tiles of kTile keys of all (sequence, kv head) items, laid end to end and dealt out evenly (attn_plan.h), so that one
 // long sequence, many short ones and any mixture fill the device alike. A warp owns 16 (head_dim 64: 32) keys of each
 // tile and runs by itself: its own ring of cp.async copies that runs on across items, its own running maximum and sums; the
@@ -137,7 +141,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
   using Cfg = DecodeCfg<A, C, kHd, kNT>;
   constexpr int kKeys = Cfg::kKeys, kSub = Cfg::kSub, kRow = Cfg::kRow, kUnit = Cfg::kUnit, kRing = Cfg::kRing, kKs = Cfg::kKs,
                 kMt = Cfg::kMt, kParts = Cfg::kParts, kHeads = Cfg::kHeads;
-  constexpr bool kF32 = Cfg::kF32;
+  constexpr bool kF32 = Cfg::kF32, kF16 = std::is_same<C, __half>::value;
+  constexpr float kWeightTop = 16384.f, kPartStep = 2048.f;
   extern __shared__ __align__(128) uint8_t dec_smem[];
   __shared__ int64_t start_s[3];
   __shared__ int scan_s[kDecodeWarps];
@@ -491,7 +496,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     request();
     out_slot = out_slot + 1 == kRing ? 0 : out_slot + 1;
 
-    // weights: the running maximum moves only when a score passes it by 2^8, so that it is looked for across lanes rarely
+    // weights: relative to the running maximum, which moves only when a score passes it by 2^8, so that it is looked for across lanes
+    // rarely; f16 caches: to the largest score of the tile, times 2^14, for f16's range (`take` brings the tile's sums to the maximum)
     bool up = false;
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
@@ -506,19 +512,29 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
           s[sub][nt][j] = x;
           up |= x > m[nt][j & 1] + 8.f;
         }
-    if (__any_sync(0xffffffffu, up)) {
+    float top[kNT][2], take[kNT][2];
+    auto find_top = [&]() {
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float top = m[nt][j];
+          top[nt][j] = -INFINITY;
 #pragma unroll
-          for (int sub = 0; sub < kSub; ++sub) top = fmaxf(top, fmaxf(s[sub][nt][j], s[sub][nt][j + 2]));
+          for (int sub = 0; sub < kSub; ++sub) top[nt][j] = fmaxf(top[nt][j], fmaxf(s[sub][nt][j], s[sub][nt][j + 2]));
 #pragma unroll
-          for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-          const bool move = top > m[nt][j] + 8.f;  // by this head's scores alone: its bits do not depend on the others'
-          const float keep = move ? exp2f(m[nt][j] - top) : 1.f;
-          if (move) m[nt][j] = top;
+          for (int off = 4; off < 32; off <<= 1) top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(0xffffffffu, top[nt][j], off));
+        }
+    };
+    if constexpr (kF16) find_top();
+    if (__any_sync(0xffffffffu, up)) {
+      if constexpr (!kF16) find_top();
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const bool move = top[nt][j] > m[nt][j] + 8.f;  // by this head's scores alone: its bits do not depend on the others'
+          const float keep = move ? exp2f(m[nt][j] - top[nt][j]) : 1.f;
+          if (move) m[nt][j] = top[nt][j];
           l[nt][j] *= keep;
 #pragma unroll
           for (int t = 0; t < kMt; ++t) o[nt][t][j] *= keep, o[nt][t][j + 2] *= keep;
@@ -527,14 +543,25 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     uint32_t pf[kSub][kNT][kParts][kF32 ? 4 : 2];  // p as the second operand of the products with V
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
-      const float ref0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], ref1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+      float ref[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float to = kF16 ? top[nt][j] : m[nt][j];
+        ref[j] = to == -INFINITY ? 0.f : to;
+        take[nt][j] = !kF16 ? 1.f : to == -INFINITY ? 0.f : exp2f(to - m[nt][j]);
+      }
 #pragma unroll
       for (int sub = 0; sub < kSub; ++sub) {
         float e[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          e[j] = exp2f(s[sub][nt][j] - (j & 1 ? ref1 : ref0));
-          l[nt][j & 1] += e[j];
+          e[j] = exp2_approx(s[sub][nt][j] - ref[j & 1]);
+          if constexpr (kF16) {
+            l[nt][j & 1] = fmaf(e[j], take[nt][j & 1], l[nt][j & 1]);
+            e[j] *= kWeightTop;
+          } else {
+            l[nt][j & 1] += e[j];
+          }
         }
         if constexpr (kF32) {
           // this lane wants keys tq, tq + 4, tq + 8, tq + 12 of head g; lane 4 * key + g / 2 has them for keys below 8 in e[g & 1]
@@ -554,6 +581,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
               float ra, rb;
               unpack2<C>(u, ra, rb);
               a -= ra, b -= rb;
+              if constexpr (kF16) a *= kPartStep, b *= kPartStep;
               pf[sub][nt][part][half] = transpose8(u);
             }
           }
@@ -569,7 +597,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     // a tile's products by themselves, then added to O with a sum that rounds to nearest
 #pragma unroll
     for (int t = 0; t < kMt; ++t) {
-      float tile[kNT][4] = {};
+      float tile[kNT][4] = {}, low[kNT][4] = {};  // low: the second parts of f16 weights, kPartStep times too large
 #pragma unroll
       for (int sub = 0; sub < kSub; ++sub) {
         if constexpr (kF32) {
@@ -597,13 +625,21 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
 #pragma unroll
           for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-            for (int part = kParts - 1; part >= 0; --part) mma16(tile[nt], a, pf[sub][nt][part][0], pf[sub][nt][part][1], C());
+            for (int part = kParts - 1; part >= 0; --part)
+              mma16(kF16 && part ? low[nt] : tile[nt], a, pf[sub][nt][part][0], pf[sub][nt][part][1], C());
         }
       }
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[nt][t][i] += tile[nt][i];
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (kF16) {
+            const float all = kParts > 1 ? fmaf(low[nt][i], 1.f / kPartStep, tile[nt][i]) : tile[nt][i];
+            o[nt][t][i] = fmaf(all, take[nt][i & 1] * (1.f / kWeightTop), o[nt][t][i]);
+          } else {
+            o[nt][t][i] += tile[nt][i];
+          }
+        }
     }
     __syncwarp();
     request();

@@ -158,11 +158,6 @@ __device__ __forceinline__ uint64_t lds_pair(uint32_t addr) {
   asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // the largest of three, NaN if one is
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float d;

@@ -1,0 +1,86 @@
+"""Attention at the ends of the number ranges: scores near and beyond f32's ends, one key far above all others, infinities among
+the values that a row sees, large values behind it. Against the definitions in 64 bits, or against the same call without them.
+
+Tolerances. `_HALF` is half a step of a 16-bit type. Results in 32 bits: 4.1e-6 of the norm for scores of a standard deviation
+below 2.5 (every factor keeps 21 bits, 16 partial sums rounded towards zero), and a score of g adds its own 22 bits, g * 2^-22.
+"""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+_HALF = {F16: 2.0 ** -11, BF16: 2.0 ** -8}
+_PAIRS = [(F32, F32), (F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)]
+
+
+@pytest.fixture(autouse=True)
+def _device():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from fuel_b200 import ops
+    ops.device_error(clear=True)
+    yield
+    assert ops.device_error(clear=True) == 0
+
+
+def _randn(shape, seed, dtype, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def _ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def _sink(n, h, d, act, cache, gap, seed):
+    """q [1, h, d], k and v [n, 1, d]: the first key scores `gap` in every head and holds values of zero, the others' scores have a
+    standard deviation of 0.3."""
+    q, k, v = _randn((1, h, d), seed, act, 0.3), _randn((n, 1, d), seed + 1, cache), _randn((n, 1, d), seed + 2, cache)
+    q[..., 0] = 8.0
+    k[..., 0] = 0.0
+    k[0] = 0.0
+    k[0, 0, 0] = gap / (8.0 * d ** -0.5)
+    v[0] = 0.0
+    return q, k, v
+
+
+def _attend(q, k, v, scale):
+    """q [h, d], k and v [n, d] in 64 bits -> (out, sum of p |v|)"""
+    p = torch.softmax(q @ k.T * scale, -1)
+    return p @ v, p @ v.abs()
+
+
+def _pages(k, v, page):
+    """k and v [n, 1, d] as a paged cache of one sequence, its pages in reverse"""
+    n, _, d = k.shape
+    pages = -(-n // page)
+    kc, vc = (torch.zeros(pages * page, 1, d, dtype=k.dtype, device="cuda") for _ in range(2))
+    kc[:n], vc[:n] = k, v
+    kc, vc = (c.view(pages, page, 1, d).transpose(1, 2).flip(0).contiguous() for c in (kc, vc))
+    return kc, vc, _ints([list(range(pages - 1, -1, -1))])
+
+
+# ---- one key far above all others
+
+@pytest.mark.parametrize("gap", [8.0, 12.0, 16.0, 20.0])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("act,cache", _PAIRS)
+def test_decode_keeps_small_weights_beside_one_large(act, cache, d, gap):
+    """The result is the sum of two thousand weights of e^-gap: each has to keep its type's bits."""
+    from fuel_b200 import ops
+    n, h = 2049, 4
+    q, k, v = _sink(n, h, d, act, cache, gap, 3)
+    kc, vc, table = _pages(k, v, 16)
+    out = ops.paged_attn_decode(q, kc, vc, table, _ints([n]))
+    want, mag = _attend(q[0].double(), k[:, 0].double(), v[:, 0].double(), d ** -0.5)
+    err = (out[0].double() - want).abs()
+    if act == F32:
+        assert (err.norm() / want.norm()).item() <= 4.1e-6 + gap * 2.0 ** -22
+    else:
+        # beside the roundings of the weights and of the result: scores of `gap` in f32 sums of 128 terms. Results below 2^-14 are
+        # whole multiples of 2^-24 in f16, whatever they come from: half of one is off
+        least = 2.0 ** -25 if act == F16 else 0.0
+        assert (err <= _HALF[act] * (want.abs() + mag) + (2.0 ** -15 + gap * 2.0 ** -17) * mag + least).all()
