@@ -90,6 +90,23 @@ __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
   a = to_f32(reinterpret_cast<const T*>(&w)[0]), b = to_f32(reinterpret_cast<const T*>(&w)[1]);
 }
 
+// What a column of the values of keys [from, to) holds that is not finite: the sum of it, 0 if there is nothing. column: of page 0,
+// row 0. An infinite value is infinite in the result whatever its weight, but its product with a part of the weight that is negative
+// or zero is not; so a result that is not finite while the sum of its weights is is looked up again here. (Only then: an infinity in
+// the cache costs its batch time, finite ones nothing.)
+template <typename C>
+__device__ __noinline__ float sum_not_finite(const C* column, const int* pages, int from, int to, int page_shift, int n_pages, int64_t page_stride, int row_stride) {
+  float sum = 0.f;
+#pragma unroll 4
+  for (int key = from; key < to; ++key) {
+    const int page = pages[key >> page_shift];
+    const bool is = page >= 0 && page < n_pages;
+    const float x = is ? to_f32(column[page * page_stride + (int64_t)(key & ((1 << page_shift) - 1)) * row_stride]) : 0.f;
+    if (!isfinite(x)) sum += x;
+  }
+  return sum;
+}
+
 template <typename A, typename C, int kHd_, int kNT_>
 struct DecodeCfg {
   static constexpr int kHd = kHd_, kNT = kNT_, kHeads = 8 * kNT;  // heads of an item
@@ -392,6 +409,12 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     const bool whole = done && item_first >= x0;
     float* slot = p.slots + (int64_t)split_slot(total, blocks, blockIdx.x, item_first) * Cfg::kSlot;
     A* dst = reinterpret_cast<A*>(p.out) + ((int64_t)at.seq * p.n_heads + kvh * p.group + part * kHeads) * kHd;
+    const int64_t page_stride = (int64_t)p.n_kv * kHd << p.page_shift;
+    auto look_again = [&](int d) {  // at column d of the piece's keys
+      const int from = (int)max(x0 - item_first, (int64_t)0) * Cfg::kTile, to = (int)min((int64_t)(at.tile + 1) * Cfg::kTile, (int64_t)at.keys);
+      return sum_not_finite(reinterpret_cast<const C*>(p.v) + ((int64_t)kvh * kHd << p.page_shift) + d, p.table + (int64_t)at.seq * p.max_pages,
+                            from, to, p.page_shift, p.n_pages, page_stride, kHd);
+    };
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
       float4 st[kDecodeWarps];
@@ -427,6 +450,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
         for (int i = 0; i < 4; ++i) {
           const int h = nt * 8 + 2 * tq + (i & 1), d = 16 * (warp * kQ + q) + g + 8 * (i >> 1);
           if (h < heads) {
+            if (!isfinite(r[i]) && isfinite(sum[i & 1])) {
+              const float f = look_again(d);
+              if (f != 0.f) r[i] = f;
+            }
             if (whole) dst[h * kHd + d] = from_f32<A>(r[i] * inv[i & 1]);
             else slot[h * kHd + d] = r[i];
           }
@@ -706,7 +733,10 @@ __global__ void __launch_bounds__(kHd) paged_join_kernel(const DecodeParams p) {
   for (int w = 0; w < kHd / 32; ++w) sum += red_s[1][w];
   float acc = 0.f;
 #pragma unroll 4
-  for (int i = 0; i < n; ++i) acc += weight_s[i] * slot(i)[h * kHd + threadIdx.x];
+  for (int i = 0; i < n; ++i) {
+    const float x = slot(i)[h * kHd + threadIdx.x];
+    acc += isinf(x) ? x : weight_s[i] * x;  // infinite also where the piece's weight has come to nothing
+  }
   const int kvh = a.y / p.chunks;
   reinterpret_cast<A*>(p.out)[((int64_t)a.x * p.n_heads + kvh * p.group + part * Cfg::kHeads + h) * kHd + threadIdx.x] =
       from_f32<A>(sum == 0.f ? 0.f : acc / sum);

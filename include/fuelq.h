@@ -436,7 +436,8 @@ int32_t fuelq_paged_append(int32_t act_type, int32_t cache_type, const void* k, 
  * new token already appended). seq_lens[s] <= 0, a free slot of the batch, gives a row of zeros. The workspace is
  * fuelq_paged_attn_workspace_bytes() bytes, holds nothing between calls and needs no clearing; calls that may run at the same
  * time need one each. 32-bit activations are multiplied to 32-bit accuracy whatever the cache's type; with 16-bit ones the
- * softmax's weights are rounded once to their type, however far below the largest they are. */
+ * softmax's weights are rounded once to their type, however far below the largest they are. An infinite value makes its
+ * column of the result infinite, infinities of both signs make it NaN. */
 size_t fuelq_paged_attn_workspace_bytes(int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t head_dim);
 int32_t fuelq_paged_attn_decode(int32_t act_type, int32_t cache_type, const void* q, int64_t q_stride, const void* kcache,
                                 const void* vcache, void* out, const int32_t* page_table, const int32_t* seq_lens,

@@ -84,3 +84,30 @@ def test_decode_keeps_small_weights_beside_one_large(act, cache, d, gap):
         # whole multiples of 2^-24 in f16, whatever they come from: half of one is off
         least = 2.0 ** -25 if act == F16 else 0.0
         assert (err <= _HALF[act] * (want.abs() + mag) + (2.0 ** -15 + gap * 2.0 ** -17) * mag + least).all()
+
+
+# ---- values that are not finite, seen by the row
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("act,cache", _PAIRS)
+def test_decode_of_infinite_values(act, cache, d, bad):
+    """A value of infinity has a weight above zero: its column is that infinity, the others are as they were. Infinities of both
+    signs make NaN."""
+    from fuel_b200 import ops
+    h, n = 6, 700
+    q, k, v = _randn((2, h, d), 3, act), _randn((n, 1, d), 4, cache), _randn((n, 1, d), 5, cache)
+    for at in (0, 77, 699):
+        b = v.clone()
+        b[at, 0, 9] = bad
+        b[at, 0, 40] = -bad
+        b[at // 2, 0, 50], b[at // 2 + 300 if at < 699 else 3, 0, 50] = math.inf, -math.inf
+        kc, vc, table = _pages(k, v, 16)
+        _, bc, _ = _pages(k, b, 16)
+        table, lens = table.repeat(2, 1), _ints([n, n])
+        good, out = ops.paged_attn_decode(q, kc, vc, table, lens), ops.paged_attn_decode(q, kc, bc, table, lens)
+        for c, want in ((9, bad), (40, -bad), (50, math.nan)):
+            col = out[..., c].float()
+            assert (col.isnan() if want != want else col == want).all(), (at, c, col)
+        cols = [c for c in range(d) if c not in (9, 40, 50)]
+        assert torch.equal(out[..., cols], good[..., cols])
