@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
   constexpr int kKeys = Cfg::kKeys, kSub = Cfg::kSub, kRow = Cfg::kRow, kUnit = Cfg::kUnit, kRing = Cfg::kRing, kKs = Cfg::kKs,
                 kMt = Cfg::kMt, kParts = Cfg::kParts, kHeads = Cfg::kHeads;
   constexpr bool kF32 = Cfg::kF32, kF16 = std::is_same<C, __half>::value;
+  constexpr float kMost = 3.402823466e38f;
   constexpr float kWeightTop = 16384.f, kPartStep = 2048.f;
   extern __shared__ __align__(128) uint8_t dec_smem[];
   __shared__ int64_t start_s[3];
@@ -525,19 +526,41 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
 
     // weights: relative to the running maximum, which moves only when a score passes it by 2^8, so that it is looked for across lanes
     // rarely; f16 caches: to the largest score of the tile, times 2^14, for f16's range (`take` brings the tile's sums to the maximum)
-    bool up = false;
+    bool up = false, far = false;
+    float x[kSub][kNT][4];
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
       for (int sub = 0; sub < kSub; ++sub)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float x = s[sub][nt][j] * factor[nt][j & 1];
-          // scores at the ends of f32 stay finite; NaN stays NaN
-          x = x < -3.402823466e38f ? -3.402823466e38f : x > 3.402823466e38f ? 3.402823466e38f : x;
-          if (!((seen >> (sub * 16 + g + 8 * (j >> 1))) & 1)) x = -INFINITY;
-          s[sub][nt][j] = x;
-          up |= x > m[nt][j & 1] + 8.f;
+          x[sub][nt][j] = s[sub][nt][j] * factor[nt][j & 1];
+          far |= fabsf(x[sub][nt][j]) > kMost;
+        }
+    if (__any_sync(0xffffffffu, far)) {
+      // finite products stay finite when they are scaled. A product of -inf is a weight of zero, one of +inf makes the row NaN as inf - inf
+      // does. (f32 caches: infinite factors have made NaN of it in their second parts, and an infinite product is one at f32's end)
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+        for (int sub = 0; sub < kSub; ++sub)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float& y = x[sub][nt][j];
+            if (!(fabsf(y) > kMost)) continue;
+            if (kF32 || fabsf(s[sub][nt][j]) <= kMost) y = copysignf(kMost, y);
+            else if (y > 0.f) y = __int_as_float(0x7fc00000);
+          }
+    }
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+      for (int sub = 0; sub < kSub; ++sub)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (!((seen >> (sub * 16 + g + 8 * (j >> 1))) & 1)) x[sub][nt][j] = -INFINITY;
+          s[sub][nt][j] = x[sub][nt][j];
+          up |= x[sub][nt][j] > m[nt][j & 1] + 8.f;
         }
     float top[kNT][2], take[kNT][2];
     auto find_top = [&]() {

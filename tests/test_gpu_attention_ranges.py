@@ -111,3 +111,25 @@ def test_decode_of_infinite_values(act, cache, d, bad):
             assert (col.isnan() if want != want else col == want).all(), (at, c, col)
         cols = [c for c in range(d) if c not in (9, 40, 50)]
         assert torch.equal(out[..., cols], good[..., cols])
+
+
+@pytest.mark.parametrize("act,cache", [(F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_decode_of_scores_of_infinity(act, cache, d):
+    """+inf makes the row NaN, -inf is a weight of zero, and a row with no other scores has no weights: zeros."""
+    from fuel_b200 import ops
+    n, h = 300, 3
+    q, k, v = _randn((1, h, d), 1, act), _randn((n, 1, d), 2, cache), _randn((n, 1, d), 3, cache)
+    q[..., 0] = 1.0
+    for at in (0, 5, 150, 299):
+        b = k.clone()
+        b[at, 0, 0] = math.inf
+        kc, vc, table = _pages(b, v, 32)
+        assert ops.paged_attn_decode(q, kc, vc, table, _ints([n])).isnan().all(), at
+    b = k.clone()
+    b[:290, 0, 0] = -math.inf
+    kc, vc, table = _pages(b, v, 32)
+    out = ops.paged_attn_decode(q, kc, vc, table, _ints([n]))
+    want, mag = _attend(q[0].double(), k[290:, 0].double(), v[290:, 0].double(), d ** -0.5)
+    assert ((out[0].double() - want).abs() <= _HALF[act] * (want.abs() + mag) + 2.0 ** -15 * mag).all()
+    assert not ops.paged_attn_decode(q, kc, vc, table, _ints([290])).any()
