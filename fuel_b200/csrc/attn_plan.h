@@ -30,6 +30,12 @@ FQ_HD int seq_keys(int len, int max_pages, int page_shift) {
 FQ_HD int seq_tiles(int len, int max_pages, int page_shift, int tile) { return (int)(((int64_t)seq_keys(len, max_pages, page_shift) + tile - 1) / tile); }
 
 FQ_HD int item_units(int tiles) { return tiles ? tiles + kItemUnits : 0; }
+// places of one kv head of sequences [from, to): more than 32 bits count where long sequences share their pages
+FQ_HD int64_t seq_units(const int* lens, int from, int to, int max_pages, int page_shift, int tile) {
+  int64_t sum = 0;
+  for (int s = from; s < to; ++s) sum += item_units(seq_tiles(lens[s], max_pages, page_shift, tile));
+  return sum;
+}
 
 // ---- prompts. An item is a block of `rows` rows of one sequence and one query head. Sequence s has the block numbers ("slots")
 // from prompt_slot(cu[s], s) up to the next sequence's: at least as many as it has blocks, without any sum over the

@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
   constexpr float kWeightTop = 16384.f, kPartStep = 2048.f;
   extern __shared__ __align__(128) uint8_t dec_smem[];
   __shared__ int64_t start_s[3];
-  __shared__ int scan_s[kDecodeWarps];
+  __shared__ int64_t scan_s[kDecodeWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   uint8_t* ring = dec_smem + warp * kRing * kUnit;
   uint8_t* shared = dec_smem + kDecodeWarps * kRing * kUnit;  // q, and between items the warps' results
@@ -176,34 +176,28 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
   const int items = p.n_kv * p.chunks;
   const int per = (p.n_seqs + 32 * kDecodeWarps - 1) / (32 * kDecodeWarps);
   const int s0 = min((int)threadIdx.x * per, p.n_seqs), s1 = min(s0 + per, p.n_seqs);
-  int mine = 0;
-  bool bad = false;
-  for (int s = s0; s < s1; ++s) {
-    const int len = p.lens[s];
-    bad |= len > ((int64_t)p.max_pages << p.page_shift);
-    mine += item_units(seq_tiles(len, p.max_pages, p.page_shift, Cfg::kTile));
-  }
-  int incl = mine;
+  const int64_t mine = seq_units(p.lens, s0, s1, p.max_pages, p.page_shift, Cfg::kTile);
+  int64_t incl = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const int o = __shfl_up_sync(0xffffffffu, incl, off);
+    const int64_t o = __shfl_up_sync(0xffffffffu, incl, off);
     if (lane >= off) incl += o;
   }
   if (lane == 31) scan_s[warp] = incl;
   __syncthreads();
-  int total1 = 0, before = 0;
+  int64_t total1 = 0, before = 0;
 #pragma unroll
   for (int w = 0; w < kDecodeWarps; ++w) {
     if (w < warp) before += scan_s[w];
     total1 += scan_s[w];
   }
-  const int64_t total = (int64_t)total1 * items;
+  const int64_t total = total1 * items;
   const int blocks = total < (int64_t)gridDim.x ? (int)total : (int)gridDim.x;
   const bool active = (int)blockIdx.x < blocks;
   const int64_t x0 = active ? split_begin(total, blocks, blockIdx.x) : 0, x1 = active ? split_begin(total, blocks, blockIdx.x + 1) : 0;
   {
-    int64_t at = (int64_t)(before + incl - mine) * items;  // first tile of this thread's sequences
-    if (active && at <= x0 && x0 < at + (int64_t)mine * items) {
+    int64_t at = (before + incl - mine) * items;  // first tile of this thread's sequences
+    if (active && at <= x0 && x0 < at + mine * items) {
       int s = s0;
       for (;; ++s) {
         const int64_t n = (int64_t)item_units(seq_tiles(p.lens[s], p.max_pages, p.page_shift, Cfg::kTile)) * items;
@@ -215,12 +209,13 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
   }
   // free slots of the batch: rows of zeros
   for (int s = blockIdx.x; s < p.n_seqs; s += gridDim.x) {
-    if (seq_keys(p.lens[s], p.max_pages, p.page_shift) == 0) {
+    const int len = p.lens[s];
+    if (len > ((int64_t)p.max_pages << p.page_shift) && threadIdx.x == 0) record_dev_error(kErrIndex);
+    if (seq_keys(len, p.max_pages, p.page_shift) == 0) {
       uint32_t* o = reinterpret_cast<uint32_t*>(reinterpret_cast<A*>(p.out) + (int64_t)s * p.n_heads * kHd);
       for (int i = threadIdx.x; i < p.n_heads * kHd * (int)sizeof(A) / 4; i += 32 * kDecodeWarps) o[i] = 0;
     }
   }
-  if (bad && blockIdx.x == 0) record_dev_error(kErrIndex);
   __syncthreads();
   TilePos use;
   use.x = x1;
