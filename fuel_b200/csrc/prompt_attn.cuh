@@ -192,17 +192,18 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return r;
 }
 // 2^x of two values on the multiply-add pipes: x = n + f with n the nearest integer, found by adding 1.5 2^23, 2^f by a polynomial of
-// degree four (fitted to the least relative error over [-1/2, 1/2]: 2.6e-6), n added to its exponent. Below 2^-126: some
-// denormal. NaN does not pass
+// degree four (fitted to the least relative error over [-1/2, 1/2], its constant held at 1: 2.9e-6), n added to its exponent. From
+// -127 down, -inf among them, the exponent comes to nothing and the result is zero itself: a masked key's weight, which the largest
+// bf16 value behind the row must not show through. NaN does not pass
 __device__ __forceinline__ void exp2_poly2(uint64_t x, float& a, float& b) {
   unpair(x, a, b);
-  x = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  x = pair(fmaxf(a, -127.f), fmaxf(b, -127.f));
   const uint64_t magic = pair(12582912.f, 12582912.f), t = add2(x, magic);
   const uint64_t f = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), x);
-  uint64_t y = fma2(f, pair(0x1.3997d4p-7f, 0x1.3997d4p-7f), pair(0x1.ca1442p-5f, 0x1.ca1442p-5f));
-  y = fma2(y, f, pair(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-  y = fma2(y, f, pair(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-  y = fma2(y, f, pair(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  uint64_t y = fma2(f, pair(0x1.3a1804p-7f, 0x1.3a1804p-7f), pair(0x1.c9fcb2p-5f, 0x1.c9fcb2p-5f));
+  y = fma2(y, f, pair(0x1.ec0326p-3f, 0x1.ec0326p-3f));
+  y = fma2(y, f, pair(0x1.62e12cp-1f, 0x1.62e12cp-1f));
+  y = fma2(y, f, pair(1.f, 1.f));
   float ta, tb;
   unpair(t, ta, tb);
   unpair(y, a, b);
@@ -355,8 +356,8 @@ template <typename T, int kHd>
 struct PromptCfg {
   static constexpr int kStages = kHd == 128 ? 4 : 8;
   // one pair of scores in so many has its exponentials on the multiply-add pipes (the exponential unit does 16 a clock and SM).
-  // 24 prompts up to 2048, head_dim 128: none 393, one in eight 392, six 389, four 395 us; 8192 tokens, head_dim 64, where half the
-  // products meet as many exponentials: 452, 461, 450, 433 us
+  // 24 prompts up to 2048, head_dim 128: none 374, one in eight 335, six 340, five 341 us; one prompt of 256: 13.5, 11.8, 11.8, 11.8.
+  // 8192 tokens, head_dim 64, where half the products meet as many exponentials: none 484, one in six 501, five 465, four 483 us
   static constexpr int kPolyEvery = kHd == 128 ? 6 : 4;
   static constexpr int kTileBytes = kPaTile * kHd * 2;
   static constexpr int kSmem = 1024 + (2 + kStages) * kTileBytes + 8 * kStageBytes + (int)sizeof(PromptCtl<kHd, kStages>) + 16;

@@ -133,3 +133,22 @@ def test_decode_of_scores_of_infinity(act, cache, d):
     want, mag = _attend(q[0].double(), k[290:, 0].double(), v[290:, 0].double(), d ** -0.5)
     assert ((out[0].double() - want).abs() <= _HALF[act] * (want.abs() + mag) + 2.0 ** -15 * mag).all()
     assert not ops.paged_attn_decode(q, kc, vc, table, _ints([290])).any()
+
+
+# ---- large values behind a row
+
+@pytest.mark.parametrize("act", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_rows_do_not_see_large_values_behind_them(act, d):
+    """The type's largest values in later rows of the sequence, in the next one and behind the last: weights of zero, not nearly."""
+    from fuel_b200 import ops
+    rows, cu = 360, _ints([0, 300, 350])
+    q, k, v = _randn((rows, 2, d), 1, act), _randn((rows, 1, d), 2, act), _randn((rows, 1, d), 3, act)
+    want = ops.prompt_attn(q, k, v, cu)
+    for bad in (torch.finfo(act).max, torch.finfo(act).min):
+        for at in list(range(1, 19)) + [137, 138, 256, 299]:
+            b = v.clone()
+            b[at:300] = bad
+            b[300:] = bad
+            out = ops.prompt_attn(q, k, b, cu)
+            assert torch.equal(out[:at], want[:at]), (bad, at)
