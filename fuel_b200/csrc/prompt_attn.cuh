@@ -536,7 +536,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
         uint64_t c2, m2;
         // the row's reference, once its maximum is in top[]
         auto refer = [&]() {
-          const float most = max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3]));
+          float most = max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3]));
+          if (most == INFINITY) most = __int_as_float(0x7fc00000);  // inf - inf is in this row's softmax
           if (j == 0) {
             ref = most;
             mc = ref == -INFINITY ? 0.f : ref * p.c;

@@ -113,6 +113,23 @@ def test_decode_of_infinite_values(act, cache, d, bad):
         assert torch.equal(out[..., cols], good[..., cols])
 
 
+@pytest.mark.parametrize("act", [F32, BF16, F16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_rows_with_a_score_of_infinity_are_nan(act, d):
+    """inf - inf is in the softmax of such a row, wherever the key lies; the rows before it do not see it."""
+    from fuel_b200 import ops
+    n = 400
+    q, k, v = _randn((n, 2, d), 1, act), _randn((n, 1, d), 2, act), _randn((n, 1, d), 3, act)
+    q[..., 0] = 1.0
+    want = ops.prompt_attn(q, k, v, _ints([0, n]))
+    for at in list(range(0, 34)) + [129, 138, 139, 143, 255, 256, 300, 399]:
+        b = k.clone()
+        b[at, 0, 0] = math.inf
+        out = ops.prompt_attn(q, b, v, _ints([0, n]))
+        assert out[at:].isnan().all(), at
+        assert torch.equal(out[:at], want[:at])
+
+
 @pytest.mark.parametrize("act,cache", [(F16, F16), (BF16, BF16)])
 @pytest.mark.parametrize("d", [64, 128])
 def test_decode_of_scores_of_infinity(act, cache, d):
