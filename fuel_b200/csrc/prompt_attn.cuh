@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
             const bool move = !((most - ref) * p.c <= 8.f);
             if (__any_sync(0xffffffffu, move)) {  // O is complete up to the tile before: S of this one came after it
               // each row by its own scores alone: its bits do not depend on what else is in the warp
-              const float keep = move ? exp2_approx((ref - most) * p.c) : 1.f;
+              const float keep = move && most != ref ? exp2_approx((ref - most) * p.c) : 1.f;  // both -inf: nothing of weight yet
               if (move) ref = most;
               mc = ref == -INFINITY ? 0.f : ref * p.c;
 #pragma unroll 1

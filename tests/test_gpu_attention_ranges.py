@@ -152,6 +152,22 @@ def test_decode_of_scores_of_infinity(act, cache, d):
     assert not ops.paged_attn_decode(q, kc, vc, table, _ints([290])).any()
 
 
+@pytest.mark.parametrize("act", [BF16, F16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_rows_whose_first_keys_score_minus_infinity(act, d):
+    """Two key tiles and more of weights of zero, then others."""
+    from fuel_b200 import ops
+    n, first = 500, 300
+    q, k, v = _randn((n, 2, d), 1, act), _randn((n, 1, d), 2, act), _randn((n, 1, d), 3, act)
+    q[..., 0] = 1.0
+    k[:first, 0, 0] = -math.inf
+    out = ops.prompt_attn(q, k, v, _ints([0, n]))
+    assert not out[:first].any()
+    for row in (300, 301, 383, 384, 499):
+        want, mag = _attend(q[row].double(), k[first:row + 1, 0].double(), v[first:row + 1, 0].double(), d ** -0.5)
+        assert ((out[row].double() - want).abs() <= _HALF[act] * (want.abs() + mag) + 2.0 ** -15 * mag).all(), row
+
+
 # ---- large values behind a row
 
 @pytest.mark.parametrize("act", [F16, BF16])
