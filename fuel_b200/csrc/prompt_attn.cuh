@@ -3,7 +3,9 @@
 //   S = Q K^T,  P = exp2(c S - c m),  O += P V,  out = O / sum(P),   c = scale log2(e)
 //
 // with m a reference that follows the running maximum of the row: it moves only when the maximum has passed it by 2^8, so that
-// O, which stays in tensor memory, is hardly ever rescaled (P then reaches 2^8 at most; sums and products are f32).
+// O, which stays in tensor memory, is hardly ever rescaled (P then reaches 2^8 at most, in f16, whose weights are 2^7 times larger to
+// keep clear of its lower end, 2^15; sums and products are f32). P is rounded once to the inputs' type: half a step of each weight,
+// in f16 2^-32 of the largest at least. P in two parts would be half as many products again.
 // Bound by the tensor cores and, at head_dim 64 above all, by the 16 exponentials a clock and SM.
 // A persistent thread block per SM takes blocks of 256 query rows of one head, the longest of a sequence first, as two tiles of
 // 128 rows that take turns: while the tensor cores multiply for one tile, the other one's softmax runs.
@@ -533,6 +535,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
         tc_fence_after();
         const bool last = j + 1 == mine;
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // NaN where a visible score is: then the whole row is
+        // f16 ends at 2^-24: its weights are 2^7 times larger, up to 2^15
+        constexpr float kUp = std::is_same<T, __half>::value ? 7.f : 0.f;
         uint64_t c2, m2;
         // the row's reference, once its maximum is in top[]
         auto refer = [&]() {
@@ -564,7 +568,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
               }
             }
           }
-          c2 = pair(p.c, p.c), m2 = pair(-mc, -mc);
+          c2 = pair(p.c, p.c), m2 = pair(kUp - mc, kUp - mc);
         };
         auto weight2 = [&](int i, uint32_t s0, uint32_t s1) {  // of pair i of the tile
           float a, b;

@@ -86,6 +86,24 @@ def test_decode_keeps_small_weights_beside_one_large(act, cache, d, gap):
         assert (err <= _HALF[act] * (want.abs() + mag) + (2.0 ** -15 + gap * 2.0 ** -17) * mag + least).all()
 
 
+@pytest.mark.parametrize("act,gap", [(F16, 12.0), (F16, 16.0), (BF16, 16.0), (F32, 16.0)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_keeps_small_weights_beside_one_large(act, d, gap):
+    from fuel_b200 import ops
+    n, h = 1500, 2
+    q1, k, v = _sink(n, h, d, act, act, gap, 3)
+    q = q1.expand(n, h, d).contiguous()
+    out = ops.prompt_attn(q, k, v, _ints([0, n]))
+    for row in (500, 1023, 1499):
+        want, mag = _attend(q[row].double(), k[:row + 1, 0].double(), v[:row + 1, 0].double(), d ** -0.5)
+        err = (out[row].double() - want).abs()
+        if act == F32:
+            assert (err.norm() / want.norm()).item() <= 4.1e-6 + gap * 2.0 ** -22
+        else:
+            least = 2.0 ** -25 if act == F16 else 0.0       # as above
+            assert (err <= _HALF[act] * (want.abs() + mag) + (2.0 ** -15 + gap * 2.0 ** -17) * mag + least).all(), row
+
+
 # ---- values that are not finite, seen by the row
 
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
