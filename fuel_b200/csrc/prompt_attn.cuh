@@ -344,7 +344,7 @@ template <int kHd, int kStages>
 struct PromptCtl {
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];
   uint64_t kv_full[kStages], kv_empty[kStages];
-  uint64_t taken_free;  // tile 1 has read the record of tile 0 (once per item with a tile 1)
+  uint64_t taken_free[2];  // the threads of a tile have read the records of an item (tile 1 reads both)
   TakenOut<kHd> taken[2];
   ItemRing items;
   uint32_t tmem_base;
@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
       ctl->taken[x].last = 0;
     }
     for (int s = 0; s < kStages; ++s) mbar_init(&ctl->kv_full[s], 1), mbar_init(&ctl->kv_empty[s], 1);
-    mbar_init(&ctl->taken_free, 128);
+    mbar_init(&ctl->taken_free[0], 128), mbar_init(&ctl->taken_free[1], 128);
     for (int s = 0; s < kItemRing; ++s) mbar_init(&ctl->items.full[s], 1), mbar_init(&ctl->items.empty[s], 10);  // warps 0 to 9
     ctl->abort_flag = 0;
     mbar_init_fence();
@@ -644,8 +644,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
             odd |= not_finite2<T>(q.x) | not_finite2<T>(q.y) | not_finite2<T>(q.z) | not_finite2<T>(q.w);
           }
           const bool found = (odd & 0x80008000u) != 0;
-          // tile 0's record is read by tile 1 too, perhaps still for the last item that had one
-          if (found && (t || !done1 || wait(&ctl->taken_free, done1 - 1, kErrMmaWait))) {
+          // the record may still be read for the item before: by a slower warp of this tile, and tile 0's by tile 1, whose last item may
+          // lie further back
+          if (found && (t || !done || wait(&ctl->taken_free[0], done - 1, kErrMmaWait)) && (!done1 || wait(&ctl->taken_free[1], done1 - 1, kErrMmaWait))) {
 #pragma unroll 1
             for (int i = 0; i < kTileBytes / 16 / 128; ++i) {
               const int at = (i * 128 + r) * 16, box = at / kBoxBytes, key = (at % kBoxBytes) / 128, chunk = ((at % 128) / 16) ^ (key & 7);
@@ -706,7 +707,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
           store_rows64(smem_u32(stages) + warp * kStageBytes, lane, v, dst + 64 * i, row_bytes, it.len - row0);
         }
         tc_fence_before();
-        if (t) mbar_arrive(&ctl->taken_free);
+        mbar_arrive(&ctl->taken_free[t]);
       }
       unit += 2 * n;
       ++done;

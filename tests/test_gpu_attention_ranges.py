@@ -131,6 +131,30 @@ def test_decode_of_infinite_values(act, cache, d, bad):
         assert torch.equal(out[..., cols], good[..., cols])
 
 
+@pytest.mark.parametrize("act", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_of_infinite_values_in_every_short_prompt(act, d):
+    """Each thread block takes many items one after the other, nearly all of them with an infinity in their last key tile: what is
+    noted of one is not lost to the next."""
+    from fuel_b200 import ops
+    g = torch.Generator().manual_seed(5)
+    lens = torch.randint(1, 129, (2500,), generator=g)
+    lens[::9] += 128
+    start = torch.cat((torch.zeros(1, dtype=torch.long), lens.cumsum(0)))
+    rows, h = int(start[-1]), 2
+    q, k, v = _randn((rows, h, d), 1, act), _randn((rows, 1, d), 2, act), _randn((rows, 1, d), 3, act)
+    where, col = start[:-1] + (torch.rand(2500, generator=g) * lens).long(), torch.randint(0, d, (2500,), generator=g)
+    sign = torch.where(torch.rand(2500, generator=g) < 0.5, -1.0, 1.0)
+    v[where.cuda(), 0, col.cuda()] = (sign * math.inf).to(act).cuda()
+    want = torch.zeros(rows, d)
+    for a, b, c, x in zip(where.tolist(), start[1:].tolist(), col.tolist(), sign.tolist()):
+        want[a:b, c] = x
+    want = want.cuda()[:, None].expand(rows, h, d)
+    for _ in range(10):
+        out = ops.prompt_attn(q, k, v, start.int().cuda()).float()
+        assert torch.equal(torch.where(out.isinf(), out.sign(), 0.0 * out), want)
+
+
 @pytest.mark.parametrize("act", [F32, BF16, F16])
 @pytest.mark.parametrize("d", [64, 128])
 def test_prompt_rows_with_a_score_of_infinity_are_nan(act, d):
