@@ -155,6 +155,51 @@ def test_prompt_of_infinite_values_in_every_short_prompt(act, d):
         assert torch.equal(torch.where(out.isinf(), out.sign(), 0.0 * out), want)
 
 
+# ---- scores at the ends of their range
+
+@pytest.mark.parametrize("act", [BF16, F16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("scale", [1.0, 5.0])
+def test_prompt_of_scores_at_the_ends_of_their_type(act, d, scale):
+    """Scores whose product with log2(e) passes f32's range: the softmax is that of the scores. Among keys of the type's lowest value
+    another takes all; if there are no others they share alike; a key at the highest value takes all."""
+    from fuel_b200 import ops
+    n, h = 300, 2
+    low = torch.finfo(act).min
+    if act == F16:
+        scale *= 2.0 ** 110         # f16's ends are not f32's: the scale takes the scores there
+    v = _randn((n, 1, d), 2, act)
+    q = torch.zeros(n, h, d, dtype=act, device="cuda")
+    q[..., 0] = 1.0
+    half = _HALF.get(act, 0.0)
+    cu = _ints([0, n])
+
+    def close(got, want, mag):      # means of 300 values in f32 sums: 300 * 2^-24 at most
+        assert ((got.double() - want).abs() <= half * (want.abs() + mag) + 2.0 ** -15 * mag).all()
+
+    def same(got, want):            # 32 bits: two f16 parts of each value, the lower one a whole multiple of 2^-24 beside 2^14
+        off = (got.double() - want.double()).abs()
+        assert (off <= (2.0 ** -21 * want.abs() + 2.0 ** -37 * want.abs().max() if act == F32 else 0.0)).all()
+
+    k = torch.zeros(n, 1, d, dtype=act, device="cuda")
+    k[..., 0] = low
+    k[130, 0, 0] = 2.0
+    out = ops.prompt_attn(q, k, v, cu, scale=scale)
+    for row in (0, 1, 127, 129):
+        close(out[row, 0], v[:row + 1, 0].double().mean(0), v[:row + 1, 0].double().abs().mean(0))
+    for row in (130, 131, 255, 299):
+        same(out[row, 0], v[130, 0])
+    k.zero_()
+    for high in (140, 290):
+        k[high, 0, 0] = -low
+    out = ops.prompt_attn(q, k, v, cu, scale=scale)
+    close(out[139, 1], v[:140, 0].double().mean(0), v[:140, 0].double().abs().mean(0))
+    for row in (140, 200, 256, 289):
+        same(out[row, 1], v[140, 0])
+    two = v[[140, 290], 0].double()
+    close(out[295, 0], two.mean(0), two.abs().mean(0))
+
+
 @pytest.mark.parametrize("act", [F32, BF16, F16])
 @pytest.mark.parametrize("d", [64, 128])
 def test_prompt_rows_with_a_score_of_infinity_are_nan(act, d):
