@@ -155,7 +155,7 @@ PromptF32Workspace prompt_f32_workspace(int64_t rows, int heads, int kv, int hea
   w.v = take((size_t)rows * kv * head_dim * 4);
   w.q_up = take((size_t)rows * heads * sizeof(float));
   w.kv_up = take((size_t)rows * kv * sizeof(float2));
-  w.marked = take((size_t)rows * kv * sizeof(int));
+  w.marked = take((size_t)rows * kv * sizeof(int2));
   w.bytes = at;
   return w;
 }
@@ -173,7 +173,7 @@ int32_t launch_prompt_f32(const PromptArgs& r, cudaStream_t stream) {
   p.q_stride = r.q_stride, p.k_stride = r.k_stride, p.v_stride = r.v_stride, p.cu = r.cu, p.n_rows = r.n_rows;
   p.n_items = slots * r.n_heads, p.n_seqs = r.n_seqs, p.n_heads = r.n_heads, p.n_kv = r.n_kv, p.group = r.n_heads / r.n_kv, p.c = r.c;
   p.qp = (__half*)(r.workspace + w.q), p.kp = (__half*)(r.workspace + w.k), p.vp = (__half*)(r.workspace + w.v);
-  p.q_up = (float*)(r.workspace + w.q_up), p.kv_up = (float2*)(r.workspace + w.kv_up), p.marked = (int*)(r.workspace + w.marked);
+  p.q_up = (float*)(r.workspace + w.q_up), p.kv_up = (float2*)(r.workspace + w.kv_up), p.marked = (int2*)(r.workspace + w.marked);
   CUtensorMap qmap, kmap, vmap;  // both parts in one map, the second behind the first
   if (!make_rows_map(p.qp, 2 * r.n_rows, r.n_heads, kHd, (int64_t)r.n_heads * kHd, kPaTile, &qmap) ||
       !make_rows_map(p.kp, 2 * r.n_rows, r.n_kv, kHd, (int64_t)r.n_kv * kHd, kPaTile, &kmap) ||

@@ -7,7 +7,9 @@
 //   v      one for each row and head, put into the weight: with f_j the row's power, w_ij = 2^(s_ij + f_j - m_i), m the maximum of
 //          s + f in the key tile, so that w V' has f16's range whatever the rows' magnitudes. sum_j w_ij 2^-f_j is the softmax's
 //          sum in the same unit as O = sum_j w_ij V'_j, so the result is their quotient
-// so no row loses bits to a larger one, in front of it or behind it, up to 2^100 apart (the powers of a tile of v are held within that of
+// A score is added to a power of two there, which leaves it fewer bits the larger it is, and scores at f32's ends leave it. Rows with a
+// score beyond 2^16 (in units of the exponent) are computed once more at the end, in 64 bits (weigh_again).
+// So no row loses bits to a larger one, in front of it or behind it, up to 2^100 apart (the powers of a tile of v are held within that of
 // its largest, and above 2^-80, for the sums' range). prompt_split_kernel writes the parts and powers (bound by HBM: 4 bytes in,
 // 4 out); values that are not finite are taken out of v there, and the tiles that had some are marked: the few rows that see
 // one add it again from the original at the end.
@@ -42,7 +44,7 @@ struct PromptF32Params {
   __half *qp, *kp, *vp;  // parts: [2][n_rows][heads][hd]
   float* q_up;           // [heads][n_rows]    c 2^eq
   float2* kv_up;         // [n_kv][n_rows]     2^ek, f
-  int* marked;           // [n_kv][n_rows]     at the first row of a tile: does it hold a value that is not finite?
+  int2* marked;          // [n_kv][n_rows]     at the first row of a tile: does it hold a value that is not finite? Its largest ek
 };
 
 // one tile of 128 rows of one head; 64 registers, so that two blocks an SM have 64 KB each in flight (512 rows, 96 heads: one block of 256
@@ -130,9 +132,11 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) prompt_split_kernel(const
       else p.kv_up[at].y = (float)e0;
     }
   }
+  int2* mark = &p.marked[(int64_t)head * p.n_rows + b.first + b.row];
+  if (kind == 1 && threadIdx.x == 0) mark->y = max(most, -112);
   if (kind == 2) {
     const int any = __syncthreads_or(odd);
-    if (threadIdx.x == 0) p.marked[(int64_t)head * p.n_rows + b.first + b.row] = any;
+    if (threadIdx.x == 0) mark->x = any;
   }
 }
 
@@ -152,6 +156,7 @@ struct PromptF32Ctl {
   uint64_t k_full[kPfaRing], k_empty[kPfaRing], v_full[kPfaRing], v_empty[kPfaRing];
   uint32_t tmem_base;
   int abort_flag;
+  int busy[4];  // a warp that holds rows of O is computing some again: the others' waits may take longer
 };
 
 template <int kHd>
@@ -162,15 +167,71 @@ struct PromptF32Cfg {
   static constexpr int kSmem = 1024 + 2 * kTileBytes + 2 * kPfaRing * kUnitBytes + 4 * kStageBytes + (int)sizeof(PromptF32Ctl) + 16;
 };
 
+// Rows of a warp (the bits of `which`) once more, in 64 bits and by the definition: lanes over 32 keys for the scores, over the columns for
+// the values; two passes, so that no sum exceeds the largest value. Values that are not finite are left to add_not_finite. q: the first
+// parts of the warp's first row, the second ones `parts` behind them (the queries themselves may lie under the result); k, v: of the
+// sequence's first; row: the first's number; up: c 2^eq of the lane's row. Some 200 cycles a key and row: for scores that no
+// softmax was meant for
+template <int kHd>
+__device__ __noinline__ void weigh_again(const __half* q, int64_t q_stride, int64_t parts, float up, const float* k, int64_t k_stride, const float* v, int64_t v_stride, int row,
+                                         uint32_t which, float* dst, int64_t dst_stride, int lane) {
+  constexpr int kMine = kHd / 32;
+  for (; which; which &= which - 1) {
+    const int r = __ffs(which) - 1, keys = row + r + 1;
+    const __half2 *hi = reinterpret_cast<const __half2*>(q + r * q_stride), *lo = reinterpret_cast<const __half2*>(q + r * q_stride + parts);
+    const double times = (double)__shfl_sync(0xffffffffu, up, r);
+    auto score = [&](int64_t key) {
+      if (key >= keys) return -(double)INFINITY;
+      const float4* to = reinterpret_cast<const float4*>(k + key * k_stride);
+      double dot = 0.0;
+#pragma unroll 4
+      for (int i = 0; i < kHd / 4; ++i) {
+        const float4 b = to[i];
+        const float2 h0 = __half22float2(hi[2 * i]), h1 = __half22float2(hi[2 * i + 1]), l0 = __half22float2(lo[2 * i]), l1 = __half22float2(lo[2 * i + 1]);
+        dot = fma((double)(h0.x + l0.x), (double)b.x, dot), dot = fma((double)(h0.y + l0.y), (double)b.y, dot);
+        dot = fma((double)(h1.x + l1.x), (double)b.z, dot), dot = fma((double)(h1.y + l1.y), (double)b.w, dot);
+      }
+      return dot * times;
+    };
+    double top = -(double)INFINITY, sum = 0.0;
+    for (int64_t key = 0; key < keys; key += 32) {
+      const double s = score(key + lane);
+      double most = s;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) most = fmax(most, __shfl_xor_sync(0xffffffffu, most, off));
+      if (most > top) sum *= exp2f((float)(top - most)), top = most;
+      if (!(s == -(double)INFINITY)) sum += exp2f((float)(s - top));  // +inf and NaN: NaN
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    const double inv = sum == 0.0 ? 0.0 : 1.0 / sum;
+    double o[kMine] = {};
+    for (int64_t key = 0; key < keys; key += 32) {
+      const double s = score(key + lane);
+      const float w = s == -(double)INFINITY ? 0.f : exp2f((float)(s - top));
+      for (int i = 0; i < min((int64_t)32, keys - key); ++i) {
+        const double wi = (double)__shfl_sync(0xffffffffu, w, i) * inv;
+#pragma unroll
+        for (int e = 0; e < kMine; ++e) {
+          const float x = v[(key + i) * v_stride + lane + 32 * e];
+          o[e] = fma(wi, isfinite(x) ? (double)x : 0.0, o[e]);
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kMine; ++e) dst[r * dst_stride + lane + 32 * e] = (float)o[e];
+  }
+}
+
 // A row of the result whose key tiles hold values that are not finite: adds those that the row sees. v: the head's values of the
 // sequence's first row; marked: the marks of its tiles. (By value: a reference to the kernel's parameters would put all of them on
 // every thread's stack)
 template <int kHd>
-__device__ __noinline__ void add_not_finite(const float* v, int64_t v_stride, const int* marked, int row, float* dst) {
+__device__ __noinline__ void add_not_finite(const float* v, int64_t v_stride, const int2* marked, int row, float* dst) {
   for (int d = 0; d < kHd; ++d) {
     float sum = dst[d];
     for (int tile = 0; tile <= row && !isnan(sum); tile += kPaTile) {
-      if (!marked[tile]) continue;
+      if (!marked[tile].x) continue;
       for (int key = tile; key < tile + kPaTile && key <= row; ++key) {
         const float f = v[key * v_stride + d];
         if (!isfinite(f)) sum += f;
@@ -202,6 +263,7 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
       mbar_init(&ctl->v_full[s], 1), mbar_init(&ctl->v_empty[s], 1);
     }
     ctl->abort_flag = 0;
+    for (int i = 0; i < 4; ++i) ctl->busy[i] = 0;
     mbar_init_fence();
   }
   if (warp == 13) tmem_alloc(&ctl->tmem_base, 512);  // two S (the weights' upper parts over each), their lower parts, O of a tile
@@ -213,6 +275,9 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
   volatile int* abort_flag = &ctl->abort_flag;
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
     if (mbar_poll_bounded(bar, parity & 1u)) return true;
+    const volatile int* busy = ctl->busy;
+    for (int more = 0; more < 1000 && !*abort_flag && (busy[0] | busy[1] | busy[2] | busy[3]); ++more)
+      if (mbar_poll_bounded(bar, parity & 1u)) return true;
     if (!*abort_flag) record_dev_error(code);
     *abort_flag = 1;
     return false;
@@ -489,8 +554,19 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
       const int64_t rows_at = (int64_t)(it.head / p.group) * p.n_rows + it.first;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       bool odd = false;
-      for (int j = lane; j < it.n; j += 32) odd |= p.marked[rows_at + (int64_t)j * kPaTile] != 0;
+      int up = -1000;
+      for (int j = lane; j < it.n; j += 32) {
+        const int2 mark = p.marked[rows_at + (int64_t)j * kPaTile];
+        odd |= mark.x != 0, up = max(up, mark.y);
+      }
       odd = __any_sync(0xffffffffu, odd);
+      up = __reduce_max_sync(0xffffffffu, up);
+      // rows to be computed again: their maximum is beyond 2^16 or has left f32; the product of the powers of their factors may have where
+      // the score itself is of any size
+      bool far = !(fabsf(ref) <= 65536.f);
+      const float q_up = row < it.len ? p.q_up[(int64_t)it.head * p.n_rows + it.first + row] : 0.f;
+      far |= !(q_up * exp2f((float)up) <= 0x1p120f);
+      const uint32_t again = __ballot_sync(0xffffffffu, far && row < it.len);
       const int row0 = row - lane;  // of the warp
       float* dst = p.out + ((it.first + row0) * p.n_heads + it.head) * kHd;
 #pragma unroll
@@ -500,6 +576,15 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e] = o[16 * i + e] * inv;
         store_rows64(smem_u32(stages) + (warp & 3) * kStageBytes, lane, v, reinterpret_cast<uint8_t*>(dst + 16 * i), (int64_t)p.n_heads * kHd * 4, it.len - row0);
+      }
+      if (again) {
+        ctl->busy[warp & 3] = 1;
+        __syncwarp();  // the rows are written
+        const int kvh = it.head / p.group;
+        weigh_again<kHd>(p.qp + ((it.first + row0) * p.n_heads + it.head) * kHd, (int64_t)p.n_heads * kHd, p.n_rows * p.n_heads * kHd, q_up, p.k + it.first * p.k_stride + kvh * kHd, p.k_stride,
+                         p.v + it.first * p.v_stride + kvh * kHd, p.v_stride, row0, again, dst, (int64_t)p.n_heads * kHd, lane);
+        __syncwarp();
+        ctl->busy[warp & 3] = 0;
       }
       if (odd) {
         __syncwarp();  // the rows are written: each lane completes its own

@@ -157,7 +157,7 @@ def test_prompt_of_infinite_values_in_every_short_prompt(act, d):
 
 # ---- scores at the ends of their range
 
-@pytest.mark.parametrize("act", [BF16, F16])
+@pytest.mark.parametrize("act", [F32, BF16, F16])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("scale", [1.0, 5.0])
 def test_prompt_of_scores_at_the_ends_of_their_type(act, d, scale):
@@ -198,6 +198,33 @@ def test_prompt_of_scores_at_the_ends_of_their_type(act, d, scale):
         same(out[row, 1], v[140, 0])
     two = v[[140, 290], 0].double()
     close(out[295, 0], two.mean(0), two.abs().mean(0))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_of_large_scores_alike(d):
+    """Equal keys whose scores lie beyond 2^16, in two key tiles and more, values of different magnitudes: every row is the mean of the
+    values, in place of the queries too."""
+    from fuel_b200 import ops
+    n, h = 1000, 2
+    q, k, v = _randn((n, h, d), 1, F32), _randn((1, 1, d), 2, F32, 2.0 ** 20).expand(n, 1, d).contiguous(), _randn((n, 1, d), 3, F32)
+    v[::7] *= 2.0 ** -12
+    out = ops.prompt_attn(q, k, v, _ints([0, n]))
+    want = v.double().cumsum(0) / torch.arange(1, n + 1, device="cuda")[:, None, None]
+    assert ((out.double() - want).norm() / (want.norm() * h ** 0.5)).item() <= 4.1e-6
+    assert torch.equal(ops.prompt_attn(q, k, v, _ints([0, n]), out=q), out) and torch.equal(q, out)
+
+
+def test_prompt_of_factors_whose_powers_pass_f32():
+    """Large columns of q meet columns of zero in k and the other way round: the scores are of a few units."""
+    from fuel_b200 import ops
+    n, d = 200, 64
+    q, k, v = (_randn((n, 1, d), s, F32) for s in (1, 2, 3))
+    q[..., 0], k[..., 0] = 2.0 ** 100, 0.0
+    q[..., 1], k[..., 1] = 0.0, 2.0 ** 100
+    q[..., 2:], k[..., 2:] = 0.0, 0.0         # what is left of them beside 2^100 is zero in any 22 bits
+    out = ops.prompt_attn(q, k, v, _ints([0, n]))
+    want = v.double().cumsum(0) / torch.arange(1, n + 1, device="cuda")[:, None, None]
+    assert ((out.double() - want).norm() / want.norm()).item() <= 4.1e-6
 
 
 @pytest.mark.parametrize("act", [F32, BF16, F16])
