@@ -9,8 +9,8 @@
 //          sum in the same unit as O = sum_j w_ij V'_j, so the result is their quotient
 // A score is added to a power of two there, which leaves it fewer bits the larger it is, and scores at f32's ends leave it. Rows with a
 // score beyond 2^16 (in units of the exponent) are computed once more at the end, in 64 bits (weigh_again).
-// So no row loses bits to a larger one, in front of it or behind it, up to 2^100 apart (the powers of a tile of v are held within that of
-// its largest, and above 2^-80, for the sums' range). prompt_split_kernel writes the parts and powers (bound by HBM: 4 bytes in,
+// So do rows that see values of more than 2^100 apart, whose sums would need more than f32's range. The powers of v stay above 2^-80 and,
+// in a tile, within 2^100 of the largest before them: no row loses bits to a larger one behind it. prompt_split_kernel writes the parts and powers (bound by HBM: 4 bytes in,
 // 4 out); values that are not finite are taken out of v there, and the tiles that had some are marked: the few rows that see
 // one add it again from the original at the end.
 // The tensor cores' f32 sums round towards zero, which over a long row adds up (1.6e-5 of it at 4000 keys). So they sum one
@@ -44,7 +44,8 @@ struct PromptF32Params {
   __half *qp, *kp, *vp;  // parts: [2][n_rows][heads][hd]
   float* q_up;           // [heads][n_rows]    c 2^eq
   float2* kv_up;         // [n_kv][n_rows]     2^ek, f
-  int2* marked;          // [n_kv][n_rows]     at the first row of a tile: does it hold a value that is not finite? Its largest ek
+  int2* marked;          // [n_kv][n_rows]     at the first row of a tile: does it hold a value that is not finite (bit 0), 128 + its largest
+                         //                    f (bits 8 to 15) and its least (16 to 23); its largest ek
 };
 
 // one tile of 128 rows of one head; 64 registers, so that two blocks an SM have 64 KB each in flight (512 rows, 96 heads: one block of 256
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) prompt_split_kernel(const
     }
   }
   bool odd = false;
-  int power[kMine], most = -1000;  // the largest value of a row comes to [2^14, 2^15)
+  int power[kMine];  // the largest value of a row comes to [2^14, 2^15)
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
     float top = 0.f;
@@ -96,19 +97,37 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) prompt_split_kernel(const
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
     power[i] = top > 0.f ? ilogbf(top) - 14 : -1000;
-    most = max(most, power[i]);
   }
-  __shared__ int most_s[kSplitWarps];
-  if (lane == 0) most_s[warp] = most;
-  __syncthreads();
+  // k, v: the largest power of a row and those before it in the tile. Lane l finds it for row 4 l + the last two bits of this warp's rows
+  __shared__ alignas(16) int power_s[kPaTile];
+  __shared__ int least_s;
+  int before = 0, most = 0, least = 1000;
+  if (kind != 0) {
+    if (threadIdx.x == 0) least_s = 1000;
 #pragma unroll
-  for (int w = 0; w < kSplitWarps; ++w) most = max(most, most_s[w]);
+    for (int i = 0; i < kMine; ++i)
+      if (lane == 0) power_s[warp + kSplitWarps * i] = power[i];
+    __syncthreads();
+    const int4 q = reinterpret_cast<const int4*>(power_s)[lane];
+    const int of[4] = {q.x, max(q.x, q.y), max(max(q.x, q.y), q.z), max(max(q.x, q.y), max(q.z, q.w))};
+    int upto = of[3];
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto = max(upto, o);
+    }
+    const int lower = __shfl_up_sync(0xffffffffu, upto, 1), own = warp & 2 ? (warp & 1 ? of[3] : of[2]) : (warp & 1 ? of[1] : of[0]);
+    before = lane ? max(lower, own) : own;
+    most = __shfl_sync(0xffffffffu, upto, 31);
+  }
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
+    const int largest = __shfl_sync(0xffffffffu, before, (warp + kSplitWarps * i) >> 2);
     if (warp + kSplitWarps * i >= rows) break;
     const int64_t row = b.first + b.row + warp + kSplitWarps * i;
     // q, k: a row of zeros or nothing but denormals keeps a power in f32's range
-    const int e0 = kind == 2 ? max(power[i], max(most - 100, -80)) : max(power[i], -112);
+    const int e0 = kind == 2 ? max(power[i], max(largest - 100, -80)) : max(power[i], -112);
+    least = min(least, e0);
     const float down = exp2f((float)-e0);
     alignas(8) __half hi[kPer], lo[kPer];
 #pragma unroll
@@ -135,8 +154,9 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) prompt_split_kernel(const
   int2* mark = &p.marked[(int64_t)head * p.n_rows + b.first + b.row];
   if (kind == 1 && threadIdx.x == 0) mark->y = max(most, -112);
   if (kind == 2) {
+    if (lane == 0) atomicMin(&least_s, least);
     const int any = __syncthreads_or(odd);
-    if (threadIdx.x == 0) mark->x = any;
+    if (threadIdx.x == 0) mark->x = (any ? 1 : 0) | (128 + max(most, -80)) << 8 | (128 + least_s) << 16;
   }
 }
 
@@ -166,6 +186,24 @@ struct PromptF32Cfg {
   static constexpr int kUnits = kTileBytes / kUnitBytes, kUnitKeys = kPaTile / kUnits;
   static constexpr int kSmem = 1024 + 2 * kTileBytes + 2 * kPfaRing * kUnitBytes + 4 * kStageBytes + (int)sizeof(PromptF32Ctl) + 16;
 };
+
+// Whether the values that row `row0 + lane` of a sequence of `len` rows sees lie more than 2^100 apart; up: of its first row
+__device__ __noinline__ bool sees_far_apart(const float2* up, int row0, int len, int lane) {
+  float above = -INFINITY, below = INFINITY;
+  for (int key = lane; key < row0; key += 32) above = fmaxf(above, up[key].y), below = fminf(below, up[key].y);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    above = fmaxf(above, __shfl_xor_sync(0xffffffffu, above, off));
+    below = fminf(below, __shfl_xor_sync(0xffffffffu, below, off));
+  }
+  if (row0 + lane < len) above = fmaxf(above, up[row0 + lane].y), below = fminf(below, up[row0 + lane].y);
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const float a = __shfl_up_sync(0xffffffffu, above, off), b = __shfl_up_sync(0xffffffffu, below, off);
+    if (lane >= off) above = fmaxf(above, a), below = fminf(below, b);
+  }
+  return above - below > 100.f;
+}
 
 // Rows of a warp (the bits of `which`) once more, in 64 bits and by the definition: lanes over 32 keys for the scores, over the columns for
 // the values; two passes, so that no sum exceeds the largest value. Values that are not finite are left to add_not_finite. q: the first
@@ -231,7 +269,7 @@ __device__ __noinline__ void add_not_finite(const float* v, int64_t v_stride, co
   for (int d = 0; d < kHd; ++d) {
     float sum = dst[d];
     for (int tile = 0; tile <= row && !isnan(sum); tile += kPaTile) {
-      if (!marked[tile].x) continue;
+      if (!(marked[tile].x & 1)) continue;
       for (int key = tile; key < tile + kPaTile && key <= row; ++key) {
         const float f = v[key * v_stride + d];
         if (!isfinite(f)) sum += f;
@@ -551,23 +589,25 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
       }
       if (!ok) break;
       const int row = it.row + r;
+      const int row0 = row - lane;  // of the warp
       const int64_t rows_at = (int64_t)(it.head / p.group) * p.n_rows + it.first;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       bool odd = false;
-      int up = -1000;
+      int up = -1000, above = 0, below = 255;
       for (int j = lane; j < it.n; j += 32) {
         const int2 mark = p.marked[rows_at + (int64_t)j * kPaTile];
-        odd |= mark.x != 0, up = max(up, mark.y);
+        odd |= mark.x & 1, up = max(up, mark.y);
+        above = max(above, mark.x >> 8 & 255), below = min(below, mark.x >> 16);
       }
       odd = __any_sync(0xffffffffu, odd);
       up = __reduce_max_sync(0xffffffffu, up);
       // rows to be computed again: their maximum is beyond 2^16 or has left f32; the product of the powers of their factors may have where
-      // the score itself is of any size
+      // the score itself is of any size; they see values too far apart
       bool far = !(fabsf(ref) <= 65536.f);
       const float q_up = row < it.len ? p.q_up[(int64_t)it.head * p.n_rows + it.first + row] : 0.f;
       far |= !(q_up * exp2f((float)up) <= 0x1p120f);
+      if (__reduce_max_sync(0xffffffffu, above) - __reduce_min_sync(0xffffffffu, below) > 100) far |= sees_far_apart(p.kv_up + rows_at, row0, it.len, lane);
       const uint32_t again = __ballot_sync(0xffffffffu, far && row < it.len);
-      const int row0 = row - lane;  // of the warp
       float* dst = p.out + ((it.first + row0) * p.n_heads + it.head) * kHd;
 #pragma unroll
       for (int i = 0; i < kHd / 16; ++i) {

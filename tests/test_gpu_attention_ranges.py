@@ -282,9 +282,29 @@ def test_prompt_rows_whose_first_keys_score_minus_infinity(act, d):
         assert ((out[row].double() - want).abs() <= _HALF[act] * (want.abs() + mag) + 2.0 ** -15 * mag).all(), row
 
 
+# ---- large values
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("gap", [-30.0, 0.0, 10.0, 14.0])
+def test_prompt_of_values_as_far_apart_as_f32_goes(d, gap):
+    """A value of 2^125 among values of one, in the same key tile and in others: what the others weigh is in the softmax's sum."""
+    from fuel_b200 import ops
+    n = 400
+    q, k, v = _randn((n, 1, d), 1, F32, 0.3), _randn((n, 1, d), 2, F32), _randn((n, 1, d), 3, F32)
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    for at in (50, 300):
+        k[at], v[at] = 0.0, v[at] * 2.0 ** 125
+        k[at, 0, 0] = gap / (8.0 * d ** -0.5)
+    out = ops.prompt_attn(q, k, v, _ints([0, n]))
+    for row in (0, 49, 50, 51, 127, 128, 255, 299, 300, 399):
+        want, _ = _attend(q[row].double(), k[:row + 1, 0].double(), v[:row + 1, 0].double(), d ** -0.5)
+        off = out[row].double() - want
+        assert (off.norm() / want.norm()).item() <= 4.1e-6 + abs(gap) * 2.0 ** -22, row
+
+
 # ---- large values behind a row
 
-@pytest.mark.parametrize("act", [F16, BF16])
+@pytest.mark.parametrize("act", [F32, F16, BF16])
 @pytest.mark.parametrize("d", [64, 128])
 def test_prompt_rows_do_not_see_large_values_behind_them(act, d):
     """The type's largest values in later rows of the sequence, in the next one and behind the last: weights of zero, not nearly."""
