@@ -261,22 +261,44 @@ __device__ __noinline__ void weigh_again(const __half* q, int64_t q_stride, int6
   }
 }
 
-// A row of the result whose key tiles hold values that are not finite: adds those that the row sees. v: the head's values of the
-// sequence's first row; marked: the marks of its tiles. (By value: a reference to the kernel's parameters would put all of them on
-// every thread's stack)
+// The rows of a warp whose key tiles hold values that are not finite: adds those that each row sees, the lanes' columns side by side: the
+// first key with +inf, -inf, NaN of every column, looked for once for all rows. (A lane by itself for its row, column after column,
+// takes seconds where a long prompt's values are infinite throughout, and the block's other warps wait two.) v: the head's values of the
+// sequence's first row; marked: the marks of its tiles; row: the warp's first; dst: its result. (By value: a reference to the
+// kernel's parameters would put all of them on every thread's stack)
 template <int kHd>
-__device__ __noinline__ void add_not_finite(const float* v, int64_t v_stride, const int2* marked, int row, float* dst) {
-  for (int d = 0; d < kHd; ++d) {
-    float sum = dst[d];
-    for (int tile = 0; tile <= row && !isnan(sum); tile += kPaTile) {
-      if (!(marked[tile].x & 1)) continue;
-      for (int key = tile; key < tile + kPaTile && key <= row; ++key) {
-        const float f = v[key * v_stride + d];
-        if (!isfinite(f)) sum += f;
-      }
+__device__ __noinline__ void add_not_finite(const float* v, int64_t v_stride, const int2* marked, int row, int rows, float* dst, int64_t dst_stride, int lane) {
+  constexpr int kMine = kHd / 32, kNone = 0x7fffffff;
+  int first[3][kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) first[0][i] = first[1][i] = first[2][i] = kNone;
+  const int end = row + rows;
+  for (int64_t from = 0; from < end; from += 32 * kPaTile) {
+    const int64_t mine = from + lane * kPaTile;
+    uint32_t tiles = __ballot_sync(0xffffffffu, mine < end && (marked[mine].x & 1));
+    for (; tiles; tiles &= tiles - 1) {
+      const int key0 = (int)from + (__ffs(tiles) - 1) * kPaTile, key1 = min(key0 + kPaTile, end);
+#pragma unroll 8
+      for (int key = key0; key < key1; ++key)
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const float f = v[key * v_stride + lane + 32 * i];
+          if (!isfinite(f)) {
+            int& at = f != f ? first[2][i] : f < 0.f ? first[1][i] : first[0][i];
+            at = min(at, key);
+          }
+        }
     }
-    dst[d] = sum;
   }
+  for (int r = 0; r < rows; ++r)
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      float sum = dst[r * dst_stride + lane + 32 * i];
+      if (first[0][i] <= row + r) sum += INFINITY;
+      if (first[1][i] <= row + r) sum -= INFINITY;
+      if (first[2][i] <= row + r) sum += __int_as_float(0x7fc00000);
+      dst[r * dst_stride + lane + 32 * i] = sum;
+    }
 }
 
 template <int kHd>
@@ -626,10 +648,13 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
         __syncwarp();
         ctl->busy[warp & 3] = 0;
       }
-      if (odd) {
-        __syncwarp();  // the rows are written: each lane completes its own
-        if (row < it.len)
-          add_not_finite<kHd>(p.v + it.first * p.v_stride + (it.head / p.group) * kHd, p.v_stride, p.marked + rows_at, row, dst + (int64_t)lane * p.n_heads * kHd);
+      if (odd && row0 < it.len) {
+        ctl->busy[warp & 3] = 1;
+        __syncwarp();  // the rows are written
+        add_not_finite<kHd>(p.v + it.first * p.v_stride + (it.head / p.group) * kHd, p.v_stride, p.marked + rows_at, row0, min(32, it.len - row0), dst,
+                            (int64_t)p.n_heads * kHd, lane);
+        __syncwarp();
+        ctl->busy[warp & 3] = 0;
       }
       __syncwarp();
     }
