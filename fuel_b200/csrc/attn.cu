@@ -27,6 +27,8 @@ inline int page_shift_of(int page_size) {
 inline bool stride_ok(int64_t stride, int heads, int head_dim, int act) {
   return stride >= (int64_t)heads * head_dim && stride * type_bytes(act) % 16 == 0;
 }
+// the kernels take scale log2(e), which has to be a number too
+inline bool scale_ok(float scale) { return scale > 0.f && scale <= 0x1p127f; }
 constexpr int64_t kMaxRows = 0x7fffffff, kMaxPromptRows = (1 << 30) - 256;  // prompts: twice as many are a coordinate of a copy
 constexpr int64_t kMaxSlots = 1 << 26;  // empty sequences times heads, which a warp looks through while the others' waits run
 constexpr int kMaxHeads = 16383;  // q, k and v heads together are a grid dimension
@@ -258,7 +260,7 @@ int32_t fuelq_paged_attn_decode(int32_t act_type, int32_t cache_type, const void
   if (!type_pair(act_type, cache_type) || (head_dim != 64 && head_dim != 128)) return kNotSupported;
   const int shift = page_shift_of(page_size);
   if (shift < 0) return kNotSupported;
-  if (n_seqs < 0 || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !(scale > 0.f) || std::isinf(scale) || n_pages < 0 || max_pages < 0) return kInvalidProblem;
+  if (n_seqs < 0 || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !scale_ok(scale) || n_pages < 0 || max_pages < 0) return kInvalidProblem;
   if (n_seqs == 0) return kOk;
   if (!q || !kcache || !vcache || !out || !page_table || !seq_lens) return kInvalidProblem;
   if (!stride_ok(q_stride, n_heads, head_dim, act_type)) return kInvalidProblem;
@@ -291,7 +293,7 @@ int32_t fuelq_prompt_attn(int32_t act_type, const void* q, int64_t q_stride, con
                           int32_t n_heads, int32_t n_kv, int32_t head_dim, float scale, void* workspace,
                           size_t workspace_bytes, void* stream) {
   if (!type_bytes(act_type) || (head_dim != 64 && head_dim != 128)) return kNotSupported;
-  if (n_seqs < 0 || n_rows < 0 || n_rows > kMaxPromptRows || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !(scale > 0.f) || std::isinf(scale)) return kInvalidProblem;
+  if (n_seqs < 0 || n_rows < 0 || n_rows > kMaxPromptRows || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !scale_ok(scale)) return kInvalidProblem;
   if ((int64_t)n_seqs * n_heads > kMaxSlots) return kNotSupported;
   if (n_seqs == 0 || n_rows == 0) return kOk;
   if (!q || !k || !v || !out || !cu_seqlens) return kInvalidProblem;

@@ -409,7 +409,7 @@ int32_t fuelq_argmax_last(const float* x, int64_t n, int32_t* out_index, void* s
  * with the maximum taken off, f32 sums.
  * Types: act_type is the type of q, k, v and the outputs, cache_type that of the pages: F32, F16 or BF16. f32 activations go
  * with every cache type, 16-bit ones with a cache of their own type. head_dim is 64 or 128, n_heads a multiple of n_kv (query
- * head h reads kv head h / (n_heads / n_kv)); scale is finite and positive.
+ * head h reads kv head h / (n_heads / n_kv)); scale is positive and at most 2^127.
  * Scores: a score of -inf is a weight of zero, and a row with no other scores gives zeros; one of +inf or NaN makes its row NaN.
  * Finite products of q and k stay finite when they are scaled. With 32-bit activations an infinity in q or k makes its scores
  * NaN.
