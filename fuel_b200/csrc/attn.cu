@@ -219,7 +219,10 @@ int32_t fuelq_paged_append(int32_t act_type, int32_t cache_type, const void* k, 
   if (n_rows < 0 || n_rows > kMaxRows || n_seqs < 0 || n_kv <= 0 || n_pages < 0 || max_pages < 0 || max_pos < 0) return kInvalidProblem;
   if (q && (n_heads <= 0 || n_heads % n_kv)) return kInvalidProblem;
   if (n_rows == 0) return kOk;
-  if (!k || !v || !kcache || !vcache || !page_table || !positions || !cos_table || !sin_table || (q && !q_out)) return kInvalidProblem;
+  // a cache without pages, a table without columns, angles of no positions: nothing is read of them
+  if (!k || !v || (n_pages && (!kcache || !vcache)) || (max_pages && n_seqs && !page_table) || !positions || (max_pos && (!cos_table || !sin_table)) ||
+      (q && !q_out))
+    return kInvalidProblem;
   if (!stride_ok(k_stride, n_kv, head_dim, act_type) || !stride_ok(v_stride, n_kv, head_dim, act_type)) return kInvalidProblem;
   if (q && !stride_ok(q_stride, n_heads, head_dim, act_type)) return kInvalidProblem;
   if (!seq_ids && n_rows > n_seqs) return kInvalidProblem;
@@ -262,7 +265,7 @@ int32_t fuelq_paged_attn_decode(int32_t act_type, int32_t cache_type, const void
   if (shift < 0) return kNotSupported;
   if (n_seqs < 0 || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !scale_ok(scale) || n_pages < 0 || max_pages < 0) return kInvalidProblem;
   if (n_seqs == 0) return kOk;
-  if (!q || !kcache || !vcache || !out || !page_table || !seq_lens) return kInvalidProblem;
+  if (!q || (n_pages && (!kcache || !vcache)) || !out || (max_pages && !page_table) || !seq_lens) return kInvalidProblem;
   if (!stride_ok(q_stride, n_heads, head_dim, act_type)) return kInvalidProblem;
   const size_t need = fuelq_paged_attn_workspace_bytes(n_seqs, n_heads, n_kv, head_dim);
   if (need && (!workspace || workspace_bytes < need)) return kWorkspace;

@@ -334,3 +334,22 @@ def test_prompt_rows_do_not_see_large_values_behind_them(act, d):
             b[300:] = bad
             out = ops.prompt_attn(q, k, b, cu)
             assert torch.equal(out[:at], want[:at]), (bad, at)
+
+
+# ---- nothing in the cache yet
+
+@pytest.mark.parametrize("act,cache", [(F32, F16), (BF16, BF16)])
+def test_a_batch_of_free_slots_without_pages(act, cache):
+    """No page and no column of the table: padding is skipped, free slots are zeros, anything else is told."""
+    from fuel_b200 import _lib, ops
+    n, h, kv, d = 3, 4, 2, 64
+    q, k, v = _randn((n, h, d), 1, act), _randn((n, kv, d), 2, act), _randn((n, kv, d), 3, act)
+    kc, vc = (torch.empty(0, kv, 16, d, dtype=cache, device="cuda") for _ in range(2))
+    table, cos = torch.empty(n, 0, dtype=torch.int32, device="cuda"), torch.empty(0, d, device="cuda")
+    ops.paged_append(k, v, kc, vc, table, _ints([-1, -1, -1]), cos, cos, q=q)
+    assert not ops.paged_attn_decode(q, kc, vc, table, _ints([0, -3, 0])).any()
+    assert ops.device_error() == 0
+    ops.paged_append(k, v, kc, vc, table, _ints([-1, 0, -1]), cos, cos, q=q)
+    assert ops.device_error() == _lib.DEVICE_ERROR_INDEX
+    assert not ops.paged_attn_decode(q, kc, vc, table, _ints([0, 2, 0])).any()
+    assert ops.device_error() == _lib.DEVICE_ERROR_INDEX
