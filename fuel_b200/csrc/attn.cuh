@@ -75,10 +75,11 @@ struct AppendParams {
 };
 constexpr int kAppendThreads = 128;
 
-// 16-bit rows: 64 registers, so that eight blocks an SM keep enough rows in flight (13009 rows of bf16, 32/8 heads of 128: 58.9 us
-// = 5.9 TB/s, with 92 registers and four lines in flight 70.5; 32-bit rows lose by it: 1023 of them 5.7 us against 4.9)
+// 64 registers, so that eight blocks an SM keep enough rows in flight. 13009 rows, 32/8 heads of 128: bf16 56.7 us, 5.6 TB/s of rows and
+// cache (with more registers and fewer blocks 75.5), f32 98.4, 6.5 TB/s (106.5), f32 over f16 89.3, 6.6 TB/s (99.6). 1023 rows: 5.7 (7.4),
+// 10.9 (10.5), 9.8 (9.7)
 template <typename A, typename C, int kHd>
-__global__ void __launch_bounds__(kAppendThreads, sizeof(A) == 4 ? 1 : 8) paged_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, 8) paged_append_kernel(const AppendParams p) {
   constexpr int kHalf = kHd / 2, kChunks = kHalf / 8, kSlots = kAppendThreads / kChunks;
   constexpr int kBatch = 2;  // lines a thread has in flight
   pdl_launch_dependents();
