@@ -7,8 +7,8 @@
 //   v      one for each row and head, put into the weight: with f_j the row's power, w_ij = 2^(s_ij + f_j - m_i), m the maximum of
 //          s + f in the key tile, so that w V' has f16's range whatever the rows' magnitudes. sum_j w_ij 2^-f_j is the softmax's
 //          sum in the same unit as O = sum_j w_ij V'_j, so the result is their quotient
-// A score is added to a power of two there, which leaves it fewer bits the larger it is, and scores at f32's ends leave it. Rows with a
-// score beyond 2^16 (in units of the exponent) are computed once more at the end, in 64 bits (weigh_again).
+// A score is added to a whole power there, which loses nothing while the score is below 2^23 or so, and scores at f32's ends leave it. Rows
+// whose largest is beyond 2^22 (in units of the exponent) are computed once more at the end, with sums in 64 bits (weigh_again).
 // So do rows that see values of more than 2^100 apart, whose sums would need more than f32's range. The powers of v stay above 2^-80 and,
 // in a tile, within 2^100 of the largest before them: no row loses bits to a larger one behind it. prompt_split_kernel writes the parts and powers (bound by HBM: 4 bytes in,
 // 4 out); values that are not finite are taken out of v there, and the tiles that had some are marked: the few rows that see
@@ -205,59 +205,61 @@ __device__ __noinline__ bool sees_far_apart(const float2* up, int row0, int len,
   return above - below > 100.f;
 }
 
-// Rows of a warp (the bits of `which`) once more, in 64 bits and by the definition: lanes over 32 keys for the scores, over the columns for
-// the values; two passes, so that no sum exceeds the largest value. Values that are not finite are left to add_not_finite. q: the first
-// parts of the warp's first row, the second ones `parts` behind them (the queries themselves may lie under the result); k, v: of the
-// sequence's first; row: the first's number; up: c 2^eq of the lane's row. Some 200 cycles a key and row: for scores that no
-// softmax was meant for
+// Rows of a warp (the bits of `which`) once more, by the definition with sums in 64 bits: four keys at a time, the lanes over the columns.
+// Values that are not finite are left to add_not_finite. q: the first parts of the warp's first row, the second ones `parts` behind them
+// (the queries themselves may lie under the result); k, v: of the sequence's first; row: the first's number; up: c 2^eq of the
+// lane's row
 template <int kHd>
-__device__ __noinline__ void weigh_again(const __half* q, int64_t q_stride, int64_t parts, float up, const float* k, int64_t k_stride, const float* v, int64_t v_stride, int row,
-                                         uint32_t which, float* dst, int64_t dst_stride, int lane) {
-  constexpr int kMine = kHd / 32;
+__device__ __noinline__ void weigh_again(const __half* q, int64_t q_stride, int64_t parts, float up, const float* k, int64_t k_stride, const float* v,
+                                         int64_t v_stride, int row, uint32_t which, float* dst, int64_t dst_stride, int lane) {
+  constexpr int kMine = kHd / 32, kKeys = 4;
   for (; which; which &= which - 1) {
-    const int r = __ffs(which) - 1, keys = row + r + 1;
-    const __half2 *hi = reinterpret_cast<const __half2*>(q + r * q_stride), *lo = reinterpret_cast<const __half2*>(q + r * q_stride + parts);
+    const int r = __ffs(which) - 1;
+    double x[kMine], o[kMine] = {}, top = -(double)INFINITY, sum = 0.0;
     const double times = (double)__shfl_sync(0xffffffffu, up, r);
-    auto score = [&](int64_t key) {
-      if (key >= keys) return -(double)INFINITY;
-      const float4* to = reinterpret_cast<const float4*>(k + key * k_stride);
-      double dot = 0.0;
-#pragma unroll 4
-      for (int i = 0; i < kHd / 4; ++i) {
-        const float4 b = to[i];
-        const float2 h0 = __half22float2(hi[2 * i]), h1 = __half22float2(hi[2 * i + 1]), l0 = __half22float2(lo[2 * i]), l1 = __half22float2(lo[2 * i + 1]);
-        dot = fma((double)(h0.x + l0.x), (double)b.x, dot), dot = fma((double)(h0.y + l0.y), (double)b.y, dot);
-        dot = fma((double)(h1.x + l1.x), (double)b.z, dot), dot = fma((double)(h1.y + l1.y), (double)b.w, dot);
-      }
-      return dot * times;
-    };
-    double top = -(double)INFINITY, sum = 0.0;
-    for (int64_t key = 0; key < keys; key += 32) {
-      const double s = score(key + lane);
-      double most = s;
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) most = fmax(most, __shfl_xor_sync(0xffffffffu, most, off));
-      if (most > top) sum *= exp2f((float)(top - most)), top = most;
-      if (!(s == -(double)INFINITY)) sum += exp2f((float)(s - top));  // +inf and NaN: NaN
+    for (int e = 0; e < kMine; ++e) {
+      const __half* at = q + r * q_stride + lane + 32 * e;
+      x[e] = (double)(__half2float(at[0]) + __half2float(at[parts])) * times;
     }
+    for (int64_t key = 0; key <= row + r; key += kKeys) {
+      double s[kKeys], most = top;
+      float y[kKeys][kMine];
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    const double inv = sum == 0.0 ? 0.0 : 1.0 / sum;
-    double o[kMine] = {};
-    for (int64_t key = 0; key < keys; key += 32) {
-      const double s = score(key + lane);
-      const float w = s == -(double)INFINITY ? 0.f : exp2f((float)(s - top));
-      for (int i = 0; i < min((int64_t)32, keys - key); ++i) {
-        const double wi = (double)__shfl_sync(0xffffffffu, w, i) * inv;
+      for (int i = 0; i < kKeys; ++i) {
+        const int64_t at = min(key + i, (int64_t)(row + r));
+        s[i] = 0.0;
 #pragma unroll
         for (int e = 0; e < kMine; ++e) {
-          const float x = v[(key + i) * v_stride + lane + 32 * e];
-          o[e] = fma(wi, isfinite(x) ? (double)x : 0.0, o[e]);
+          s[i] = fma(x[e], (double)k[at * k_stride + lane + 32 * e], s[i]);
+          y[i][e] = v[at * v_stride + lane + 32 * e];
         }
       }
-    }
 #pragma unroll
-    for (int e = 0; e < kMine; ++e) dst[r * dst_stride + lane + 32 * e] = (float)o[e];
+      for (int i = 0; i < kKeys; ++i) {
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], off);
+        if (key + i > row + r) s[i] = -(double)INFINITY;
+        most = fmax(most, s[i]);
+      }
+      if (most > top) {
+        const double keep = exp2f((float)(top - most));
+        sum *= keep;
+#pragma unroll
+        for (int e = 0; e < kMine; ++e) o[e] *= keep;
+        top = most;
+      }
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i) {
+        const double w = s[i] == -(double)INFINITY ? 0.0 : exp2f((float)(s[i] - top));  // +inf and NaN: NaN
+        sum += w;
+#pragma unroll
+        for (int e = 0; e < kMine; ++e) o[e] = fma(w, isfinite(y[i][e]) ? (double)y[i][e] : 0.0, o[e]);
+      }
+    }
+    const double inv = sum == 0.0 ? 0.0 : 1.0 / sum;
+#pragma unroll
+    for (int e = 0; e < kMine; ++e) dst[r * dst_stride + lane + 32 * e] = (float)(o[e] * inv);
   }
 }
 
@@ -623,11 +625,11 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
       }
       odd = __any_sync(0xffffffffu, odd);
       up = __reduce_max_sync(0xffffffffu, up);
-      // rows to be computed again: their maximum is beyond 2^16 or has left f32; the product of the powers of their factors may have where
-      // the score itself is of any size; they see values too far apart
-      bool far = !(fabsf(ref) <= 65536.f);
-      const float q_up = row < it.len ? p.q_up[(int64_t)it.head * p.n_rows + it.first + row] : 0.f;
-      far |= !(q_up * exp2f((float)up) <= 0x1p120f);
+      // rows to be computed again: their maximum is beyond 2^22 or has left f32, where the powers of their factors allow it (a product of two
+      // parts is below 2^37; otherwise an infinity in q or k has made it); the powers' product may leave f32 where the score itself is
+      // of any size; the values lie too far apart
+      const float q_up = row < it.len ? p.q_up[(int64_t)it.head * p.n_rows + it.first + row] : 0.f, reach = q_up * exp2f((float)up);
+      bool far = (reach > 0x1p-15f && !(fabsf(ref) <= 0x1p22f)) || !(reach <= 0x1p120f);
       if (__reduce_max_sync(0xffffffffu, above) - __reduce_min_sync(0xffffffffu, below) > 100) far |= sees_far_apart(p.kv_up + rows_at, row0, it.len, lane);
       const uint32_t again = __ballot_sync(0xffffffffu, far && row < it.len);
       float* dst = p.out + ((it.first + row0) * p.n_heads + it.head) * kHd;

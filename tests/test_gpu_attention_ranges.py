@@ -201,12 +201,13 @@ def test_prompt_of_scores_at_the_ends_of_their_type(act, d, scale):
 
 
 @pytest.mark.parametrize("d", [64, 128])
-def test_prompt_of_large_scores_alike(d):
-    """Equal keys whose scores lie beyond 2^16, in two key tiles and more, values of different magnitudes: every row is the mean of the
-    values, in place of the queries too."""
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 17, 2.0 ** 20, 2.0 ** 24, 2.0 ** 60])
+def test_prompt_of_large_scores_alike(d, size):
+    """Equal keys of large scores, in two key tiles and more, values of different magnitudes: every row is the mean of the values, in
+    place of the queries too."""
     from fuel_b200 import ops
     n, h = 1000, 2
-    q, k, v = _randn((n, h, d), 1, F32), _randn((1, 1, d), 2, F32, 2.0 ** 20).expand(n, 1, d).contiguous(), _randn((n, 1, d), 3, F32)
+    q, k, v = _randn((n, h, d), 1, F32), _randn((1, 1, d), 2, F32, size).expand(n, 1, d).contiguous(), _randn((n, 1, d), 3, F32)
     v[::7] *= 2.0 ** -12
     out = ops.prompt_attn(q, k, v, _ints([0, n]))
     want = v.double().cumsum(0) / torch.arange(1, n + 1, device="cuda")[:, None, None]
