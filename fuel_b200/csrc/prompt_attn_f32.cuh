@@ -279,28 +279,31 @@ __device__ __noinline__ void add_not_finite(const float* v, int64_t v_stride, co
     const int64_t mine = from + lane * kPaTile;
     uint32_t tiles = __ballot_sync(0xffffffffu, mine < end && (marked[mine].x & 1));
     for (; tiles; tiles &= tiles - 1) {
-      const int key0 = (int)from + (__ffs(tiles) - 1) * kPaTile, key1 = min(key0 + kPaTile, end);
+      const int key0 = (int)from + (__ffs(tiles) - 1) * kPaTile;
 #pragma unroll 8
-      for (int key = key0; key < key1; ++key)
+      for (int n = 0; n < kPaTile; ++n)
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
+          const int key = min(key0 + n, end - 1);
           const float f = v[key * v_stride + lane + 32 * i];
-          if (!isfinite(f)) {
-            int& at = f != f ? first[2][i] : f < 0.f ? first[1][i] : first[0][i];
-            at = min(at, key);
-          }
+          first[0][i] = f == INFINITY ? min(first[0][i], key) : first[0][i];
+          first[1][i] = f == -INFINITY ? min(first[1][i], key) : first[1][i];
+          first[2][i] = f != f ? min(first[2][i], key) : first[2][i];
         }
     }
   }
-  for (int r = 0; r < rows; ++r)
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
+  for (int i = 0; i < kMine; ++i) {
+    if (min(first[0][i], min(first[1][i], first[2][i])) >= end) continue;
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
       float sum = dst[r * dst_stride + lane + 32 * i];
       if (first[0][i] <= row + r) sum += INFINITY;
       if (first[1][i] <= row + r) sum -= INFINITY;
       if (first[2][i] <= row + r) sum += __int_as_float(0x7fc00000);
       dst[r * dst_stride + lane + 32 * i] = sum;
     }
+  }
 }
 
 template <int kHd>
