@@ -115,6 +115,8 @@ struct DecodeCfg {
   static constexpr int kTile = kDecodeWarps * kKeys;
   static constexpr int kRow = kHd * (int)sizeof(C), kUnit = kKeys * kRow;  // bytes of a row; of a warp's keys (or values) of a tile
   static constexpr int kParts = !kWideAct ? 1 : kF32 ? 2 : sizeof(C) == 2 && std::is_same<C, __nv_bfloat16>::value ? 3 : 2;
+  // weights meet the values times this: for f16's range, and elsewhere so that values at f32's ends can be summed
+  static constexpr float kWeightTop = std::is_same<C, __half>::value ? 0x1p14f : 0x1p-24f;
   static constexpr int kKs = kF32 ? kHd / 8 : kHd / 16, kMt = kHd / 16;
   static constexpr int kQBytes = kNT * kParts * kKs * 256;             // q in the order of the instruction's operand
   // at the end of an item: a warp's statistics, and three quarters of its sums, for the other warps to join
@@ -160,7 +162,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
                 kMt = Cfg::kMt, kParts = Cfg::kParts, kHeads = Cfg::kHeads;
   constexpr bool kF32 = Cfg::kF32, kF16 = std::is_same<C, __half>::value;
   constexpr float kMost = 3.402823466e38f;
-  constexpr float kWeightTop = 16384.f, kPartStep = 2048.f;
+  constexpr float kWeightTop = Cfg::kWeightTop, kPartStep = 2048.f;
   extern __shared__ __align__(128) uint8_t dec_smem[];
   __shared__ int64_t start_s[3];
   __shared__ int64_t scan_s[kDecodeWarps];
@@ -426,7 +428,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
         f[w][0] = exp2f(st[w].x - ref[0]), f[w][1] = exp2f(st[w].y - ref[1]);
         sum[0] += st[w].z * f[w][0], sum[1] += st[w].w * f[w][1];
       }
-      const float inv[2] = {sum[0] == 0.f ? 0.f : 1.f / sum[0], sum[1] == 0.f ? 0.f : 1.f / sum[1]};
+      const float inv[2] = {sum[0] == 0.f ? 0.f : 1.f / kWeightTop / sum[0], sum[1] == 0.f ? 0.f : 1.f / kWeightTop / sum[1]};
       const float own[2] = {exp2f(m[nt][0] - ref[0]), exp2f(m[nt][1] - ref[1])};
 #pragma unroll
       for (int q = 0; q < kQ; ++q) {
@@ -520,7 +522,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     out_slot = out_slot + 1 == kRing ? 0 : out_slot + 1;
 
     // weights: relative to the running maximum, which moves only when a score passes it by 2^8, so that it is looked for across lanes
-    // rarely; f16 caches: to the largest score of the tile, times 2^14, for f16's range (`take` brings the tile's sums to the maximum)
+    // rarely; f16 caches: to the largest score of the tile, for f16's range (`take` brings the tile's sums to the maximum)
     bool up = false, far = false;
     float x[kSub][kNT][4];
 #pragma unroll
@@ -601,12 +603,9 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           e[j] = exp2_approx(s[sub][nt][j] - ref[j & 1]);
-          if constexpr (kF16) {
-            l[nt][j & 1] = fmaf(e[j], take[nt][j & 1], l[nt][j & 1]);
-            e[j] *= kWeightTop;
-          } else {
-            l[nt][j & 1] += e[j];
-          }
+          if constexpr (kF16) l[nt][j & 1] = fmaf(e[j], take[nt][j & 1], l[nt][j & 1]);
+          else l[nt][j & 1] += e[j];
+          e[j] *= kWeightTop;
         }
         if constexpr (kF32) {
           // this lane wants keys tq, tq + 4, tq + 8, tq + 12 of head g; lane 4 * key + g / 2 has them for keys below 8 in e[g & 1]
@@ -680,7 +679,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
         for (int i = 0; i < 4; ++i) {
           if constexpr (kF16) {
             const float all = kParts > 1 ? fmaf(low[nt][i], 1.f / kPartStep, tile[nt][i]) : tile[nt][i];
-            o[nt][t][i] = fmaf(all, take[nt][i & 1] * (1.f / kWeightTop), o[nt][t][i]);
+            o[nt][t][i] = fmaf(all, take[nt][i & 1], o[nt][t][i]);
           } else {
             o[nt][t][i] += tile[nt][i];
           }
@@ -757,7 +756,7 @@ __global__ void __launch_bounds__(kHd) paged_join_kernel(const DecodeParams p) {
   }
   const int kvh = a.y / p.chunks;
   reinterpret_cast<A*>(p.out)[((int64_t)a.x * p.n_heads + kvh * p.group + part * Cfg::kHeads + h) * kHd + threadIdx.x] =
-      from_f32<A>(sum == 0.f ? 0.f : acc / sum);
+      from_f32<A>(sum == 0.f ? 0.f : acc * (1.f / Cfg::kWeightTop / sum));
 }
 
 }  // namespace fq

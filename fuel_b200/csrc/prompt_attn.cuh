@@ -3,8 +3,8 @@
 //   S = Q K^T,  P = exp2(c S - c m),  O += P V,  out = O / sum(P),   c = scale log2(e)
 //
 // with m a reference that follows the running maximum of the row: it moves only when the maximum has passed it by 2^8, so that
-// O, which stays in tensor memory, is hardly ever rescaled (P then reaches 2^8 at most, in f16, whose weights are 2^7 times larger to
-// keep clear of its lower end, 2^15; sums and products are f32). P is rounded once to the inputs' type: half a step of each weight,
+// O, which stays in tensor memory, is hardly ever rescaled (P then reaches 2^8 at most, times 2^7 in f16, to keep clear of its lower end,
+// and times 2^-24 in bf16, to keep O clear of f32's upper end; sums and products are f32). P is rounded once to the inputs' type: half a step of each weight,
 // in f16 2^-32 of the largest at least. P in two parts would be half as many products again.
 // Bound by the tensor cores and, at head_dim 64 above all, by the 16 exponentials a clock and SM.
 // A persistent thread block per SM takes blocks of 256 query rows of one head, the longest of a sequence first, as two tiles of
@@ -543,8 +543,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
         tc_fence_after();
         const bool last = j + 1 == mine;
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // NaN where a visible score is: then the whole row is
-        // f16 ends at 2^-24: its weights are 2^7 times larger, up to 2^15
-        constexpr float kUp = std::is_same<T, __half>::value ? 7.f : 0.f;
+        // f16 ends at 2^-24: its weights are 2^7 times larger, up to 2^15; bf16's 2^24 times smaller, so that values at f32's ends can be summed
+        constexpr float kUp = std::is_same<T, __half>::value ? 7.f : -24.f;
         uint64_t c2, m2;
         bool far = false;
         // the row's reference, once its maximum is in top[]

@@ -53,6 +53,12 @@ def _attend(q, k, v, scale):
     return p @ v, p @ v.abs()
 
 
+def _near_the_end(shape, seed, dtype):
+    """Values up to 0.95 of the type's largest"""
+    return (torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").clamp(-1.9, 1.9) / 2.0
+            * torch.finfo(dtype).max).to(dtype)
+
+
 def _pages(k, v, page):
     """k and v [n, 1, d] as a paged cache of one sequence, its pages in reverse"""
     n, _, d = k.shape
@@ -284,6 +290,42 @@ def test_prompt_rows_whose_first_keys_score_minus_infinity(act, d):
 
 
 # ---- large values
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("act", [F32, F16, BF16])
+def test_prompt_of_values_at_the_ends_of_their_type(act, d):
+    """Their means are finite, whatever their sums are."""
+    from fuel_b200 import ops
+    n = 700
+    q, k, v = _randn((n, 2, d), 1, act), _randn((n, 1, d), 2, act), _near_the_end((n, 1, d), 3, act)
+    v[::5] = torch.finfo(act).max * 0.9
+    out = ops.prompt_attn(q, k, v, _ints([0, n]))
+    for row in (0, 1, 127, 128, 300, 699):
+        want, mag = _attend(q[row].double(), k[:row + 1, 0].double(), v[:row + 1, 0].double(), d ** -0.5)
+        off = (out[row].double() - want).abs()
+        if act == F32:
+            assert (off.norm() / want.norm()).item() <= 4.1e-6, row
+        else:
+            assert (off <= _HALF[act] * (want.abs() + mag) + 2.0 ** -15 * mag).all(), row
+
+
+@pytest.mark.parametrize("act,cache", _PAIRS)
+def test_decode_of_values_at_the_ends_of_their_type(act, cache):
+    """One row in one block's run and one that is joined from several."""
+    from fuel_b200 import ops
+    n, h, d = 3000, 3, 128
+    q, k, v = _randn((2, h, d), 1, act), _randn((n, 1, d), 2, cache), _near_the_end((n, 1, d), 3, cache)
+    v[::5] = torch.finfo(cache).max * 0.9
+    kc, vc, table = _pages(k, v, 16)
+    out = ops.paged_attn_decode(q, kc, vc, table.repeat(2, 1), _ints([n, 5]))
+    for s, m in ((0, n), (1, 5)):
+        want, mag = _attend(q[s].double(), k[:m, 0].double(), v[:m, 0].double(), d ** -0.5)
+        off = (out[s].double() - want).abs()
+        if act == F32:
+            assert (off.norm() / want.norm()).item() <= 4.1e-6, s
+        else:
+            assert (off <= _HALF[act] * (want.abs() + mag) + 2.0 ** -15 * mag).all(), s
+
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("gap", [-30.0, 0.0, 10.0, 14.0])
