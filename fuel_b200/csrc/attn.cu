@@ -79,8 +79,8 @@ int32_t launch_decode(DecodeParams& p, cudaStream_t stream) {
   const int blocks = sms * Cfg::kPerSm < kDecodeMaxBlocks ? sms * Cfg::kPerSm : kDecodeMaxBlocks;
   cudaError_t e = launch(kernel, dim3((unsigned)blocks), dim3(32 * kDecodeWarps), Cfg::kSmem, stream, p);
   if (e == cudaSuccess)
-    e = launch(paged_join_kernel<A, C, kHd, kNT>, dim3((unsigned)blocks, (unsigned)(p.group < Cfg::kHeads ? p.group : Cfg::kHeads)), dim3(kHd), 0,
-               stream, p);
+    e = launch(paged_join_kernel<A, C, kHd, kNT>, dim3((unsigned)blocks, (unsigned)(p.group < Cfg::kHeads ? p.group : Cfg::kHeads)),
+               dim3(kHd), 0, stream, p);
   return e == cudaSuccess ? kOk : kLaunchFailure;
 }
 
@@ -220,14 +220,15 @@ int32_t fuelq_paged_append(int32_t act_type, int32_t cache_type, const void* k, 
   if (q && (n_heads <= 0 || n_heads % n_kv)) return kInvalidProblem;
   if (n_rows == 0) return kOk;
   // a cache without pages, a table without columns, angles of no positions: nothing is read of them
-  if (!k || !v || (n_pages && (!kcache || !vcache)) || (max_pages && n_seqs && !page_table) || !positions || (max_pos && (!cos_table || !sin_table)) ||
-      (q && !q_out))
+  if (!k || !v || !positions || (q && !q_out) || (n_pages && (!kcache || !vcache)) || (max_pages && n_seqs && !page_table) ||
+      (max_pos && (!cos_table || !sin_table)))
     return kInvalidProblem;
   if (!stride_ok(k_stride, n_kv, head_dim, act_type) || !stride_ok(v_stride, n_kv, head_dim, act_type)) return kInvalidProblem;
   if (q && !stride_ok(q_stride, n_heads, head_dim, act_type)) return kInvalidProblem;
   if (!seq_ids && n_rows > n_seqs) return kInvalidProblem;
   // in place only where a row is written where it was read
-  if ((q && q_out == q && q_stride != (int64_t)n_heads * head_dim) || (k_out == k && k_stride != (int64_t)n_kv * head_dim)) return kInvalidProblem;
+  if ((q && q_out == q && q_stride != (int64_t)n_heads * head_dim) || (k_out == k && k_stride != (int64_t)n_kv * head_dim))
+    return kInvalidProblem;
   if (!aligned16(k) || !aligned16(v) || !aligned16(kcache) || !aligned16(vcache) || !aligned16(cos_table) || !aligned16(sin_table) ||
       (q && (!aligned16(q) || !aligned16(q_out))) || !aligned16(k_out))
     return kMisaligned;
@@ -263,7 +264,8 @@ int32_t fuelq_paged_attn_decode(int32_t act_type, int32_t cache_type, const void
   if (!type_pair(act_type, cache_type) || (head_dim != 64 && head_dim != 128)) return kNotSupported;
   const int shift = page_shift_of(page_size);
   if (shift < 0) return kNotSupported;
-  if (n_seqs < 0 || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !scale_ok(scale) || n_pages < 0 || max_pages < 0) return kInvalidProblem;
+  if (n_seqs < 0 || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !scale_ok(scale) || n_pages < 0 || max_pages < 0)
+    return kInvalidProblem;
   if (n_seqs == 0) return kOk;
   if (!q || (n_pages && (!kcache || !vcache)) || !out || (max_pages && !page_table) || !seq_lens) return kInvalidProblem;
   if (!stride_ok(q_stride, n_heads, head_dim, act_type)) return kInvalidProblem;
@@ -296,7 +298,9 @@ int32_t fuelq_prompt_attn(int32_t act_type, const void* q, int64_t q_stride, con
                           int32_t n_heads, int32_t n_kv, int32_t head_dim, float scale, void* workspace,
                           size_t workspace_bytes, void* stream) {
   if (!type_bytes(act_type) || (head_dim != 64 && head_dim != 128)) return kNotSupported;
-  if (n_seqs < 0 || n_rows < 0 || n_rows > kMaxPromptRows || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv || !scale_ok(scale)) return kInvalidProblem;
+  if (n_seqs < 0 || n_rows < 0 || n_rows > kMaxPromptRows || n_kv <= 0 || n_heads <= 0 || n_heads > kMaxHeads || n_heads % n_kv ||
+      !scale_ok(scale))
+    return kInvalidProblem;
   if ((int64_t)n_seqs * n_heads > kMaxSlots) return kNotSupported;
   if (n_seqs == 0 || n_rows == 0) return kOk;
   if (!q || !k || !v || !out || !cu_seqlens) return kInvalidProblem;

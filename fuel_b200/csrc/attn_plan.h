@@ -27,7 +27,9 @@ FQ_HD int seq_keys(int len, int max_pages, int page_shift) {
   const int64_t room = (int64_t)max_pages << page_shift;
   return len < 0 ? 0 : len > room ? (int)room : len;
 }
-FQ_HD int seq_tiles(int len, int max_pages, int page_shift, int tile) { return (int)(((int64_t)seq_keys(len, max_pages, page_shift) + tile - 1) / tile); }
+FQ_HD int seq_tiles(int len, int max_pages, int page_shift, int tile) {
+  return (int)(((int64_t)seq_keys(len, max_pages, page_shift) + tile - 1) / tile);
+}
 
 FQ_HD int item_units(int tiles) { return tiles ? tiles + kItemUnits : 0; }
 // places of one kv head of sequences [from, to): more than 32 bits count where long sequences share their pages

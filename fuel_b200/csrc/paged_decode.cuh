@@ -18,11 +18,14 @@
 // Work: tiles of kTile keys of all (sequence, kv head) items, laid end to end and dealt out evenly (attn_plan.h), so that one
 // long sequence, many short ones and any mixture fill the device alike. A warp owns 16 (head_dim 64: 32) keys of each
 // tile and runs by itself: its own ring of cp.async copies that runs on across items, its own running maximum and sums; the
-// block's four warps join their results in shared memory at the end of an item, a quarter of the columns each, pieces of an item in other blocks by
-// paged_join_kernel in a fixed order.
-// Measured: 100003 keys, 32/8 heads of 128, f16 cache, f32 activations 70 to 79 us by card (5.2 to 5.8 TB/s); 64 sequences up to 8192, bf16, 91 to 95
-// us (5.6 to 5.8 TB/s); 256 up to 2047, 32/4 heads of 64, f16, 36 to 38 us (3.7 to 3.9 TB/s: two or three short items a block, whose beginnings and
-// ends are latency; without places for them in the split 64 us); 513 keys, 32 heads, f32, 15 us, nearly all latency.
+// block's four warps join their results in shared memory at the end of an item, a quarter of the columns each, pieces of an item
+// in other blocks by paged_join_kernel in a fixed order.
+// Measured: 100003 keys, 32/8 heads of 128, f32 activations over f16 71 to 79 us by card (5.2 to 5.8 TB/s), over bf16 75; 64 sequences
+// up to 8192, bf16, 91 to 94 us (5.6 to 5.8 TB/s); 32 of 2000, f32 98 us; 256 up to 2047, 32/4 heads of 64, f16, 37 to 39 us (3.6 to
+// 3.8 TB/s: two or three short items a block, whose beginnings and ends are latency; without places for them in the split 64 us);
+// 64 of 2000, 32/2 heads of 128, bf16 36 us; 513 keys, 32 heads, f32, 15 us: one tile a block, its join and the second launch.
+// Weights of 16-bit activations in two parts would leave only the result's own rounding (bf16 2.2e-3 -> 1.7e-3 of the result): 256
+// sequences 36.8 -> 38.8 us, 64 of 2000 with 16 heads a kv head 36.2 -> 38.0.
 #pragma once
 #include <type_traits>
 
@@ -52,10 +55,12 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int kPending>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   uint32_t d;
@@ -95,7 +100,8 @@ __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
 // or zero is not; so a result that is not finite while the sum of its weights is is looked up again here. (Only then: an infinity in
 // the cache costs its batch time, finite ones nothing.)
 template <typename C>
-__device__ __noinline__ float sum_not_finite(const C* column, const int* pages, int from, int to, int page_shift, int n_pages, int64_t page_stride, int row_stride) {
+__device__ __noinline__ float sum_not_finite(const C* column, const int* pages, int from, int to, int page_shift, int n_pages,
+                                             int64_t page_stride, int row_stride) {
   float sum = 0.f;
 #pragma unroll 4
   for (int key = from; key < to; ++key) {
@@ -275,7 +281,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     values_due = get.x < x1;
     if (values_due) {
       const int key = get.tile * Cfg::kTile + warp * kKeys + (lane & (kKeys - 1));
-      place = next_page < 0 ? -1 : (((int64_t)next_page * p.n_kv + get.chunk / p.chunks) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
+      place = next_page < 0 ? -1
+                            : (((int64_t)next_page * p.n_kv + get.chunk / p.chunks) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
       const uint32_t seen = __ballot_sync(0xffffffffu, place >= 0);
       if (lane == 0) seen_s[fetched & 7] = seen;
       ++fetched;
@@ -399,7 +406,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
 #pragma unroll
       for (int t = 0; t < kMt; ++t) {
         const int to = t / kQ, from = warp - (warp > to ? 1 : 0);
-        if (to != warp) box[(((to * 3 + from) * kNT + nt) * kQ + t % kQ) * 32] = make_float4(o[nt][t][0], o[nt][t][1], o[nt][t][2], o[nt][t][3]);
+        const float(&x)[4] = o[nt][t];
+        if (to != warp) box[(((to * 3 + from) * kNT + nt) * kQ + t % kQ) * 32] = make_float4(x[0], x[1], x[2], x[3]);
       }
     }
     __syncthreads();
@@ -409,9 +417,10 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     A* dst = reinterpret_cast<A*>(p.out) + ((int64_t)at.seq * p.n_heads + kvh * p.group + part * kHeads) * kHd;
     const int64_t page_stride = (int64_t)p.n_kv * kHd << p.page_shift;
     auto look_again = [&](int d) {  // at column d of the piece's keys
-      const int from = (int)max(x0 - item_first, (int64_t)0) * Cfg::kTile, to = (int)min((int64_t)(at.tile + 1) * Cfg::kTile, (int64_t)at.keys);
-      return sum_not_finite(reinterpret_cast<const C*>(p.v) + ((int64_t)kvh * kHd << p.page_shift) + d, p.table + (int64_t)at.seq * p.max_pages,
-                            from, to, p.page_shift, p.n_pages, page_stride, kHd);
+      const int from = (int)max(x0 - item_first, (int64_t)0) * Cfg::kTile;
+      const int to = (int)min((int64_t)(at.tile + 1) * Cfg::kTile, (int64_t)at.keys);
+      return sum_not_finite(reinterpret_cast<const C*>(p.v) + ((int64_t)kvh * kHd << p.page_shift) + d,
+                            p.table + (int64_t)at.seq * p.max_pages, from, to, p.page_shift, p.n_pages, page_stride, kHd);
     };
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
@@ -459,13 +468,17 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
       }
       if (!whole && warp == 0 && g == 0) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) slot[kHeads * kHd + nt * 8 + 2 * tq + j] = top[j], slot[kHeads * (kHd + 1) + nt * 8 + 2 * tq + j] = sum[j];
+        for (int j = 0; j < 2; ++j) {
+          const int h = nt * 8 + 2 * tq + j;
+          slot[kHeads * kHd + h] = top[j], slot[kHeads * (kHd + 1) + h] = sum[j];
+        }
       }
     }
     if (last && threadIdx.x == 0) {  // the end of this block's run: does an item go on from here that began here?
       const bool first_piece = !done && item_first >= x0;
       p.meta[2 * blockIdx.x] = make_int4(first_piece ? at.seq : -1, at.chunk, at.tiles, blocks);
-      p.meta[2 * blockIdx.x + 1] = make_int4((int)(item_first & 0xffffffff), (int)(item_first >> 32), (int)(total & 0xffffffff), (int)(total >> 32));
+      p.meta[2 * blockIdx.x + 1] =
+          make_int4((int)(item_first & 0xffffffff), (int)(item_first >> 32), (int)(total & 0xffffffff), (int)(total >> 32));
     }
     __syncthreads();
   };
@@ -651,7 +664,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int key = sub * 16 + 8 * half + tq + 4 * (j >> 1), d = 16 * t + g + 8 * (j & 1);
-              const uint32_t x = *reinterpret_cast<const uint32_t*>(vunit + key * kRow + (((d >> 2) ^ ((key & 3) << 1)) * 16) + (d & 3) * 4);
+              const uint8_t* at = vunit + key * kRow + (((d >> 2) ^ ((key & 3) << 1)) * 16) + (d & 3) * 4;
+              const uint32_t x = *reinterpret_cast<const uint32_t*>(at);
               split_tf32(x, hi[j], lo[j]);
             }
 #pragma unroll
@@ -720,7 +734,8 @@ __global__ void __launch_bounds__(kHd) paged_join_kernel(const DecodeParams p) {
   const int part = a.y % p.chunks, h = blockIdx.y;
   if (h >= min(Cfg::kHeads, p.group - part * Cfg::kHeads)) return;
   const int4 b = p.meta[2 * blockIdx.x + 1];
-  const int64_t first = (int64_t)(((uint64_t)(uint32_t)b.y << 32) | (uint32_t)b.x), total = (int64_t)(((uint64_t)(uint32_t)b.w << 32) | (uint32_t)b.z);
+  const int64_t first = (int64_t)(((uint64_t)(uint32_t)b.y << 32) | (uint32_t)b.x);
+  const int64_t total = (int64_t)(((uint64_t)(uint32_t)b.w << 32) | (uint32_t)b.z);
   const int blocks = a.w, b0 = blockIdx.x, n = split_block(total, blocks, first + a.z - 1) - b0 + 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // pieces behind the first begin with their blocks' runs: slot 2 b

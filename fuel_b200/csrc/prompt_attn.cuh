@@ -4,8 +4,8 @@
 //
 // with m a reference that follows the running maximum of the row: it moves only when the maximum has passed it by 2^8, so that
 // O, which stays in tensor memory, is hardly ever rescaled (P then reaches 2^8 at most, times 2^7 in f16, to keep clear of its lower end,
-// and times 2^-24 in bf16, to keep O clear of f32's upper end; sums and products are f32). P is rounded once to the inputs' type: half a step of each weight,
-// in f16 2^-32 of the largest at least. P in two parts would be half as many products again.
+// and times 2^-24 in bf16, to keep O clear of f32's upper end; sums and products are f32). P is rounded once to the inputs' type: half a
+// step of each weight, in f16 2^-32 of the largest at least. P in two parts would be half as many products again.
 // Bound by the tensor cores and, at head_dim 64 above all, by the 16 exponentials a clock and SM.
 // A persistent thread block per SM takes blocks of 256 query rows of one head, the longest of a sequence first, as two tiles of
 // 128 rows that take turns: while the tensor cores multiply for one tile, the other one's softmax runs.
@@ -18,10 +18,12 @@
 // Keys behind a row: the scores of the last key tile are masked. A value of NaN or infinity there would still reach earlier rows
 // as 0 x NaN, so the softmax warps take such values out of the last tile in shared memory and add them to the rows they
 // belong to at the end. Rows of the next sequence, or of nobody, that the last tile touches are taken out the same way.
-// Measured, 32/8 heads of 128: one prompt of 16384 tokens, f16, 1.87 to 2.26 ms by card (970 to 1175 TFLOP/s of the scores that are seen, the
-// card under its power limit), 4096 tokens 158 us; 24 prompts up to 2048, bf16, 326 to 337 us (522 to 539). A row tile's softmax (ld 250,
-// maximum 450, exponentials 1370 cycles) and its own products (1380 from the last weight to the next scores) follow one
-// another, so with two tiles in turn the tensor cores wait a quarter of the time; tensor memory has no room for a third.
+// Measured, 32/8 heads of 128: one prompt of 16384 tokens, f16, 1.90 to 2.26 ms by card (970 to 1160 TFLOP/s of the scores that are
+// seen, the card under its power limit), 4096 tokens 160 us; 24 prompts up to 2048, bf16, 331 to 343 us (513 to 532). A row tile's
+// softmax (ld 250, maximum 450, exponentials 1370 cycles) and its own products (1380 from the last weight to the next scores) follow
+// one another, so with two tiles in turn the tensor cores wait a quarter of the time. Tensor memory has no room for a third; the
+// products could begin on half of the weights, which is not done. Blocks of rows are dealt round the thread blocks whatever they
+// cost: in the 24 prompts the fullest has 157 key tiles and item ends where the average is 115, in one prompt of 4096 80 of 62.
 #pragma once
 #include <type_traits>
 
@@ -39,7 +41,8 @@ struct PromptParams {
   float c;
 };
 constexpr int kPaThreads = 384, kPaTile = 128, kPaRows = 2 * kPaTile;
-// registers of a softmax thread (its row of S is 128 of them) and of the others: 256 x 208 + 128 x 80 of the launch's 384 x 168
+// registers of a softmax thread (its row of S is 128 of them) and of the others: 256 x 208 + 128 x 80 of the launch's 384 x 168. (The
+// form for heads of 64 keeps 56 to 64 bytes of a thread on its stack all the same, that for 128 nothing)
 constexpr int kPaSoftmaxRegs = 208, kPaOtherRegs = 80;
 
 // ---- PTX wrappers
@@ -136,17 +139,18 @@ __device__ __forceinline__ void tmem_wait_ld8(uint32_t (&r)[8]) {
                : "memory");
 }
 __device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%4], {%0,%1,%2,%3};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(taddr) : "memory");
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%4], {%0,%1,%2,%3};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(taddr)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-               "r"(r[15]), "r"(taddr)
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+               "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
                : "memory");
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
-               "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
                : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -295,7 +299,8 @@ struct ItemRing {
   PromptItem item[kItemRing];
 };
 // The next item from x on (in steps of the grid) whose block has rows; the whole warp looks
-__device__ __forceinline__ PromptItem find_item(const int* cu, int n_seqs, int64_t n_rows, int n_heads, int64_t n_items, int rows, int64_t& x, int lane) {
+__device__ __forceinline__ PromptItem find_item(const int* cu, int n_seqs, int64_t n_rows, int n_heads, int64_t n_items, int rows,
+                                                int64_t& x, int lane) {
   PromptItem it;
   for (; x < n_items; x += gridDim.x) {
     const int64_t slot = x / n_heads;
@@ -470,7 +475,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
     for (uint32_t items = 0; ok && get_item<true>(ctl->items, items, it, wait); ++items) {
       const int n1 = second_tiles(it), n = n1 ? n1 : it.n, nt[2] = {it.n, n1};
       auto stage = [&](int j, bool value) { return (unit + 2 * j + value) % kStages; };
-      auto kv_ready = [&](int j, bool value) { return ready(&ctl->kv_full[stage(j, value)], (unit + 2 * j + value) / kStages, kErrFullWait); };
+      auto kv_ready = [&](int j, bool value) {
+        return ready(&ctl->kv_full[stage(j, value)], (unit + 2 * j + value) / kStages, kErrFullWait);
+      };
       auto scores = [&](int t, int j) {
         const uint64_t a = q_desc + (uint64_t)(t * kTileBytes >> 4), b = k_desc + (uint64_t)(stage(j, false) * kTileBytes >> 4);
         if (leader) {
@@ -543,7 +550,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
         tc_fence_after();
         const bool last = j + 1 == mine;
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // NaN where a visible score is: then the whole row is
-        // f16 ends at 2^-24: its weights are 2^7 times larger, up to 2^15; bf16's 2^24 times smaller, so that values at f32's ends can be summed
+        // f16 ends at 2^-24: its weights are 2^7 times larger, up to 2^15; bf16's 2^24 times smaller, so that values at f32's ends can be
+        // summed
         constexpr float kUp = std::is_same<T, __half>::value ? 7.f : -24.f;
         uint64_t c2, m2;
         bool far = false;
@@ -601,7 +609,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
 #pragma unroll
           for (int i = 0; i < 4; ++i) tmem_wait_ld(s + 32 * i);
 #pragma unroll
-          for (int i = 0; i < kPaTile; i += 2) top[(i >> 1) & 3] = max3_nan(top[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+          for (int i = 0; i < kPaTile; i += 2)
+            top[(i >> 1) & 3] = max3_nan(top[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
           refer();
           uint32_t w[kPaTile / 2];
 #pragma unroll
@@ -623,7 +632,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
             for (int i = 0; i < 32; ++i)
               if (i > seen) s[i] = 0xff800000u;
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) top[(i >> 1) & 3] = max3_nan(top[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+            for (int i = 0; i < 32; i += 2)
+              top[(i >> 1) & 3] = max3_nan(top[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
           }
           refer();
           uint32_t s[2][16];
@@ -637,7 +647,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
               if (c < 7) tmem_ld16_nowait(s_addr + 16 * (c + 1), s[h ^ 1]);
               uint32_t w[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) w[i] = weight2(i, 2 * i > seen ? 0xff800000u : s[h][2 * i], 2 * i + 1 > seen ? 0xff800000u : s[h][2 * i + 1]);
+              for (int i = 0; i < 8; ++i)
+                w[i] = weight2(i, 2 * i > seen ? 0xff800000u : s[h][2 * i], 2 * i + 1 > seen ? 0xff800000u : s[h][2 * i + 1]);
               tmem_st8(s_addr + 8 * c, w);  // over scores that have been read: in front of the ones in flight
             }
           }
@@ -658,7 +669,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
           const bool found = (odd & 0x80008000u) != 0;
           // the record may still be read for the item before: by a slower warp of this tile, and tile 0's by tile 1, whose last item may
           // lie further back
-          if (found && (t || !done || wait(&ctl->taken_free[0], done - 1, kErrMmaWait)) && (!done1 || wait(&ctl->taken_free[1], done1 - 1, kErrMmaWait))) {
+          if (found && (t || !done || wait(&ctl->taken_free[0], done - 1, kErrMmaWait)) &&
+              (!done1 || wait(&ctl->taken_free[1], done1 - 1, kErrMmaWait))) {
 #pragma unroll 1
             for (int i = 0; i < kTileBytes / 16 / 128; ++i) {
               const int at = (i * 128 + r) * 16, box = at / kBoxBytes, key = (at % kBoxBytes) / 128, chunk = ((at % 128) / 16) ^ (key & 7);

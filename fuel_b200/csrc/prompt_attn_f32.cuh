@@ -7,12 +7,12 @@
 //   v      one for each row and head, put into the weight: with f_j the row's power, w_ij = 2^(s_ij + f_j - m_i), m the maximum of
 //          s + f in the key tile, so that w V' has f16's range whatever the rows' magnitudes. sum_j w_ij 2^-f_j is the softmax's
 //          sum in the same unit as O = sum_j w_ij V'_j, so the result is their quotient
-// A score is added to a whole power there, which loses nothing while the score is below 2^23 or so, and scores at f32's ends leave it. Rows
-// whose largest is beyond 2^22 (in units of the exponent) are computed once more at the end, with sums in 64 bits (weigh_again).
-// So do rows that see values of more than 2^100 apart, whose sums would need more than f32's range. The powers of v stay above 2^-80 and,
-// in a tile, within 2^100 of the largest before them: no row loses bits to a larger one behind it. prompt_split_kernel writes the parts and powers (bound by HBM: 4 bytes in,
-// 4 out); values that are not finite are taken out of v there, and the tiles that had some are marked: the few rows that see
-// one add it again from the original at the end.
+// A score is added to a whole power there, which loses nothing while the score is below 2^23 or so, and scores at f32's ends leave it.
+// Rows whose largest is beyond 2^22 (in units of the exponent) are computed once more at the end, with sums in 64 bits
+// (weigh_again), and so are rows that see values of more than 2^100 apart, whose sums would need more than f32's range. The powers
+// of v stay above 2^-80 and, in a tile, within 2^100 of the largest before them: no row loses bits to a larger one behind it.
+// prompt_split_kernel writes the parts and powers (bound by HBM: 4 bytes in, 4 out); values that are not finite are taken out of v
+// there, and the tiles that had some are marked: the few rows that see one add it again from the original at the end.
 // The tensor cores' f32 sums round towards zero, which over a long row adds up (1.6e-5 of it at 4000 keys). So they sum one
 // key tile at a time, and the tiles' results are added in registers, rounded to nearest, each with its maximum: the softmax of a
 // tile needs nothing from the tile before, and two warpgroups take the tiles in turn.
@@ -25,8 +25,9 @@
 //   warps 12, 15    copies: the parts of Q and K, of V
 //   warp 13         issues the MMAs
 //   warp 14         finds the block's items and brings the powers of each key tile
-// Measured, 32/8 heads of 128: 512 tokens 39 us (the split 8 of them), 4096 tokens 524 us: 262 TFLOP/s of the scores that are seen,
-// 787 of f16 products. An issuing warp that waits for ten units and flags a key tile bounds it now, some 300 cycles each.
+// Measured, 32/8 heads of 128: 512 tokens 35.5 us (the split some 8 of them), 4096 tokens 528 us: 260 TFLOP/s of the scores that are
+// seen, 780 of f16 products; heads of 64 410 us. An issuing warp that waits for ten units and flags a key tile bounds it now, some 300
+// cycles each. Of 4096 rows of four heads, 125 us, one infinite column of the values makes 0.37 ms, scores beyond 2^22 in every row 21 ms.
 #pragma once
 #include "prompt_attn.cuh"
 
@@ -44,8 +45,8 @@ struct PromptF32Params {
   __half *qp, *kp, *vp;  // parts: [2][n_rows][heads][hd]
   float* q_up;           // [heads][n_rows]    c 2^eq
   float2* kv_up;         // [n_kv][n_rows]     2^ek, f
-  int2* marked;          // [n_kv][n_rows]     at the first row of a tile: does it hold a value that is not finite (bit 0), 128 + its largest
-                         //                    f (bits 8 to 15) and its least (16 to 23); its largest ek
+  int2* marked;          // [n_kv][n_rows]     at the first row of a tile: does it hold a value that is not finite (bit 0), 128 + its
+                         //                    largest f (bits 8 to 15) and its least (16 to 23); its largest ek
 };
 
 // one tile of 128 rows of one head; 64 registers, so that two blocks an SM have 64 KB each in flight (512 rows, 96 heads: one block of 256
@@ -162,6 +163,8 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) prompt_split_kernel(const
 
 constexpr int kPfaThreads = 512;
 // registers of a softmax thread, of one that holds a row of O, of the others: 128 x (2 x 120 + 192 + 80) of the launch's 512 x 128
+// (heads of 128: 8 bytes of a thread on its stack). Functions that are not inlined are called by the second kind alone: what they may
+// use is what the launch has
 constexpr int kPfaSoftmaxRegs = 120, kPfaSumRegs = 192, kPfaOtherRegs = 80;
 constexpr int kPfaAhead = 4;  // key tiles that the softmax may be ahead of the sums (two, for the tensor memory), and their own
 
@@ -210,8 +213,9 @@ __device__ __noinline__ bool sees_far_apart(const float2* up, int row0, int len,
 // (the queries themselves may lie under the result); k, v: of the sequence's first; row: the first's number; up: c 2^eq of the
 // lane's row
 template <int kHd>
-__device__ __noinline__ void weigh_again(const __half* q, int64_t q_stride, int64_t parts, float up, const float* k, int64_t k_stride, const float* v,
-                                         int64_t v_stride, int row, uint32_t which, float* dst, int64_t dst_stride, int lane) {
+__device__ __noinline__ void weigh_again(const __half* q, int64_t q_stride, int64_t parts, float up, const float* k, int64_t k_stride,
+                                         const float* v, int64_t v_stride, int row, uint32_t which, float* dst, int64_t dst_stride,
+                                         int lane) {
   constexpr int kMine = kHd / 32, kKeys = 4;
   for (; which; which &= which - 1) {
     const int r = __ffs(which) - 1;
@@ -269,7 +273,8 @@ __device__ __noinline__ void weigh_again(const __half* q, int64_t q_stride, int6
 // sequence's first row; marked: the marks of its tiles; row: the warp's first; dst: its result. (By value: a reference to the
 // kernel's parameters would put all of them on every thread's stack)
 template <int kHd>
-__device__ __noinline__ void add_not_finite(const float* v, int64_t v_stride, const int2* marked, int row, int rows, float* dst, int64_t dst_stride, int lane) {
+__device__ __noinline__ void add_not_finite(const float* v, int64_t v_stride, const int2* marked, int row, int rows, float* dst,
+                                            int64_t dst_stride, int lane) {
   constexpr int kMine = kHd / 32, kNone = 0x7fffffff;
   int first[3][kMine];
 #pragma unroll
@@ -321,7 +326,10 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(&ctl->q_full, 1), mbar_init(&ctl->q_empty, 1), mbar_init(&ctl->pv_full, 1), mbar_init(&ctl->pv_empty, 128);
-    for (int i = 0; i < 2; ++i) mbar_init(&ctl->s_full[i], 1), mbar_init(&ctl->p_full[i], 128), mbar_init(&ctl->up_full[i], 1), mbar_init(&ctl->up_empty[i], 128);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl->s_full[i], 1), mbar_init(&ctl->p_full[i], 128);
+      mbar_init(&ctl->up_full[i], 1), mbar_init(&ctl->up_empty[i], 128);
+    }
     for (int s = 0; s < kItemRing; ++s) mbar_init(&ctl->items.full[s], 1), mbar_init(&ctl->items.empty[s], 16);  // every warp
     for (int s = 0; s < kPfaRing; ++s) {
       mbar_init(&ctl->k_full[s], 1), mbar_init(&ctl->k_empty[s], 1);
@@ -366,7 +374,8 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
           mbar_arrive_expect_tx(&ctl->q_full, 2 * kTileBytes);
           for (int part = 0; part < 2; ++part)
             for (int b = 0; b < kUnits; ++b)
-              tma_load_3d(q_addr + part * kTileBytes + b * kUnitBytes, &qmap, 64 * b, it.head, (int)(part * p.n_rows + it.first + it.row), &ctl->q_full);
+              tma_load_3d(q_addr + part * kTileBytes + b * kUnitBytes, &qmap, 64 * b, it.head, (int)(part * p.n_rows + it.first + it.row),
+                          &ctl->q_full);
         }
         for (int j = 0; j < it.n && ok && !*abort_flag; ++j)
           for (int u = 0; u < 2 * kUnits && ok; ++u, ++unit) {
@@ -409,7 +418,8 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
           const int piece = u % kUnits;
           const uint32_t n = (steps + j) * 2 * kUnits + (u < 2 * kUnits ? u : u - kUnits), st = n % kPfaRing;
           if (u < 2 * kUnits && !ready(&ctl->k_full[st], n / kPfaRing, kErrFullWait)) return false;
-          const uint64_t a = q_desc + (uint64_t)(((u / kUnits == 1 ? kTileBytes : 0) + piece * kUnitBytes) >> 4), b = k_desc + (uint64_t)(st * kUnitBytes >> 4);
+          const uint64_t a = q_desc + (uint64_t)(((u / kUnits == 1 ? kTileBytes : 0) + piece * kUnitBytes) >> 4);
+          const uint64_t b = k_desc + (uint64_t)(st * kUnitBytes >> 4);
           if (leader) {
             tc_fence_after();
 #pragma unroll
@@ -542,7 +552,8 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
               for (int i = 0; i < 8; i += 2) {
                 const float4 w = lds_f4(up + (4 * c + i / 2) * 16);
                 float a, b;
-                unpair(fma2(pair(__uint_as_float(s[h][i]), __uint_as_float(s[h][i + 1])), mul2(pair(w.x, w.y), cq2), add2(pair(w.z, w.w), rr2)), a, b);
+                const uint64_t s2 = pair(__uint_as_float(s[h][i]), __uint_as_float(s[h][i + 1]));
+                unpair(fma2(s2, mul2(pair(w.x, w.y), cq2), add2(pair(w.z, w.w), rr2)), a, b);
                 if (decltype(masked)::value && i > seen) a = -INFINITY;
                 if (decltype(masked)::value && i + 1 > seen) b = -INFINITY;
                 a = exp2_approx(a), b = exp2_approx(b);
@@ -574,7 +585,8 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
             if (!(ok = __all_sync(0xffffffffu, wait(&ctl->v_full[st], n / kPfaRing, kErrFullWait)))) break;
             uint8_t* v = v_ring + st * kUnitBytes;
             for (int i = max(from - (u % kUnits) * kUnitKeys, 0) * 8 + r; i < kUnitKeys * 8; i += 128)
-              for (int box = 0; box < kHd / 64; ++box) *reinterpret_cast<uint4*>(v + box * kUnitKeys * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+              for (int box = 0; box < kHd / 64; ++box)
+                *reinterpret_cast<uint4*>(v + box * kUnitKeys * 128 + i * 16) = make_uint4(0, 0, 0, 0);
           }
           if (!ok) break;
           fence_proxy_async();
@@ -628,12 +640,14 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
       }
       odd = __any_sync(0xffffffffu, odd);
       up = __reduce_max_sync(0xffffffffu, up);
-      // rows to be computed again: their maximum is beyond 2^22 or has left f32, where the powers of their factors allow it (a product of two
-      // parts is below 2^37; otherwise an infinity in q or k has made it); the powers' product may leave f32 where the score itself is
-      // of any size; the values lie too far apart
-      const float q_up = row < it.len ? p.q_up[(int64_t)it.head * p.n_rows + it.first + row] : 0.f, reach = q_up * exp2f((float)up);
+      // rows to be computed again: their maximum is beyond 2^22 or has left f32, where the powers of their factors allow it (a product of
+      // two parts is below 2^37; otherwise an infinity in q or k has made it); the powers' product may leave f32 where the score
+      // itself is of any size; the values lie too far apart
+      const float q_up = row < it.len ? p.q_up[(int64_t)it.head * p.n_rows + it.first + row] : 0.f;
+      const float reach = q_up * exp2f((float)up);
       bool far = (reach > 0x1p-15f && !(fabsf(ref) <= 0x1p22f)) || !(reach <= 0x1p120f);
-      if (__reduce_max_sync(0xffffffffu, above) - __reduce_min_sync(0xffffffffu, below) > 100) far |= sees_far_apart(p.kv_up + rows_at, row0, it.len, lane);
+      if (__reduce_max_sync(0xffffffffu, above) - __reduce_min_sync(0xffffffffu, below) > 100)
+        far |= sees_far_apart(p.kv_up + rows_at, row0, it.len, lane);
       const uint32_t again = __ballot_sync(0xffffffffu, far && row < it.len);
       float* dst = p.out + ((it.first + row0) * p.n_heads + it.head) * kHd;
 #pragma unroll
@@ -642,22 +656,24 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
         float* w = reinterpret_cast<float*>(v);
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e] = o[16 * i + e] * inv;
-        store_rows64(smem_u32(stages) + (warp & 3) * kStageBytes, lane, v, reinterpret_cast<uint8_t*>(dst + 16 * i), (int64_t)p.n_heads * kHd * 4, it.len - row0);
+        store_rows64(smem_u32(stages) + (warp & 3) * kStageBytes, lane, v, reinterpret_cast<uint8_t*>(dst + 16 * i),
+                     (int64_t)p.n_heads * kHd * 4, it.len - row0);
       }
       if (again) {
         ctl->busy[warp & 3] = 1;
         __syncwarp();  // the rows are written
         const int kvh = it.head / p.group;
-        weigh_again<kHd>(p.qp + ((it.first + row0) * p.n_heads + it.head) * kHd, (int64_t)p.n_heads * kHd, p.n_rows * p.n_heads * kHd, q_up, p.k + it.first * p.k_stride + kvh * kHd, p.k_stride,
-                         p.v + it.first * p.v_stride + kvh * kHd, p.v_stride, row0, again, dst, (int64_t)p.n_heads * kHd, lane);
+        weigh_again<kHd>(p.qp + ((it.first + row0) * p.n_heads + it.head) * kHd, (int64_t)p.n_heads * kHd, p.n_rows * p.n_heads * kHd, q_up,
+                         p.k + it.first * p.k_stride + kvh * kHd, p.k_stride, p.v + it.first * p.v_stride + kvh * kHd, p.v_stride, row0,
+                         again, dst, (int64_t)p.n_heads * kHd, lane);
         __syncwarp();
         ctl->busy[warp & 3] = 0;
       }
       if (odd && row0 < it.len) {
         ctl->busy[warp & 3] = 1;
         __syncwarp();  // the rows are written
-        add_not_finite<kHd>(p.v + it.first * p.v_stride + (it.head / p.group) * kHd, p.v_stride, p.marked + rows_at, row0, min(32, it.len - row0), dst,
-                            (int64_t)p.n_heads * kHd, lane);
+        add_not_finite<kHd>(p.v + it.first * p.v_stride + (it.head / p.group) * kHd, p.v_stride, p.marked + rows_at, row0,
+                            min(32, it.len - row0), dst, (int64_t)p.n_heads * kHd, lane);
         __syncwarp();
         ctl->busy[warp & 3] = 0;
       }

@@ -300,7 +300,8 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: t
     if seqs < 0:
         raise ValueError("cu_seqlens needs n_seqs + 1 entries")
     out = _result(out, shape, dtype, dev, "out")
-    workspace = _scratch(workspace, _L.fuelq_prompt_attn_workspace_bytes(_TYPE_IDS[dtype], rows, heads, kv, hd) if workspace is None else 0, q)
+    workspace = _scratch(workspace, 0 if workspace is not None else
+                         _L.fuelq_prompt_attn_workspace_bytes(_TYPE_IDS[dtype], rows, heads, kv, hd), q)
     status = _L.fuelq_prompt_attn(_TYPE_IDS[dtype], q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(),
                                   cu_seqlens.data_ptr(), seqs, rows, heads, kv, hd, hd ** -0.5 if scale is None else scale,
                                   workspace.data_ptr(), workspace.nbytes, _raw_stream(dev))
