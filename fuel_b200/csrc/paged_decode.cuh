@@ -95,24 +95,6 @@ __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
   a = to_f32(reinterpret_cast<const T*>(&w)[0]), b = to_f32(reinterpret_cast<const T*>(&w)[1]);
 }
 
-// What a column of the values of keys [from, to) holds that is not finite: the sum of it, 0 if there is nothing. column: of page 0,
-// row 0. An infinite value is infinite in the result whatever its weight, but its product with a part of the weight that is negative
-// or zero is not; so a result that is not finite while the sum of its weights is is looked up again here. (Only then: an infinity in
-// the cache costs its batch time, finite ones nothing.)
-template <typename C>
-__device__ __noinline__ float sum_not_finite(const C* column, const int* pages, int from, int to, int page_shift, int n_pages,
-                                             int64_t page_stride, int row_stride) {
-  float sum = 0.f;
-#pragma unroll 4
-  for (int key = from; key < to; ++key) {
-    const int page = pages[key >> page_shift];
-    const bool is = page >= 0 && page < n_pages;
-    const float x = is ? to_f32(column[page * page_stride + (int64_t)(key & ((1 << page_shift) - 1)) * row_stride]) : 0.f;
-    if (!isfinite(x)) sum += x;
-  }
-  return sum;
-}
-
 template <typename A, typename C, int kHd_, int kNT_>
 struct DecodeCfg {
   static constexpr int kHd = kHd_, kNT = kNT_, kHeads = 8 * kNT;  // heads of an item
@@ -415,13 +397,8 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
     const bool whole = done && item_first >= x0;
     float* slot = p.slots + (int64_t)split_slot(total, blocks, blockIdx.x, item_first) * Cfg::kSlot;
     A* dst = reinterpret_cast<A*>(p.out) + ((int64_t)at.seq * p.n_heads + kvh * p.group + part * kHeads) * kHd;
-    const int64_t page_stride = (int64_t)p.n_kv * kHd << p.page_shift;
-    auto look_again = [&](int d) {  // at column d of the piece's keys
-      const int from = (int)max(x0 - item_first, (int64_t)0) * Cfg::kTile;
-      const int to = (int)min((int64_t)(at.tile + 1) * Cfg::kTile, (int64_t)at.keys);
-      return sum_not_finite(reinterpret_cast<const C*>(p.v) + ((int64_t)kvh * kHd << p.page_shift) + d,
-                            p.table + (int64_t)at.seq * p.max_pages, from, to, p.page_shift, p.n_pages, page_stride, kHd);
-    };
+    // results that are not finite while the sum of their weights is: bit 4 (nt kQ + q) + i
+    uint32_t odd = 0;
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
       float4 st[kDecodeWarps];
@@ -457,10 +434,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
         for (int i = 0; i < 4; ++i) {
           const int h = nt * 8 + 2 * tq + (i & 1), d = 16 * (warp * kQ + q) + g + 8 * (i >> 1);
           if (h < heads) {
-            if (!isfinite(r[i]) && isfinite(sum[i & 1])) {
-              const float f = look_again(d);
-              if (f != 0.f) r[i] = f;
-            }
+            if (!isfinite(r[i]) && isfinite(sum[i & 1])) odd |= 1u << (4 * (nt * kQ + q) + i);
             if (whole) dst[h * kHd + d] = from_f32<A>(r[i] * inv[i & 1]);
             else slot[h * kHd + d] = r[i];
           }
@@ -471,6 +445,34 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
         for (int j = 0; j < 2; ++j) {
           const int h = nt * 8 + 2 * tq + j;
           slot[kHeads * kHd + h] = top[j], slot[kHeads * (kHd + 1) + h] = sum[j];
+        }
+      }
+    }
+    if (__any_sync(0xffffffffu, odd != 0)) {
+      // An infinite value is infinite in the result whatever its weight, but its product with a part of the weight that is negative or
+      // zero is not. So what the piece's values hold that is not finite is summed up here, the lanes over the warp's columns, and takes
+      // the place of such a result. (An infinity in the cache costs its batch time, finite values nothing. The whole warp takes this way
+      // together, and nothing in it is a call)
+      const int from = (int)max(x0 - item_first, (int64_t)0) * Cfg::kTile;
+      const int to = (int)min((int64_t)(at.tile + 1) * Cfg::kTile, (int64_t)at.keys);
+      const int* pages = p.table + (int64_t)at.seq * p.max_pages;
+      const C* column = reinterpret_cast<const C*>(p.v) + ((int64_t)kvh * kHd << p.page_shift) + 16 * warp * kQ + lane % (16 * kQ);
+      const int64_t page_stride = (int64_t)p.n_kv * kHd << p.page_shift;
+      float found = 0.f;
+#pragma unroll 8
+      for (int key = from; key < to; ++key) {
+        const int page = pages[key >> p.page_shift];
+        const bool is = page >= 0 && page < p.n_pages;
+        const float x = is ? to_f32(column[page * page_stride + (int64_t)(key & ((1 << p.page_shift) - 1)) * kHd]) : 0.f;
+        found += isfinite(x) ? 0.f : x;
+      }
+#pragma unroll 1
+      for (int b = 0; b < 4 * kNT * kQ; ++b) {
+        const int i = b & 3, q = (b >> 2) % kQ, h = 8 * (b / (4 * kQ)) + 2 * tq + (i & 1), in_warp = 16 * q + g + 8 * (i >> 1);
+        const float f = __shfl_sync(0xffffffffu, found, in_warp);
+        if (((odd >> b) & 1) && f != 0.f) {
+          if (whole) dst[h * kHd + 16 * warp * kQ + in_warp] = from_f32<A>(f);
+          else slot[h * kHd + 16 * warp * kQ + in_warp] = f;
         }
       }
     }

@@ -161,6 +161,27 @@ def test_prompt_of_infinite_values_in_every_short_prompt(act, d):
         assert torch.equal(torch.where(out.isinf(), out.sign(), 0.0 * out), want)
 
 
+@pytest.mark.parametrize("act,cache", _PAIRS)
+def test_decode_of_nothing_but_infinite_values(act, cache):
+    """Every column of every key, in items of one block and of several; then a page of NaN."""
+    from fuel_b200 import ops
+    h, kv, d, page, lens = 8, 2, 128, 16, [5000, 1, 130, 0, 64]
+    need = [-(-n // page) for n in lens]
+    order = torch.randperm(sum(need), generator=torch.Generator().manual_seed(1)).tolist()
+    table, at = torch.full((len(lens), max(need)), -1, dtype=torch.int32), 0
+    for s, n in enumerate(need):
+        table[s, :n] = torch.tensor(order[at:at + n], dtype=torch.int32)
+        at += n
+    q, kc = _randn((len(lens), h, d), 1, act), _randn((at, kv, page, d), 2, cache)
+    vc = torch.full((at, kv, page, d), -math.inf, dtype=cache, device="cuda")
+    out = ops.paged_attn_decode(q, kc, vc, table.cuda(), _ints(lens))
+    live = [0, 1, 2, 4]
+    assert (out[live] == -math.inf).all() and not out[3].any()
+    vc[table[0, 7]] = math.nan
+    out = ops.paged_attn_decode(q, kc, vc, table.cuda(), _ints(lens))
+    assert out[0].isnan().all() and (out[live[1:]] == -math.inf).all()
+
+
 # ---- scores at the ends of their range
 
 @pytest.mark.parametrize("act", [F32, BF16, F16])
