@@ -163,8 +163,8 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) prompt_split_kernel(const
 
 constexpr int kPfaThreads = 512;
 // registers of a softmax thread, of one that holds a row of O, of the others: 128 x (2 x 120 + 192 + 80) of the launch's 512 x 128
-// (heads of 128: 8 bytes of a thread on its stack). Functions that are not inlined are called by the second kind alone: what they may
-// use is what the launch has
+// (heads of 128: 8 bytes of a thread on its stack). Nothing is called that is not inlined: a function of its own would know nothing
+// of these splits
 constexpr int kPfaSoftmaxRegs = 120, kPfaSumRegs = 192, kPfaOtherRegs = 80;
 constexpr int kPfaAhead = 4;  // key tiles that the softmax may be ahead of the sums (two, for the tensor memory), and their own
 
@@ -191,7 +191,7 @@ struct PromptF32Cfg {
 };
 
 // Whether the values that row `row0 + lane` of a sequence of `len` rows sees lie more than 2^100 apart; up: of its first row
-__device__ __noinline__ bool sees_far_apart(const float2* up, int row0, int len, int lane) {
+__device__ __forceinline__ bool sees_far_apart(const float2* up, int row0, int len, int lane) {
   float above = -INFINITY, below = INFINITY;
   for (int key = lane; key < row0; key += 32) above = fmaxf(above, up[key].y), below = fminf(below, up[key].y);
 #pragma unroll
@@ -213,7 +213,7 @@ __device__ __noinline__ bool sees_far_apart(const float2* up, int row0, int len,
 // (the queries themselves may lie under the result); k, v: of the sequence's first; row: the first's number; up: c 2^eq of the
 // lane's row
 template <int kHd>
-__device__ __noinline__ void weigh_again(const __half* q, int64_t q_stride, int64_t parts, float up, const float* k, int64_t k_stride,
+__device__ __forceinline__ void weigh_again(const __half* q, int64_t q_stride, int64_t parts, float up, const float* k, int64_t k_stride,
                                          const float* v, int64_t v_stride, int row, uint32_t which, float* dst, int64_t dst_stride,
                                          int lane) {
   constexpr int kMine = kHd / 32, kKeys = 4;
@@ -270,10 +270,9 @@ __device__ __noinline__ void weigh_again(const __half* q, int64_t q_stride, int6
 // The rows of a warp whose key tiles hold values that are not finite: adds those that each row sees, the lanes' columns side by side: the
 // first key with +inf, -inf, NaN of every column, looked for once for all rows. (A lane by itself for its row, column after column,
 // takes seconds where a long prompt's values are infinite throughout, and the block's other warps wait two.) v: the head's values of the
-// sequence's first row; marked: the marks of its tiles; row: the warp's first; dst: its result. (By value: a reference to the
-// kernel's parameters would put all of them on every thread's stack)
+// sequence's first row; marked: the marks of its tiles; row: the warp's first; dst: its result
 template <int kHd>
-__device__ __noinline__ void add_not_finite(const float* v, int64_t v_stride, const int2* marked, int row, int rows, float* dst,
+__device__ __forceinline__ void add_not_finite(const float* v, int64_t v_stride, const int2* marked, int row, int rows, float* dst,
                                             int64_t dst_stride, int lane) {
   constexpr int kMine = kHd / 32, kNone = 0x7fffffff;
   int first[3][kMine];
