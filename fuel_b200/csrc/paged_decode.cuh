@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(32 * kDecodeWarps) paged_decode_kernel(const D
         const float up = exp2f((float)(13 - e));
 #pragma unroll
         for (int i = 0; i < kPer; ++i) x[i] *= up;
-        f *= exp2f((float)(e - 13));
+        f = fminf(f * exp2f((float)(e - 13)), kMost);  // at f32's end any score but 0 takes all or nothing
       }
       const int nt = h >> 3, n = h & 7;
 #pragma unroll

@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) prompt_split_kernel(const
     }
     if (lane == 0) {
       const int64_t at = (int64_t)head * p.n_rows + row;
-      if (kind == 0) p.q_up[at] = exp2f((float)e0) * p.c;
+      if (kind == 0) p.q_up[at] = fminf(exp2f((float)e0) * p.c, 3.402823466e38f);  // at f32's end any score but 0 takes all or nothing
       else if (kind == 1) p.kv_up[at].x = exp2f((float)e0);
       else p.kv_up[at].y = (float)e0;
     }

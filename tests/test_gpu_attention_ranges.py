@@ -255,6 +255,25 @@ def test_prompt_of_factors_whose_powers_pass_f32():
     assert ((out.double() - want).norm() / want.norm()).item() <= 4.1e-6
 
 
+@pytest.mark.parametrize("act,cache", _PAIRS)
+def test_the_largest_scale(act, cache):
+    """Large queries at a scale of 2^127: the key of the largest product takes all, equal ones share, zeros are zeros."""
+    from fuel_b200 import ops
+    n, d, scale = 300, 64, 2.0 ** 127
+    q = torch.zeros(n, 1, d, dtype=act, device="cuda")
+    q[..., 0] = 2.0 ** 15
+    k, v = torch.zeros(n, 1, d, dtype=cache, device="cuda"), _randn((n, 1, d), 2, cache)
+    k[7::100, 0, 0] = 0.5
+    for last, seen in ((299, [7, 107, 207]), (6, range(7))):
+        want = v[list(seen), 0].double().mean(0)
+        tol = 2 * _HALF.get(act, 2.0 ** -17) * v.double().abs().max()
+        kc, vc, table = _pages(k, v, 16)
+        got = ops.paged_attn_decode(q[last:last + 1], kc, vc, table, _ints([last + 1]), scale=scale)
+        assert ((got[0, 0].double() - want).abs() <= tol).all(), last
+        if act == cache:
+            assert ((ops.prompt_attn(q, k, v, _ints([0, n]), scale=scale)[last, 0].double() - want).abs() <= tol).all(), last
+
+
 @pytest.mark.parametrize("act", [F32, BF16, F16])
 @pytest.mark.parametrize("d", [64, 128])
 def test_prompt_rows_with_a_score_of_infinity_are_nan(act, d):
