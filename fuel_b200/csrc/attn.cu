@@ -123,7 +123,8 @@ int32_t launch_prompt(const PromptArgs& r, cudaStream_t stream) {
   auto kernel = prompt_attn_kernel<T, kHd, kFar>;
   if (sms == 0 || !allow_smem(kernel, Cfg::kSmem, set)) return kLaunchFailure;
   PromptParams p = {};
-  p.out = r.out, p.cu = r.cu, p.n_rows = r.n_rows, p.n_items = prompt_slots(r.n_rows, r.n_seqs, kPaRows) * r.n_heads;
+  p.out = r.out, p.v = r.v, p.v_stride = r.v_stride, p.cu = r.cu, p.n_rows = r.n_rows;
+  p.n_items = prompt_slots(r.n_rows, r.n_seqs, kPaRows) * r.n_heads;
   p.n_seqs = r.n_seqs, p.n_heads = r.n_heads, p.group = r.n_heads / r.n_kv, p.c = r.c;
   CUtensorMap qmap, kmap, vmap;
   if (!make_rows_map(r.q, r.n_rows, r.n_heads, kHd, r.q_stride, kPaTile, &qmap) ||

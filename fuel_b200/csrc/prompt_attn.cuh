@@ -35,6 +35,8 @@ namespace fq {
 
 struct PromptParams {
   void* out;
+  const void* v;
+  int64_t v_stride;
   const int* cu;
   int64_t n_rows, n_items;
   int n_seqs, n_heads, group;
@@ -343,6 +345,41 @@ __device__ __forceinline__ bool get_item(ItemRing& ring, uint32_t n, PromptItem&
   if constexpr (kWarp) __syncwarp();
   if (!kWarp || (threadIdx.x & 31) == 0) mbar_arrive(&ring.empty[s]);
   return it.len >= 0;
+}
+
+// Rows of a warp (the bits of `which`) with NaN in their result beside a finite sum of weights: an infinite value whose weight has rounded to
+// zero. Each column becomes what it holds that is not finite, the lanes over the columns: the first key with +inf, -inf, NaN of
+// every column, looked for once for all rows. v: the head's values of the sequence's first row; row: the warp's first; dst: its result
+template <typename T, int kHd>
+__device__ __forceinline__ void put_not_finite(const T* v, int64_t v_stride, int row, uint32_t which, T* dst, int64_t dst_stride, int lane) {
+  constexpr int kMine = kHd / 32, kNone = 0x7fffffff;
+  int first[3][kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) first[0][i] = first[1][i] = first[2][i] = kNone;
+  const int last = row + 31 - __clz(which);  // of the rows in question
+  for (int key0 = 0; key0 <= last; key0 += 8) {
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int key = min(key0 + n, last);
+        const float f = to_f32(v[key * v_stride + lane + 32 * i]);
+        first[0][i] = f == INFINITY ? min(first[0][i], key) : first[0][i];
+        first[1][i] = f == -INFINITY ? min(first[1][i], key) : first[1][i];
+        first[2][i] = f != f ? min(first[2][i], key) : first[2][i];
+      }
+  }
+  for (; which; which &= which - 1) {
+    const int r = __ffs(which) - 1;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      float sum = 0.f;
+      if (first[0][i] <= row + r) sum += INFINITY;
+      if (first[1][i] <= row + r) sum -= INFINITY;
+      if (first[2][i] <= row + r) sum += __int_as_float(0x7fc00000);
+      if (sum != 0.f) dst[r * dst_stride + lane + 32 * i] = from_f32<T>(sum);
+    }
+  }
 }
 
 template <int kHd, int kStages>
@@ -703,11 +740,14 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
         const int row0 = row - lane;  // of the warp
         uint8_t* dst = reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(p.out) + ((it.first + row0) * p.n_heads + it.head) * kHd);
         const int64_t row_bytes = (int64_t)p.n_heads * kHd * sizeof(T);
+        float most = 0.f;  // NaN if one of the row's sums is
 #pragma unroll 1
         for (int i = 0; i < kHd / 32; ++i) {
           uint32_t o[32];
           tmem_ld32_nowait(o_addr + 32 * i, o);
           tmem_wait_ld(o);
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) most = max3_nan(most, __uint_as_float(o[e]), __uint_as_float(o[e + 1]));
           if (rec0 || rec1) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
@@ -729,6 +769,12 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
 #pragma unroll
           for (int e = 0; e < 16; ++e) w[e] = cvt2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
           store_rows64(smem_u32(stages) + warp * kStageBytes, lane, v, dst + 64 * i, row_bytes, it.len - row0);
+        }
+        const uint32_t odd = __ballot_sync(0xffffffffu, most != most && total == total && row < it.len);
+        if (odd) {
+          __syncwarp();  // the rows are written
+          put_not_finite<T, kHd>(reinterpret_cast<const T*>(p.v) + it.first * p.v_stride + it.head / p.group * kHd, p.v_stride, row0,
+                                 odd, reinterpret_cast<T*>(dst), (int64_t)p.n_heads * kHd, lane);
         }
         tc_fence_before();
         mbar_arrive(&ctl->taken_free[t]);

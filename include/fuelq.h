@@ -451,9 +451,8 @@ int32_t fuelq_paged_attn_decode(int32_t act_type, int32_t cache_type, const void
  * sequence s, and each of its rows attends to the sequence's rows up to itself; n_rows (below 2^30 - 255) is the number of rows
  * the buffers have, n_seqs * n_heads at most 2^26. Rows of out behind the last sequence are left as they were. Nothing that
  * stands behind a row in its sequence, in another sequence or behind the last one reaches it, infinities and NaN included. An
- * infinite value makes its column of the rows that see it infinite, infinities of both signs make it NaN (16-bit types: so does
- * one infinity whose weight rounds to zero: below 2^-32 of the row's largest in f16, 2^-100 in bf16). 32-bit activations are
- * multiplied to 32-bit accuracy (error against 64 bits 5e-7 of the result at 512 tokens), 16-bit ones as they are, the
+ * infinite value makes its column of the rows that see it infinite, infinities of both signs make it NaN. 32-bit activations
+ * are multiplied to 32-bit accuracy (error against 64 bits 5e-7 of the result at 512 tokens), 16-bit ones as they are, the
  * softmax's weights rounded once to their type. 32-bit rows with scores beyond 2^22, or values more than 2^100 apart, are right
  * but slow: a hundred times and more. 32-bit calls need a workspace (as much as q, k and v themselves and a little); calls that
  * may run at the same time need one each. */

@@ -139,6 +139,24 @@ def test_decode_of_infinite_values(act, cache, d, bad):
 
 @pytest.mark.parametrize("act", [F32, F16, BF16])
 @pytest.mark.parametrize("d", [64, 128])
+def test_prompt_of_infinite_values_of_hardly_any_weight(act, d):
+    """Beside a key of e^100 times their weight: the weights round to zero, the infinities are there all the same, and nowhere else."""
+    from fuel_b200 import ops
+    n, h = 700, 3
+    q, k, v = _randn((n, h, d), 1, act, 0.3), _randn((n, 1, d), 2, act), _randn((n, 1, d), 3, act)
+    q[..., 0], k[..., 0], k[0] = 16.0, 0.0, 0.0
+    k[0, 0, 0] = 100.0 / (16.0 * d ** -0.5)
+    good = ops.prompt_attn(q, k, v, _ints([0, n]))
+    b = v.clone()
+    b[50, 0, 7], b[50, 0, 9], b[300, 0, 9], b[140, 0, 11], b[699, 0, 13] = math.inf, -math.inf, math.inf, math.nan, math.inf
+    out = ops.prompt_attn(q, k, b, _ints([0, n]))
+    want = good.clone()
+    want[50:, :, 7], want[50:, :, 9], want[300:, :, 9], want[140:, :, 11], want[699:, :, 13] = math.inf, -math.inf, math.nan, math.nan, math.inf
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(nan=7.0), want.nan_to_num(nan=7.0))
+
+
+@pytest.mark.parametrize("act", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
 def test_prompt_of_infinite_values_in_every_short_prompt(act, d):
     """Each thread block takes many items one after the other, nearly all of them with an infinity in their last key tile: what is
     noted of one is not lost to the next."""
