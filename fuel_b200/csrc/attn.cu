@@ -28,7 +28,7 @@ inline bool stride_ok(int64_t stride, int heads, int head_dim, int act) {
   return stride >= (int64_t)heads * head_dim && stride * type_bytes(act) % 16 == 0;
 }
 // the kernels take scale log2(e), which has to be a number too
-inline bool scale_ok(float scale) { return scale > 0.f && scale <= 0x1p127f; }
+inline bool scale_ok(float scale) { return scale >= 0x1p-100f && scale <= 0x1p127f; }
 constexpr int64_t kMaxRows = 0x7fffffff, kMaxPromptRows = (1 << 30) - 256;  // prompts: twice as many are a coordinate of a copy
 constexpr int64_t kMaxSlots = 1 << 26;  // empty sequences times heads, which a warp looks through while the others' waits run
 constexpr int kMaxHeads = 16383;  // q, k and v heads together are a grid dimension
@@ -115,12 +115,12 @@ struct PromptArgs {
   float c;
   uint8_t* workspace;
 };
-template <typename T, int kHd, bool kFar>
+template <typename T, int kHd>
 int32_t launch_prompt(const PromptArgs& r, cudaStream_t stream) {
   using Cfg = PromptCfg<T, kHd>;
   static bool set[64] = {};
   const int sms = sm_count();
-  auto kernel = prompt_attn_kernel<T, kHd, kFar>;
+  auto kernel = prompt_attn_kernel<T, kHd>;
   if (sms == 0 || !allow_smem(kernel, Cfg::kSmem, set)) return kLaunchFailure;
   PromptParams p = {};
   p.out = r.out, p.v = r.v, p.v_stride = r.v_stride, p.cu = r.cu, p.n_rows = r.n_rows;
@@ -133,12 +133,6 @@ int32_t launch_prompt(const PromptArgs& r, cudaStream_t stream) {
     return kLaunchFailure;
   const dim3 grid((unsigned)(p.n_items < sms ? p.n_items : sms));
   return launch(kernel, grid, dim3(kPaThreads), Cfg::kSmem, stream, p, qmap, kmap, vmap) == cudaSuccess ? kOk : kLaunchFailure;
-}
-
-template <typename T>
-int32_t launch_prompt(const PromptArgs& r, int head_dim, cudaStream_t stream) {
-  if (prompt_far<T>(r.c)) return head_dim == 128 ? launch_prompt<T, 128, true>(r, stream) : launch_prompt<T, 64, true>(r, stream);
-  return head_dim == 128 ? launch_prompt<T, 128, false>(r, stream) : launch_prompt<T, 64, false>(r, stream);
 }
 
 // Workspace of the 32-bit form: the parts and powers of q, k and v; where each begins, and the whole
@@ -316,8 +310,8 @@ int32_t fuelq_prompt_attn(int32_t act_type, const void* q, int64_t q_stride, con
   a.n_rows = n_rows, a.n_seqs = n_seqs, a.n_heads = n_heads, a.n_kv = n_kv, a.c = scale * 1.4426950408889634f;
   a.workspace = (uint8_t*)workspace;
   cudaStream_t st = (cudaStream_t)stream;
-  if (act_type == kF16) return launch_prompt<__half>(a, head_dim, st);
-  if (act_type == kBF16) return launch_prompt<__nv_bfloat16>(a, head_dim, st);
+  if (act_type == kF16) return head_dim == 128 ? launch_prompt<__half, 128>(a, st) : launch_prompt<__half, 64>(a, st);
+  if (act_type == kBF16) return head_dim == 128 ? launch_prompt<__nv_bfloat16, 128>(a, st) : launch_prompt<__nv_bfloat16, 64>(a, st);
   return head_dim == 128 ? launch_prompt_f32<128>(a, st) : launch_prompt_f32<64>(a, st);
 }
 

@@ -44,7 +44,7 @@ struct PromptParams {
 };
 constexpr int kPaThreads = 384, kPaTile = 128, kPaRows = 2 * kPaTile;
 // registers of a softmax thread (its row of S is 128 of them) and of the others: 256 x 208 + 128 x 80 of the launch's 384 x 168. (The
-// form for heads of 64 keeps 56 to 64 bytes of a thread on its stack all the same, that for 128 nothing)
+// form for heads of 64 keeps 64 bytes of a thread on its stack all the same, that for 128 nothing)
 constexpr int kPaSoftmaxRegs = 208, kPaOtherRegs = 80;
 
 // ---- PTX wrappers
@@ -396,11 +396,17 @@ struct PromptCtl {
 // key tiles of the second 128 rows of a block, 0 if it has none
 __device__ __forceinline__ int second_tiles(const PromptItem& it) { return it.row + kPaTile < it.len ? it.n + 1 : 0; }
 
-// Whether s c may be infinite for a finite s: f16 products of 128 terms stay below 2^40, bf16 ones reach f32's ends. Looking for it
-// takes 4 % at head_dim 128, 10 % at 64 (bf16, scale 1: 24 prompts up to 2048 377 us, without 364; 8192 tokens 553, 501), so that
-// other scales go without.
-template <typename T>
-inline bool prompt_far(float c) { return c > (std::is_same<T, __half>::value ? 0x1p88f : 1.f); }
+// The factor that a row's scores are multiplied by, c, and the reference's product with it, mc. s c - mc is off by what mc is rounded by, for
+// all scores alike, which is nothing while mc is small; from 2^24 on, where scores differ by an exponent or not at all, and where ref c
+// leaves f32, the factor is a power of two, whose product is not rounded: the nearest to c that keeps ref's in range
+__device__ __forceinline__ void scale_row(float ref, float c, float& row_c, float& mc) {
+  row_c = c, mc = ref == -INFINITY ? 0.f : ref * c;
+  if (fabsf(ref) < INFINITY && !(fabsf(mc) <= 0x1p24f)) {
+    const uint32_t exponent = (__float_as_uint(ref) >> 23) & 255u, room = min(380u - exponent, 254u);  // ref 2^k below 2^127
+    row_c = fminf(__uint_as_float(__float_as_uint(c * 1.41421356f) & 0x7f800000u), __uint_as_float(room << 23));
+    mc = ref * row_c;
+  }
+}
 
 template <typename T, int kHd>
 struct PromptCfg {
@@ -413,9 +419,7 @@ struct PromptCfg {
   static constexpr int kSmem = 1024 + (2 + kStages) * kTileBytes + 8 * kStageBytes + (int)sizeof(PromptCtl<kHd, kStages>) + 16;
 };
 
-// kFar: for scales with which finite scores may pass f32's range once they are multiplied by c (see prompt_far): a row whose
-// reference comes near it has its weights from (s - ref) c in the place of s c - ref c
-template <typename T, int kHd, bool kFar>
+template <typename T, int kHd>
 __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap,
                                                                     const __grid_constant__ CUtensorMap kmap,
                                                                     const __grid_constant__ CUtensorMap vmap) {
@@ -580,7 +584,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
     PromptItem it;
     for (; ok && get_item<true>(ctl->items, done, it, wait);) {
       const int n1 = second_tiles(it), n = n1 ? n1 : it.n, mine = t ? n1 : it.n;
-      float ref = -INFINITY, mc = 0.f;  // the reference; c times it
+      float ref = -INFINITY, mc = 0.f, row_c = p.c;  // the reference; c times it; c
       uint64_t sum2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
       for (int j = 0; j < mine && ok; ++j) {
         if (!(ok = __all_sync(0xffffffffu, wait(&ctl->s_full[t], steps++, kErrMmaWait)))) break;
@@ -591,21 +595,20 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
         // summed
         constexpr float kUp = std::is_same<T, __half>::value ? 7.f : -24.f;
         uint64_t c2, m2;
-        bool far = false;
         // the row's reference, once its maximum is in top[]
         auto refer = [&]() {
           float most = max3_nan(top[0], top[1], max3_nan(top[2], top[3], top[3]));
           if (most == INFINITY) most = __int_as_float(0x7fc00000);  // inf - inf is in this row's softmax
           if (j == 0) {
             ref = most;
-            mc = ref == -INFINITY ? 0.f : ref * p.c;
+            scale_row(ref, p.c, row_c, mc);
           } else {
             const bool move = !((most - ref) * p.c <= 8.f);
             if (__any_sync(0xffffffffu, move)) {  // O is complete up to the tile before: S of this one came after it
               // each row by its own scores alone: its bits do not depend on what else is in the warp
               const float keep = move && most != ref ? exp2_approx((ref - most) * p.c) : 1.f;  // both -inf: nothing of weight yet
               if (move) ref = most;
-              mc = ref == -INFINITY ? 0.f : ref * p.c;
+              scale_row(ref, p.c, row_c, mc);
 #pragma unroll 1
               for (int i = 0; i < kHd / 16; ++i) {
                 uint32_t o[16];
@@ -622,14 +625,11 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
               }
             }
           }
-          if constexpr (kFar) far = fabsf(ref) < INFINITY && !(fabsf(mc) <= 0x1p126f);
-          const float m = kUp - (far ? 0.f : mc);
-          c2 = pair(p.c, p.c), m2 = pair(m, m);
+          c2 = pair(row_c, row_c), m2 = pair(kUp - mc, kUp - mc);
         };
         auto weight2 = [&](int i, uint32_t s0, uint32_t s1) {  // of pair i of the tile
-          float a = __uint_as_float(s0), b = __uint_as_float(s1);
-          if (kFar && far) a -= ref, b -= ref;
-          const uint64_t x = fma2(pair(a, b), c2, m2);
+          float a, b;
+          const uint64_t x = fma2(pair(__uint_as_float(s0), __uint_as_float(s1)), c2, m2);
           if (i % Cfg::kPolyEvery == Cfg::kPolyEvery - 1) {
             exp2_poly2(x, a, b);
           } else {

@@ -409,9 +409,9 @@ int32_t fuelq_argmax_last(const float* x, int64_t n, int32_t* out_index, void* s
  * with the maximum taken off, f32 sums.
  * Types: act_type is the type of q, k, v and the outputs, cache_type that of the pages: F32, F16 or BF16. f32 activations go
  * with every cache type, 16-bit ones with a cache of their own type. head_dim is 64 or 128, n_heads a multiple of n_kv (query
- * head h reads kv head h / (n_heads / n_kv)); scale is positive and at most 2^127.
+ * head h reads kv head h / (n_heads / n_kv)); scale is between 2^-100 and 2^127.
  * Scores: a score of -inf is a weight of zero, and a row with no other scores gives zeros; one of +inf or NaN makes its row NaN.
- * Finite products of q and k stay finite when they are scaled. With 32-bit activations the score of an infinity in q or k may be
+ * Finite products of q and k stay finite when they are scaled (fuelq_paged_attn_decode: they end at f32's largest number). With 32-bit activations the score of an infinity in q or k may be
  * NaN where the infinity itself would be expected.
  * Rows: q, k and v are [rows][heads][head_dim], the heads of a row contiguous, rows q_stride / k_stride / v_stride elements
  * apart, so that they may be column ranges of a stacked projection; outputs are contiguous. All base addresses and row
@@ -453,7 +453,7 @@ int32_t fuelq_paged_attn_decode(int32_t act_type, int32_t cache_type, const void
  * stands behind a row in its sequence, in another sequence or behind the last one reaches it, infinities and NaN included. An
  * infinite value makes its column of the rows that see it infinite, infinities of both signs make it NaN. 32-bit activations
  * are multiplied to 32-bit accuracy (error against 64 bits 5e-7 of the result at 512 tokens), 16-bit ones as they are, the
- * softmax's weights rounded once to their type. 32-bit rows with scores beyond 2^22, or values more than 2^100 apart, are right
+ * softmax's weights rounded once to their type (f16: in steps of 2^-31 of the row's largest or finer). 32-bit rows with scores beyond 2^22, or values more than 2^100 apart, are right
  * but slow: a hundred times and more. 32-bit calls need a workspace (as much as q, k and v themselves and a little); calls that
  * may run at the same time need one each. */
 size_t fuelq_prompt_attn_workspace_bytes(int32_t act_type, int64_t n_rows, int32_t n_heads, int32_t n_kv, int32_t head_dim);

@@ -1,4 +1,4 @@
-"""The largest scales that the attention entries take, before anything is launched: no GPU needed."""
+"""The largest and least scales that the attention entries take, before anything is launched: no GPU needed."""
 import pytest
 
 from fuel_b200 import _lib as L
@@ -21,4 +21,13 @@ def test_scales_that_pass_f32_with_log2_e(call, act):
     """Scores are powers of two on the way, scale * log2(e) of them: an infinite factor would make NaN of a score of zero."""
     assert call(act, 2.0 ** 127, 0) == L.OK
     for scale in (1.001 * 2.0 ** 127, 2.4e38, 3.4e38):
+        assert call(act, scale, 0) == L.INVALID_PROBLEM and call(act, scale, 4) == L.INVALID_PROBLEM
+
+
+@pytest.mark.parametrize("call", [decode, prompt])
+@pytest.mark.parametrize("act", [F32, F16, BF16])
+def test_scales_that_leave_a_factor_no_bits(call, act):
+    """Below 2^-100 the product with a row's power of two would lose its bits before the keys' powers bring it back."""
+    assert call(act, 2.0 ** -100, 0) == L.OK
+    for scale in (0.99 * 2.0 ** -100, 2.0 ** -126, 1e-44):
         assert call(act, scale, 0) == L.INVALID_PROBLEM and call(act, scale, 4) == L.INVALID_PROBLEM

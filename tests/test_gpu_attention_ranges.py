@@ -260,6 +260,34 @@ def test_prompt_of_large_scores_alike(d, size):
     assert torch.equal(ops.prompt_attn(q, k, v, _ints([0, n]), out=q), out) and torch.equal(q, out)
 
 
+@pytest.mark.parametrize("act,size", [(F16, 300.0), (F16, 5000.0), (F16, 30000.0), (BF16, 1e6), (BF16, 1e15)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_of_large_queries_and_keys(act, size, d):
+    """Scores far above what an exponent holds: the key with the largest takes all, wherever it is clear of the next. Rows beside such
+    rows keep their bits."""
+    from fuel_b200 import ops
+    n = 600
+    q, k, v = _randn((n, 2, d), 1, act), _randn((n, 1, d), 2, act), _randn((n, 1, d), 3, act)
+    size = min(size, torch.finfo(act).max / 5.0)       # five deviations
+    large_q, large_k = (q.float() * size).to(act), (k.float() * size).to(act)
+    out = ops.prompt_attn(large_q, large_k, v, _ints([0, n]))
+    s = torch.einsum("ihd,jhd->hij", large_q.double(), large_k.double().expand(n, 2, d)) * d ** -0.5
+    s = s.masked_fill(torch.arange(n, device="cuda")[None, :] > torch.arange(n, device="cuda")[:, None], -math.inf)
+    two = s.topk(2, -1)
+    clear = two.values[..., 0] - two.values[..., 1] > 40.0 + 2.0 ** -16 * s.abs().nan_to_num(posinf=0.0).amax(-1)
+    clear[:, 0] = True
+    assert clear.sum() > 0.8 * clear.numel()
+    want = v[two.indices[..., 0], 0].transpose(0, 1)
+    # one weight rounded to the type beside its sum that is not, and the result: two half steps; f16 steps are 2^-24 at least
+    tol = 2.02 * _HALF[act] * want.double().abs() + (2.0 ** -25 if act == F16 else 0.0)
+    assert ((out.double() - want.double()).abs() <= tol)[clear.T].all()
+    good, mixed = ops.prompt_attn(q, k, v, _ints([0, n])), q.clone()
+    mixed[::3] = large_q[::3]
+    out = ops.prompt_attn(mixed, k, v, _ints([0, n]))
+    keep = [i for i in range(n) if i % 3]
+    assert torch.equal(out[keep], good[keep])
+
+
 def test_prompt_of_factors_whose_powers_pass_f32():
     """Large columns of q meet columns of zero in k and the other way round: the scores are of a few units."""
     from fuel_b200 import ops
