@@ -25,8 +25,8 @@
 //   warps 12, 15    copies: the parts of Q and K, of V
 //   warp 13         issues the MMAs
 //   warp 14         finds the block's items and brings the powers of each key tile
-// Measured, 32/8 heads of 128: 512 tokens 35.5 us (the split some 8 of them), 4096 tokens 528 us: 260 TFLOP/s of the scores that are
-// seen, 780 of f16 products; heads of 64 410 us. An issuing warp that waits for ten units and flags a key tile bounds it now, some 300
+// Measured, 32/8 heads of 128: 512 tokens 34.7 us (the split some 8 of them), 4096 tokens 525 us: 262 TFLOP/s of the scores that are
+// seen, 786 of f16 products; heads of 64 410 us. An issuing warp that waits for ten units and flags a key tile bounds it now, some 300
 // cycles each. Of 4096 rows of four heads, 125 us, one infinite column of the values makes 0.37 ms, scores beyond 2^22 in every row 21 ms.
 #pragma once
 #include "prompt_attn.cuh"
@@ -605,6 +605,20 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
     bool ok = true;
     PromptItem it;
     for (uint32_t items = 0; ok && get_item<true>(ctl->items, items, it, wait); ++items) {
+      const int row = it.row + r, row0 = row - lane;  // row0: of the warp
+      const int64_t rows_at = (int64_t)(it.head / p.group) * p.n_rows + it.first;
+      // the marks of its key tiles, read while the first of them is computed
+      bool odd = false;
+      int up = -1000, above = 0, below = 255;
+      for (int j = lane; j < it.n; j += 32) {
+        const int2 mark = p.marked[rows_at + (int64_t)j * kPaTile];
+        odd |= mark.x & 1, up = max(up, mark.y);
+        above = max(above, mark.x >> 8 & 255), below = min(below, mark.x >> 16);
+      }
+      const float q_up = row < it.len ? p.q_up[(int64_t)it.head * p.n_rows + it.first + row] : 0.f;
+      odd = __any_sync(0xffffffffu, odd);
+      const float reach = q_up * exp2f((float)__reduce_max_sync(0xffffffffu, up));
+      const bool apart = __reduce_max_sync(0xffffffffu, above) - __reduce_min_sync(0xffffffffu, below) > 100;
       float o[kHd], ref = -INFINITY, sum = 0.f;
 #pragma unroll
       for (int e = 0; e < kHd; ++e) o[e] = 0.f;
@@ -626,27 +640,12 @@ __global__ void __launch_bounds__(kPfaThreads, 1) prompt_attn_f32_kernel(const P
         mbar_arrive(&ctl->pv_empty);
       }
       if (!ok) break;
-      const int row = it.row + r;
-      const int row0 = row - lane;  // of the warp
-      const int64_t rows_at = (int64_t)(it.head / p.group) * p.n_rows + it.first;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      bool odd = false;
-      int up = -1000, above = 0, below = 255;
-      for (int j = lane; j < it.n; j += 32) {
-        const int2 mark = p.marked[rows_at + (int64_t)j * kPaTile];
-        odd |= mark.x & 1, up = max(up, mark.y);
-        above = max(above, mark.x >> 8 & 255), below = min(below, mark.x >> 16);
-      }
-      odd = __any_sync(0xffffffffu, odd);
-      up = __reduce_max_sync(0xffffffffu, up);
       // rows to be computed again: their maximum is beyond 2^22 or has left f32, where the powers of their factors allow it (a product of
       // two parts is below 2^37; otherwise an infinity in q or k has made it); the powers' product may leave f32 where the score
       // itself is of any size; the values lie too far apart
-      const float q_up = row < it.len ? p.q_up[(int64_t)it.head * p.n_rows + it.first + row] : 0.f;
-      const float reach = q_up * exp2f((float)up);
       bool far = (reach > 0x1p-15f && !(fabsf(ref) <= 0x1p22f)) || !(reach <= 0x1p120f);
-      if (__reduce_max_sync(0xffffffffu, above) - __reduce_min_sync(0xffffffffu, below) > 100)
-        far |= sees_far_apart(p.kv_up + rows_at, row0, it.len, lane);
+      if (apart) far |= sees_far_apart(p.kv_up + rows_at, row0, it.len, lane);
       const uint32_t again = __ballot_sync(0xffffffffu, far && row < it.len);
       float* dst = p.out + ((it.first + row0) * p.n_heads + it.head) * kHd;
 #pragma unroll

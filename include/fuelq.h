@@ -411,8 +411,8 @@ int32_t fuelq_argmax_last(const float* x, int64_t n, int32_t* out_index, void* s
  * with every cache type, 16-bit ones with a cache of their own type. head_dim is 64 or 128, n_heads a multiple of n_kv (query
  * head h reads kv head h / (n_heads / n_kv)); scale is between 2^-100 and 2^127.
  * Scores: a score of -inf is a weight of zero, and a row with no other scores gives zeros; one of +inf or NaN makes its row NaN.
- * Finite products of q and k stay finite when they are scaled (fuelq_paged_attn_decode: they end at f32's largest number). With 32-bit activations the score of an infinity in q or k may be
- * NaN where the infinity itself would be expected.
+ * Finite products of q and k stay finite when they are scaled (fuelq_paged_attn_decode: they end at f32's largest number). With
+ * 32-bit activations the score of an infinity in q or k may be NaN where the infinity itself would be expected.
  * Rows: q, k and v are [rows][heads][head_dim], the heads of a row contiguous, rows q_stride / k_stride / v_stride elements
  * apart, so that they may be column ranges of a stacked projection; outputs are contiguous. All base addresses and row
  * strides are multiples of 16 bytes.
