@@ -44,7 +44,7 @@ struct PromptParams {
 };
 constexpr int kPaThreads = 384, kPaTile = 128, kPaRows = 2 * kPaTile;
 // registers of a softmax thread (its row of S is 128 of them) and of the others: 256 x 208 + 128 x 80 of the launch's 384 x 168. (The
-// form for heads of 64 keeps 64 bytes of a thread on its stack all the same, that for 128 nothing)
+// form for heads of 64 keeps 48 bytes of a thread on its stack all the same, that for 128 nothing)
 constexpr int kPaSoftmaxRegs = 208, kPaOtherRegs = 80;
 
 // ---- PTX wrappers
@@ -396,16 +396,22 @@ struct PromptCtl {
 // key tiles of the second 128 rows of a block, 0 if it has none
 __device__ __forceinline__ int second_tiles(const PromptItem& it) { return it.row + kPaTile < it.len ? it.n + 1 : 0; }
 
-// The factor that a row's scores are multiplied by, c, and the reference's product with it, mc. s c - mc is off by what mc is rounded by, for
-// all scores alike, which is nothing while mc is small; from 2^24 on, where scores differ by an exponent or not at all, and where ref c
-// leaves f32, the factor is a power of two, whose product is not rounded: the nearest to c that keeps ref's in range
-__device__ __forceinline__ void scale_row(float ref, float c, float& row_c, float& mc) {
-  row_c = c, mc = ref == -INFINITY ? 0.f : ref * c;
-  if (fabsf(ref) < INFINITY && !(fabsf(mc) <= 0x1p24f)) {
+// What a row's scores are multiplied by, c, and what is added, `up` - ref c (up: see PromptCfg). The sum is rounded, and its error is in all
+// of the row's weights alike: nothing while it is small. f16 has room for weights that are smaller, not larger: one more is taken off
+// where the error is above a half. From 2^28 on (bf16: 2^30), where the weights of scores that differ are 2^-16 of one another or
+// less, and where ref c leaves f32, the factor is a power of two, whose product is not rounded: the nearest to c that keeps ref's in range
+template <typename T>
+__device__ __forceinline__ void scale_row(float ref, float c, float up, float& row_c, float& add) {
+  constexpr bool kF16 = std::is_same<T, __half>::value;
+  row_c = c;
+  float product = ref == -INFINITY ? 0.f : ref * c;
+  if (fabsf(ref) < INFINITY && !(fabsf(product) <= (kF16 ? 0x1p28f : 0x1p30f))) {
     const uint32_t exponent = (__float_as_uint(ref) >> 23) & 255u, room = min(380u - exponent, 254u);  // ref 2^k below 2^127
     row_c = fminf(__uint_as_float(__float_as_uint(c * 1.41421356f) & 0x7f800000u), __uint_as_float(room << 23));
-    mc = ref * row_c;
+    product = ref * row_c;
   }
+  add = up - product;
+  if (kF16 && fmaf(ref, row_c, add) > up + 0.5f) add = __int_as_float(__float_as_int(add) + (add > 0.f ? -1 : 1));
 }
 
 template <typename T, int kHd>
@@ -415,6 +421,9 @@ struct PromptCfg {
   // 24 prompts up to 2048, head_dim 128: none 374, one in eight 335, six 340, five 341 us; one prompt of 256: 13.5, 11.8, 11.8, 11.8.
   // 8192 tokens, head_dim 64, where half the products meet as many exponentials: none 484, one in six 501, five 465, four 483 us
   static constexpr int kPolyEvery = kHd == 128 ? 6 : 4;
+  // f16 ends at 2^-24: its weights are 2^7 times larger, up to 2^15; bf16's 2^24 times smaller, so that values at f32's ends can be
+  // summed
+  static constexpr float kUp = std::is_same<T, __half>::value ? 7.f : -24.f;
   static constexpr int kTileBytes = kPaTile * kHd * 2;
   static constexpr int kSmem = 1024 + (2 + kStages) * kTileBytes + 8 * kStageBytes + (int)sizeof(PromptCtl<kHd, kStages>) + 16;
 };
@@ -584,16 +593,13 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
     PromptItem it;
     for (; ok && get_item<true>(ctl->items, done, it, wait);) {
       const int n1 = second_tiles(it), n = n1 ? n1 : it.n, mine = t ? n1 : it.n;
-      float ref = -INFINITY, mc = 0.f, row_c = p.c;  // the reference; c times it; c
+      float ref = -INFINITY, row_c = p.c, add = 0.f;  // the reference; what scores are multiplied by; what is added then
       uint64_t sum2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
       for (int j = 0; j < mine && ok; ++j) {
         if (!(ok = __all_sync(0xffffffffu, wait(&ctl->s_full[t], steps++, kErrMmaWait)))) break;
         tc_fence_after();
         const bool last = j + 1 == mine;
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // NaN where a visible score is: then the whole row is
-        // f16 ends at 2^-24: its weights are 2^7 times larger, up to 2^15; bf16's 2^24 times smaller, so that values at f32's ends can be
-        // summed
-        constexpr float kUp = std::is_same<T, __half>::value ? 7.f : -24.f;
         uint64_t c2, m2;
         // the row's reference, once its maximum is in top[]
         auto refer = [&]() {
@@ -601,14 +607,19 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
           if (most == INFINITY) most = __int_as_float(0x7fc00000);  // inf - inf is in this row's softmax
           if (j == 0) {
             ref = most;
-            scale_row(ref, p.c, row_c, mc);
+            scale_row<T>(ref, p.c, Cfg::kUp, row_c, add);
           } else {
-            const bool move = !((most - ref) * p.c <= 8.f);
+            const bool move = !((most - ref) * row_c <= 8.f);
             if (__any_sync(0xffffffffu, move)) {  // O is complete up to the tile before: S of this one came after it
               // each row by its own scores alone: its bits do not depend on what else is in the warp
-              const float keep = move && most != ref ? exp2_approx((ref - most) * p.c) : 1.f;  // both -inf: nothing of weight yet
-              if (move) ref = most;
-              scale_row(ref, p.c, row_c, mc);
+              float keep = 1.f;
+              if (move && most != ref) {  // (equal: both -inf, nothing of weight yet)
+                const float before = ref, c0 = row_c, add0 = add;
+                ref = most;
+                scale_row<T>(ref, p.c, Cfg::kUp, row_c, add);
+                keep = before == -INFINITY ? 0.f : exp2_approx(row_c == c0 ? add - add0 : (before - most) * p.c);
+                if (most != most) keep = most;
+              }
 #pragma unroll 1
               for (int i = 0; i < kHd / 16; ++i) {
                 uint32_t o[16];
@@ -625,7 +636,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_attn_kernel(const Prompt
               }
             }
           }
-          c2 = pair(row_c, row_c), m2 = pair(kUp - mc, kUp - mc);
+          c2 = pair(row_c, row_c), m2 = pair(add, add);
         };
         auto weight2 = [&](int i, uint32_t s0, uint32_t s1) {  // of pair i of the tile
           float a, b;

@@ -288,6 +288,29 @@ def test_prompt_of_large_queries_and_keys(act, size, d):
     assert torch.equal(out[keep], good[keep])
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("act", [F16, BF16])
+@pytest.mark.parametrize("large", [2.0 ** 8, 2.0 ** 11, 2.0 ** 13, 2.0 ** 14, 2.0 ** 15])
+def test_prompt_of_close_scores_far_from_zero(act, large, d):
+    """Scores of up to 2^30, exact in f32, that lie a few units apart and rise from key tile to key tile: their weights are those of the
+    distances, at either sign."""
+    from fuel_b200 import ops
+    n, scale = 500, 0.125
+    step = max(1.0, large * large * 2.0 ** -23)         # the least that f32 tells apart there
+    q, k = (torch.zeros(n, 1, d, dtype=act, device="cuda") for _ in range(2))
+    v = _randn((n, 1, d), 3, act)
+    rise = torch.randint(0, 6, (n,), generator=torch.Generator().manual_seed(1)) + 3 * (torch.arange(n) // 100)
+    q[..., 0], q[..., 1], k[..., 0], k[:, 0, 1] = large, step, large, rise.cuda().to(act)
+    for sign in (1.0, -1.0):
+        k[..., 0] = sign * large
+        out = ops.prompt_attn(q, k, v, _ints([0, n]), scale=scale)
+        for row in (0, 1, 99, 127, 128, 200, 301, 499):
+            want, mag = _attend(q[row].double(), k[:row + 1, 0].double(), v[:row + 1, 0].double(), scale)
+            off = (out[row].double() - want).abs()
+            # differences of up to 20 steps, exact but for the factor's 24 bits: the weights' rounding and the result's
+            assert (off <= _HALF[act] * (want.abs() + mag) + 2.0 ** -15 * mag).all(), (sign, row)
+
+
 def test_prompt_of_factors_whose_powers_pass_f32():
     """Large columns of q meet columns of zero in k and the other way round: the scores are of a few units."""
     from fuel_b200 import ops
